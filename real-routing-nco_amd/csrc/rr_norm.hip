@@ -1,0 +1,338 @@
+// h = x + r,  y = h * rsqrt(mean(h^2) + eps) * w  over the last axis: the residual's addition and the root-mean-square norm
+// in one pass (RMSNorm rrnco/models/nn/attn_freenet.py:13-26 behind the skip connection), its gradient, and a form
+// that hands y on in 8 bits with a scale for every 128 columns.
+//
+//   forward    s = rsqrt(mean h^2 + eps); the norm is taken of the 32-bit sum, h and y are rounded once each when stored
+//   backward   g = dy w, n = h s:   dx = dr = dh + s (g - n mean(g n)),   dw = sum over the rows of dy n
+//   8 bits     a = max |y| over a group of 128 columns, scale = a / 448 (1 for a group of zeros), q = e4m3(y / scale)
+//
+// Bound by memory: each tensor is read and written once, a row's elements stay in registers between the two uses.
+// A team of TPR lanes owns a row (TPR 16 .. 1024, chosen so that a lane holds 16 bytes up to a width of 64 such pieces and at
+// most 64 bytes beyond), so that narrow rows share a wave and the sum of squares is a few lane exchanges.
+// dw: each workgroup sums its rows in registers, the teams are joined through LDS in a fixed order and one partial row per
+// workgroup is written; a second launch adds the partials in order (no atomics: the same result every time).
+#include "rr_types.h"
+
+namespace {
+
+template <int TPR>
+__device__ __forceinline__ float team_sum(float v, float* red) {          // red: one float per wave of the workgroup
+#pragma unroll
+  for (int o = 1; o < (TPR < 64 ? TPR : 64); o <<= 1) v += __shfl_xor(v, o);
+  if constexpr (TPR > 64) {
+    constexpr int NW = TPR / 64;
+    const int wave = threadIdx.x >> 6;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[wave] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) v += red[i];                              // TPR > 64: the workgroup is one team
+  }
+  return v;
+}
+
+template <int N>
+__device__ __forceinline__ void load_w(const void* w, int w_is_f32, int dtype, long c, bool vec, float (&x)[N]) {
+  if (w == nullptr) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = 1.f;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    x[i] = (w_is_f32 || dtype == RR_F32) ? ((const float*)w)[c + i] : dtype == RR_F16 ? (float)((const rr_f16*)w)[c + i] : (float)((const rr_bf16*)w)[c + i];
+}
+template <typename T> struct code;
+template <> struct code<float> { static constexpr int v = RR_F32; };
+template <> struct code<rr_f16> { static constexpr int v = RR_F16; };
+template <> struct code<rr_bf16> { static constexpr int v = RR_BF16; };
+
+// ------------------------------------------------------------------------------------------------ forward
+template <typename T, int VEC, int TPR, int NC, bool FP8>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_fwd(const T* __restrict__ x, long ldx, const T* __restrict__ res, long ldr,
+                                                                  const void* __restrict__ w, int w32, T* __restrict__ y, T* __restrict__ h,
+                                                                  float* __restrict__ rstd, uint8_t* __restrict__ q, float* __restrict__ qs,
+                                                                  long rows, int E, float eps) {
+  constexpr int BLK = TPR > 256 ? TPR : 256, TEAMS = BLK / TPR;
+  __shared__ float red[BLK / 64];
+  __shared__ uint32_t gmax[FP8 && VEC == 1 ? TEAMS * 128 : 1];
+  const int team = threadIdx.x / TPR, lane = threadIdx.x % TPR;
+  const long row = (long)blockIdx.x * TEAMS + team;
+  const bool live = row < rows;                                            // (a dead team still takes part in the barriers)
+  float v[NC][VEC];
+  float ss = 0.f;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int col = (c * TPR + lane) * VEC;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[c][i] = 0.f;
+    if (live && col < E) {
+      rr_load_n<T, VEC>(x + row * ldx + col, v[c]);
+      if (res != nullptr) {
+        float r[VEC];
+        rr_load_n<T, VEC>(res + row * ldr + col, r);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[c][i] += r[i];
+      }
+      if (h != nullptr) rr_store_n<T, VEC>(h + row * (long)E + col, v[c]);
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) ss = fmaf(v[c][i], v[c][i], ss);
+  }
+  ss = team_sum<TPR>(ss, red);
+  const float s = 1.0f / sqrtf(ss / (float)E + eps);
+  if (rstd != nullptr && live && lane == 0) rstd[row] = s;
+  if constexpr (!FP8) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int col = (c * TPR + lane) * VEC;
+      if (live && col < E) {
+        float g[VEC];
+        load_w<VEC>(w, w32, code<T>::v, col, VEC > 1, g);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) g[i] = v[c][i] * s * g[i];
+        rr_store_n<T, VEC>(y + row * (long)E + col, g);
+      }
+    }
+  } else {
+    const int G = (E + 127) / 128;
+    if constexpr (VEC == 1) {                     // 128 columns are two waves: a group's maximum over LDS (a maximum has no order)
+      for (int i = threadIdx.x; i < TEAMS * 128; i += BLK) gmax[i] = 0u;
+      __syncthreads();
+    }
+    float a[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int col = (c * TPR + lane) * VEC;
+      a[c] = 0.f;
+      if (live && col < E) {
+        float g[VEC];
+        load_w<VEC>(w, w32, code<T>::v, col, VEC > 1, g);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) { v[c][i] = v[c][i] * s * g[i]; a[c] = fmaxf(a[c], fabsf(v[c][i])); }
+        if constexpr (VEC == 1) atomicMax(&gmax[team * 128 + col / 128], __float_as_uint(a[c]));
+      }
+      if constexpr (VEC > 1) {
+        constexpr int GL = 128 / VEC;             // lanes of a group
+#pragma unroll
+        for (int o = 1; o < (TPR < GL ? TPR : GL); o <<= 1) a[c] = fmaxf(a[c], __shfl_xor(a[c], o));
+      }
+    }
+    if constexpr (VEC == 1) __syncthreads();
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int col = (c * TPR + lane) * VEC;
+      if (live && col < E) {
+        const float am = VEC == 1 ? __uint_as_float(gmax[team * 128 + col / 128]) : a[c];
+        const float sc = am == 0.f ? 1.f : am / 448.0f;
+        if (col % 128 == 0) qs[row * G + col / 128] = sc;
+        float z[VEC < 4 ? 4 : VEC];
+#pragma unroll
+        for (int i = 0; i < (VEC < 4 ? 4 : VEC); ++i) {
+          const float e = i < VEC ? v[c][i < VEC ? i : 0] / sc : 0.f;
+          z[i] = e != e ? e : fminf(fmaxf(e, -448.f), 448.f);             // the quotient may pass 448 by a rounding
+        }
+        int p0 = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
+        p0 = __builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], p0, true);
+        uint8_t* dst = q + row * (long)E + col;
+        if constexpr (VEC == 1) dst[0] = (uint8_t)(p0 & 0xff);
+        if constexpr (VEC == 4) *reinterpret_cast<int*>(dst) = p0;
+        if constexpr (VEC == 8) {
+          int p1 = __builtin_amdgcn_cvt_pk_fp8_f32(z[4], z[5], 0, false);
+          p1 = __builtin_amdgcn_cvt_pk_fp8_f32(z[6], z[7], p1, true);
+          *reinterpret_cast<int2*>(dst) = make_int2(p0, p1);
+        }
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ backward
+template <typename T, int VEC, int TPR, int NC>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_bwd(const T* __restrict__ x, long ldx, const T* __restrict__ res, long ldr,
+                                                                  const void* __restrict__ w, int w32, const T* __restrict__ dy, long lddy,
+                                                                  const T* __restrict__ dh, long lddh, const float* __restrict__ rstd,
+                                                                  T* __restrict__ dx, float* __restrict__ dwp, long rows, int E) {
+  constexpr int BLK = TPR > 256 ? TPR : 256, TEAMS = BLK / TPR;
+  __shared__ float red[BLK / 64];
+  __shared__ float join[TEAMS > 1 ? TEAMS * TPR * VEC : 1];
+  const int team = threadIdx.x / TPR, lane = threadIdx.x % TPR;
+  float gw[NC][VEC], acc[NC][VEC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int col = (c * TPR + lane) * VEC;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) { gw[c][i] = 0.f; acc[c][i] = 0.f; }
+    if (col < E) load_w<VEC>(w, w32, code<T>::v, col, VEC > 1, gw[c]);
+  }
+  for (long r0 = (long)blockIdx.x * TEAMS; r0 < rows; r0 += (long)gridDim.x * TEAMS) {     // (uniform in the workgroup: the barriers inside are met)
+    const long row = r0 + team;
+    const bool live = row < rows;
+    float n[NC][VEC], g[NC][VEC];
+    const float s = live ? rstd[row] : 0.f;
+    float dot = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int col = (c * TPR + lane) * VEC;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) { n[c][i] = 0.f; g[c][i] = 0.f; }
+      if (live && col < E) {
+        rr_load_n<T, VEC>(x + row * ldx + col, n[c]);
+        if (res != nullptr) {
+          float r[VEC];
+          rr_load_n<T, VEC>(res + row * ldr + col, r);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) n[c][i] += r[i];
+        }
+        rr_load_n<T, VEC>(dy + row * lddy + col, g[c]);
+      }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        n[c][i] *= s;
+        acc[c][i] = fmaf(g[c][i], n[c][i], acc[c][i]);
+        g[c][i] *= gw[c][i];
+        dot = fmaf(g[c][i], n[c][i], dot);
+      }
+    }
+    dot = team_sum<TPR>(dot, red) / (float)E;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int col = (c * TPR + lane) * VEC;
+      if (live && col < E) {
+        float o[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) o[i] = 0.f;
+        if (dh != nullptr) rr_load_n<T, VEC>(dh + row * lddh + col, o);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) o[i] = fmaf(s, g[c][i] - n[c][i] * dot, o[i]);
+        rr_store_n<T, VEC>(dx + row * (long)E + col, o);
+      }
+    }
+  }
+  if (dwp == nullptr) return;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int col = (c * TPR + lane) * VEC;
+    if constexpr (TEAMS > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) join[(team * TPR + lane) * VEC + i] = acc[c][i];
+      __syncthreads();
+      if (team == 0) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          float t = 0.f;
+          for (int k = 0; k < TEAMS; ++k) t += join[(k * TPR + lane) * VEC + i];
+          acc[c][i] = t;
+        }
+      }
+    }
+    if (team == 0 && col < E) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) dwp[(long)blockIdx.x * E + col + i] = acc[c][i];
+    }
+  }
+}
+
+// dw[c] = sum of the P partial rows: 64 columns a workgroup, its 16 waves take every 16th row each, joined in order
+__global__ __launch_bounds__(1024) void k_rms_dw(const float* __restrict__ dwp, int P, int E, void* __restrict__ dw, int dtype) {
+  __shared__ float part[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
+  float t = 0.f;
+  if (c < E)
+    for (int p = wave; p < P; p += 16) t += dwp[(long)p * E + c];
+  part[wave][lane] = t;
+  __syncthreads();
+  if (wave == 0 && c < E) {
+    t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t += part[i][lane];
+    if (dtype == RR_F32) ((float*)dw)[c] = t;
+    else if (dtype == RR_F16) ((rr_f16*)dw)[c] = (rr_f16)t;
+    else ((rr_bf16*)dw)[c] = (rr_bf16)t;
+  }
+}
+
+int rms_launched(hipError_t e) { return e == hipSuccess ? RR_OK : RR_ELAUNCH; }
+
+// team size and pieces a lane by the number of pieces (VEC elements each) of a row
+#define RR_NORM_DISPATCH(T, V, RUN)                                                                                                       \
+  do {                                                                                                                                    \
+    const int pieces = (E + V - 1) / V;                                                                                                   \
+    if (pieces <= 16) { RUN(T, V, 16, 1); } else if (pieces <= 32) { RUN(T, V, 32, 1); } else if (pieces <= 64) { RUN(T, V, 64, 1); }      \
+    else if (pieces <= 128) { RUN(T, V, 64, 2); } else if (pieces <= 256) { RUN(T, V, 64, 4); } else if (pieces <= 512) { RUN(T, V, 256, 2); } \
+    else if (pieces <= 1024) { RUN(T, V, 256, 4); } else if (pieces <= 4096) { RUN(T, V, 1024, 4); }                                      \
+    else { if constexpr (V == 1) { RUN(T, V, 1024, 16); } else return RR_EINVAL; }                                                        \
+  } while (0)
+
+template <typename T>
+int norm_fwd(const void* x, long ldx, const void* res, long ldr, const void* w, int w32, void* y, void* h, float* rstd, uint8_t* q, float* qs, long rows, int E,
+             float eps, hipStream_t st) {
+  constexpr int N = rr_vec_of<T>::N;
+  const bool vec = E % N == 0 && ldx % N == 0 && ldr % N == 0 && rr_aligned16(x) && rr_aligned16(res) && rr_aligned16(y) && rr_aligned16(h) && rr_aligned16(q);
+#define RR_GO8(T_, V, TPR, NC) \
+  hipLaunchKernelGGL((k_rms_fwd<T_, V, TPR, NC, true>), dim3((unsigned)((rows + (TPR > 256 ? 1 : 256 / TPR) - 1) / (TPR > 256 ? 1 : 256 / TPR))), \
+                     dim3(TPR > 256 ? TPR : 256), 0, st, (const T*)x, ldx, (const T*)res, ldr, w, w32, (T*)y, (T*)h, rstd, q, qs, rows, E, eps)
+#define RR_GOT(T_, V, TPR, NC) \
+  hipLaunchKernelGGL((k_rms_fwd<T_, V, TPR, NC, false>), dim3((unsigned)((rows + (TPR > 256 ? 1 : 256 / TPR) - 1) / (TPR > 256 ? 1 : 256 / TPR))), \
+                     dim3(TPR > 256 ? TPR : 256), 0, st, (const T*)x, ldx, (const T*)res, ldr, w, w32, (T*)y, (T*)h, rstd, q, qs, rows, E, eps)
+  if (q != nullptr) {
+    if (vec) RR_NORM_DISPATCH(T, N, RR_GO8); else RR_NORM_DISPATCH(T, 1, RR_GO8);
+  } else {
+    if (vec) RR_NORM_DISPATCH(T, N, RR_GOT); else RR_NORM_DISPATCH(T, 1, RR_GOT);
+  }
+  return rms_launched(hipGetLastError());
+}
+
+template <typename T>
+int norm_bwd(const void* x, long ldx, const void* res, long ldr, const void* w, int w32, const void* dy, long lddy, const void* dh, long lddh, const float* rstd,
+             void* dx, void* dw, float* dwp, int parts, long rows, int E, hipStream_t st) {
+  constexpr int N = rr_vec_of<T>::N;
+  const bool vec = E % N == 0 && ldx % N == 0 && ldr % N == 0 && lddy % N == 0 && lddh % N == 0 && rr_aligned16(x) && rr_aligned16(res) && rr_aligned16(dy) &&
+                   rr_aligned16(dh) && rr_aligned16(dx);
+#define RR_GOB(T_, V, TPR, NC) \
+  hipLaunchKernelGGL((k_rms_bwd<T_, V, TPR, NC>), dim3((unsigned)parts), dim3(TPR > 256 ? TPR : 256), 0, st, (const T*)x, ldx, (const T*)res, ldr, w, w32, \
+                     (const T*)dy, lddy, (const T*)dh, lddh, rstd, (T*)dx, dw != nullptr ? dwp : (float*)nullptr, rows, E)
+  if (vec) RR_NORM_DISPATCH(T, N, RR_GOB); else RR_NORM_DISPATCH(T, 1, RR_GOB);
+  if (dw != nullptr) hipLaunchKernelGGL(k_rms_dw, dim3((E + 63) / 64), dim3(1024), 0, st, dwp, parts, E, dw, w32 ? RR_F32 : code<T>::v);
+  return rms_launched(hipGetLastError());
+}
+
+}  // namespace
+
+extern "C" int rr_add_rms_norm(int dtype, const void* x, long long ldx, const void* res, long long ldr, const void* w, int w_is_f32, void* y, void* h, float* rstd,
+                               uint8_t* q, float* qscale, long long rows, int E, float eps, hipStream_t st) {
+  if (rows < 0 || E < 1 || E > 16384 || x == nullptr || rows > 0x7fffffffLL || (y == nullptr) == (q == nullptr) || (q == nullptr) != (qscale == nullptr) || ldx < 0 || ldr < 0)
+    return RR_EINVAL;
+  if (rows == 0) return RR_OK;
+  if (res == nullptr) ldr = 0;
+  switch (dtype) {
+    case RR_F32: return norm_fwd<float>(x, ldx, res, ldr, w, w_is_f32, y, h, rstd, q, qscale, rows, E, eps, st);
+    case RR_F16: return norm_fwd<rr_f16>(x, ldx, res, ldr, w, w_is_f32, y, h, rstd, q, qscale, rows, E, eps, st);
+    case RR_BF16: return norm_fwd<rr_bf16>(x, ldx, res, ldr, w, w_is_f32, y, h, rstd, q, qscale, rows, E, eps, st);
+  }
+  return RR_EINVAL;
+}
+
+extern "C" int rr_add_rms_norm_parts(long long rows, int E) {      // workgroups of the backward = partial rows of dw (floats [parts][E])
+  const long long per = E <= 4096 ? 4 : 1;                         // about four teams a workgroup and four rows a team at the least
+  const long long want = (rows + 4 * per - 1) / (4 * per);
+  return (int)(want < 1 ? 1 : want > 1024 ? 1024 : want);
+}
+
+extern "C" int rr_add_rms_norm_bwd(int dtype, const void* x, long long ldx, const void* res, long long ldr, const void* w, int w_is_f32, const void* dy, long long lddy,
+                                   const void* dh, long long lddh, const float* rstd, void* dx, void* dw, float* workspace, int parts, long long rows, int E,
+                                   hipStream_t st) {
+  if (rows < 1 || E < 1 || E > 16384 || x == nullptr || dy == nullptr || rstd == nullptr || dx == nullptr || parts < 1 || rows > 0x7fffffffLL ||
+      (dw != nullptr && (w == nullptr || workspace == nullptr)) || ldx < 0 || ldr < 0 || lddy < 0 || lddh < 0)
+    return RR_EINVAL;
+  if (res == nullptr) ldr = 0;
+  if (dh == nullptr) lddh = 0;
+  switch (dtype) {
+    case RR_F32: return norm_bwd<float>(x, ldx, res, ldr, w, w_is_f32, dy, lddy, dh, lddh, rstd, dx, dw, workspace, parts, rows, E, st);
+    case RR_F16: return norm_bwd<rr_f16>(x, ldx, res, ldr, w, w_is_f32, dy, lddy, dh, lddh, rstd, dx, dw, workspace, parts, rows, E, st);
+    case RR_BF16: return norm_bwd<rr_bf16>(x, ldx, res, ldr, w, w_is_f32, dy, lddy, dh, lddh, rstd, dx, dw, workspace, parts, rows, E, st);
+  }
+  return RR_EINVAL;
+}
