@@ -456,6 +456,42 @@ int rr_select_matnet(const float* logits, const uint8_t* mask, const int64_t* ac
                      float* logp_out, float* logp_all, int R, int N, float tanh_clipping, float temperature,
                      int mode, uint64_t seed, uint32_t step, hipStream_t stream);
 
+/* ---- operators of a decoder at any width and in float32 (dtype 0), float16 (1) or bfloat16 (2) -------------------------------------------
+ * Cross attention: G * Hk query heads on Hk key heads, out = softmax(scale q k^T over the keys that may be seen) v, lse = log sum exp
+ * (a query that sees nothing: zeros, -inf).  q [B][Lq][G*Hk][D], k, v [B][Lk][Hk][D] by element strides (batch, position, head), the
+ * last axis contiguous, bases and strides on 16 bytes; D a multiple of 8 up to 128.  mask: bytes [B][G*Hk][Lq][Lk] by strides (batch, head,
+ * query), 1 = may be seen, or NULL; kv_lens [B] int32 / int64 or NULL.  out, dq [B][Lq][G*Hk][D], dk, dv [B][Lk][Hk][D], lse and delta
+ * [B][G*Hk][Lq] (delta: scratch of the backward) are contiguous.  workspace: rr_cross_attn_workspace bytes (-1: sizes refused). */
+typedef struct {
+  const void *q, *k, *v;
+  void* out;
+  float* lse;                  /* forward: may be NULL */
+  const uint8_t* mask;
+  const void* kv_lens;
+  const void* dout;            /* dout, delta, dq, dk, dv: backward only */
+  float* delta;
+  void *dq, *dk, *dv;
+  void* workspace;
+  long long q_stride[3], k_stride[3], v_stride[3], mask_stride[3], dout_stride[3];
+  long long workspace_bytes;
+  int lens_int64, dtype, B, Lq, Lk, Hk, G, D;
+  float scale;
+} XAttnIO;
+long long rr_cross_attn_workspace(int B, int Lq, int Lk, int Hk, int G, int D, int backward);
+int rr_cross_attn(const XAttnIO* io, hipStream_t stream);
+int rr_cross_attn_bwd(const XAttnIO* io, hipStream_t stream);
+
+/* h = x + res, y = h rsqrt(mean(h^2) + eps) w over rows of E <= 16384 (RMSNorm rrnco/models/nn/attn_freenet.py:13-26 behind a residual).  x, res
+ * by row strides in elements, the rest contiguous; res, w, h, rstd may be NULL; w in the inputs' type or float32.  Either y, or
+ * q (e4m3 bytes [rows][E]) with qscale [rows][ceil(E / 128)].  Backward: dx (= the residual's gradient), dw (or NULL) from dy, dh
+ * (or NULL) and the forward's rstd; workspace: parts * E floats with parts = rr_add_rms_norm_parts(rows, E). */
+int rr_add_rms_norm(int dtype, const void* x, long long ldx, const void* res, long long ldr, const void* w, int w_is_f32, void* y, void* h,
+                    float* rstd, uint8_t* q, float* qscale, long long rows, int E, float eps, hipStream_t stream);
+int rr_add_rms_norm_parts(long long rows, int E);
+int rr_add_rms_norm_bwd(int dtype, const void* x, long long ldx, const void* res, long long ldr, const void* w, int w_is_f32, const void* dy,
+                        long long lddy, const void* dh, long long lddh, const float* rstd, void* dx, void* dw, float* workspace, int parts,
+                        long long rows, int E, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

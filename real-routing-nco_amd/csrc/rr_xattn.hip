@@ -1,0 +1,882 @@
+// Cross attention: Lq queries of Hq heads on Lk keys of Hk heads (Hq = G Hk), forward and backward, float32 / float16 / bfloat16.
+//
+//   s = scale q.k over the visible keys (mask, kv_lens),  p = softmax(s),  o = sum p v,  lse = log sum exp s
+//   a row that sees no key: o = 0, lse = -inf, no gradient
+//   delta = sum_d do o,  ds = p (do.v - delta),  dq = scale sum ds k,  dk = scale sum ds q,  dv = sum p do   (dk, dv over the group)
+//
+// Rows: the G Lq queries that share a key head are one list of rows (row = group member * Lq + position), so that a tile of keys
+// and values is read once for all of them; with one query a group of heads still fills a matrix tile.
+// Tiles: scores are computed transposed, S^T = K Q^T in 16 x 16 tiles, so that a lane holds one query's scores of four consecutive
+// keys: the softmax's rescaling is one factor a lane, and P^T is in the registers exactly as the second product
+// O^T = V^T P^T takes it (the sum over the keys runs in the order that the registers hold, V^T is read with the same order:
+// ds_read_b64_tr_b16 for 16-bit types, four plain reads for float32).  The running maximum and sum are in 32 bits; P is rounded to
+// the inputs' type for the second product (half a step of a weight <= 1, under the rounding of the output).
+// float32 runs on v_mfma_f32_16x16x4 (exact products), 16-bit types on v_mfma_f32_16x16x32.
+// The backward recomputes P from lse; dq walks over keys, (dk, dv) over rows: no atomics, the same result every time.
+// Few rows: the key axis is split over workgroups and joined by a second launch.
+// Non-finite values where nothing may look (a masked key whose value is NaN): 0 * NaN would spoil the products, so a workgroup
+// whose accumulators end non-finite walks its tiles once more with the non-finite 16-byte pieces replaced by zeros and their
+// contribution to the rows that do see them put back: a masked key never shows, a visible one does.
+#include "rr_types.h"
+
+namespace {
+
+#define RR_XA_KT 64            // keys (or rows) of a staged tile
+#define RR_LOG2E 1.44269504088896340736f
+#define RR_LN2 0.69314718055994530942f
+
+struct XAttn {
+  const void *q, *k, *v;
+  void* out;
+  float* lse;                            // [B][Hq][Lq] or NULL
+  const uint8_t* mask;                   // [B][Hq][Lq][Lk] by strides, 1 = may be seen, or NULL
+  const void* lens;                      // [B] int32 / int64 or NULL
+  long long qb, ql, qh, kb, kl, kh, vb, vl, vh, mb, ml, mh;
+  int lens64, B, Lq, Lk, Hk, G, D;
+  float scale;
+  int nsplit, tiles_per_split, nblk;     // splits of the walked axis, its tiles a split, workgroups along the kept axis
+  float* part;                           // partial results of the splits
+  // backward
+  const void* dout;
+  long long gb, gl, gh;
+  float* delta;                          // [B][Hq][Lq]
+  void *dq, *dk, *dv;                    // contiguous
+};
+
+template <typename T> struct Mx;
+template <> struct Mx<float> {
+  typedef f32x4 Frag;
+  static constexpr int KC = 16, EPC = 4, PT = 1;          // contraction of a step, elements of 16 bytes, score tiles a second-product step takes
+  static __device__ __forceinline__ f32x4 mma(Frag a, Frag b, f32x4 c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+    return c;
+  }
+  static __device__ __forceinline__ Frag pack(const f32x4* p) { return p[0]; }
+  static __device__ __forceinline__ Frag tr(const float* t, int pitch, int row0, int col0, int lane) {      // A = X^T: rows row0 + 4g + i, column col0 + lane % 16
+    const float* p = t + (row0 + 4 * (lane >> 4)) * pitch + col0 + (lane & 15);
+    Frag f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = p[i * pitch];
+    return f;
+  }
+};
+typedef short rr_s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) rr_s16x4 rr_lds_s16x4;
+template <typename T>
+__device__ __forceinline__ void tr16(const T* t, int pitch, int row0, int col0, int lane, short (&f)[8]) {
+  const int i = lane & 15;
+  T* p = const_cast<T*>(t) + (row0 + 4 * (lane >> 4) + (i >> 2)) * pitch + col0 + 4 * (i & 3);
+  const rr_s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((rr_lds_s16x4*)p);
+  const rr_s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((rr_lds_s16x4*)(p + 16 * pitch));
+#pragma unroll
+  for (int j = 0; j < 4; ++j) { f[j] = a[j]; f[4 + j] = b[j]; }
+}
+typedef short rr_s16x8 __attribute__((ext_vector_type(8)));
+template <> struct Mx<rr_f16> {
+  typedef rr_f16x8 Frag;
+  static constexpr int KC = 32, EPC = 8, PT = 2;
+  static __device__ __forceinline__ f32x4 mma(Frag a, Frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ Frag pack(const f32x4* p) {
+    Frag f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f[i] = (rr_f16)p[0][i]; f[4 + i] = (rr_f16)p[1][i]; }
+    return f;
+  }
+  static __device__ __forceinline__ Frag tr(const rr_f16* t, int pitch, int row0, int col0, int lane) {
+    short f[8];
+    tr16(t, pitch, row0, col0, lane, f);
+    rr_s16x8 v = {f[0], f[1], f[2], f[3], f[4], f[5], f[6], f[7]};
+    return __builtin_bit_cast(Frag, v);
+  }
+};
+template <> struct Mx<rr_bf16> {
+  typedef rr_bf16x8 Frag;
+  static constexpr int KC = 32, EPC = 8, PT = 2;
+  static __device__ __forceinline__ f32x4 mma(Frag a, Frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ Frag pack(const f32x4* p) {
+    Frag f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f[i] = (rr_bf16)p[0][i]; f[4 + i] = (rr_bf16)p[1][i]; }
+    return f;
+  }
+  static __device__ __forceinline__ Frag tr(const rr_bf16* t, int pitch, int row0, int col0, int lane) {
+    short f[8];
+    tr16(t, pitch, row0, col0, lane, f);
+    rr_s16x8 v = {f[0], f[1], f[2], f[3], f[4], f[5], f[6], f[7]};
+    return __builtin_bit_cast(Frag, v);
+  }
+};
+
+template <typename T> using FragOf = typename Mx<T>::Frag;
+
+template <typename T, int DP> struct Dims {
+  static constexpr int KD = DP < Mx<T>::KC ? Mx<T>::KC : DP;      // columns of a staged row (zeros behind the head dim)
+  static constexpr int NK = KD / Mx<T>::KC;                       // steps of the first product
+  static constexpr int DT = DP / 16;                              // tiles of the second product
+  // row pitches: 16 bytes more than the row lets 16 rows' 16-byte reads start in 16 different bank groups; transposed 16-bit
+  // reads (four rows of 32 bytes a lane group) want 32
+  static constexpr int PR = KD + 16 / (int)sizeof(T);
+  static constexpr int PX = KD + (sizeof(T) == 2 ? 32 : 16) / (int)sizeof(T);
+  static constexpr int CPR = KD / Mx<T>::EPC;                     // 16-byte pieces of a staged row
+};
+
+__device__ __forceinline__ bool nonfinite4(const float4& v, int is16) {
+  const uint32_t w[4] = {__float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z), __float_as_uint(v.w)};
+  bool b = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (is16 == 0) b |= (w[i] & 0x7f800000u) == 0x7f800000u;
+    else {
+      const uint32_t e = is16 == 1 ? 0x7c00u : 0x7f80u;
+      b |= (w[i] & e) == e || (w[i] >> 16 & e) == e;
+    }
+  }
+  return b;
+}
+template <typename T> struct kind16;
+template <> struct kind16<float> { static constexpr int v = 0; };
+template <> struct kind16<rr_f16> { static constexpr int v = 1; };
+template <> struct kind16<rr_bf16> { static constexpr int v = 2; };
+
+// one row of the packed row list: group member r / Lq, position r % Lq
+struct RowAt { int g, s; };
+__device__ __forceinline__ RowAt row_at(int r, int Lq, int G) {
+  if (G == 1) return {0, r};
+  const int g = r / Lq;
+  return {g, r - g * Lq};
+}
+
+// rows [row0, row0 + 64) of a key-side tensor into LDS (zeros behind the last row and the head dim).
+// safe: pieces that hold a non-finite value become zeros and their row's bit is set in `flag`
+template <typename T, int DP, int PITCH, typename PTR>
+__device__ __forceinline__ void stage(T* lds, PTR rowptr, int row0, int valid, int D, bool safe, uint32_t* flag) {
+  using Dm = Dims<T, DP>;
+  constexpr int N = RR_XA_KT * Dm::CPR / 256;
+  float4 v[N];
+#pragma unroll
+  for (int c = 0; c < N; ++c) {
+    const int i = threadIdx.x + 256 * c, row = i / Dm::CPR, ch = i % Dm::CPR;
+    v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (row0 + row < valid && ch * Mx<T>::EPC < D) v[c] = *reinterpret_cast<const float4*>(rowptr(row0 + row) + ch * Mx<T>::EPC);
+  }
+#pragma unroll
+  for (int c = 0; c < N; ++c) {
+    const int i = threadIdx.x + 256 * c, row = i / Dm::CPR, ch = i % Dm::CPR;
+    if (safe && nonfinite4(v[c], kind16<T>::v)) {
+      v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+      atomicOr(&flag[row >> 5], 1u << (row & 31));
+    }
+    *reinterpret_cast<float4*>(lds + row * PITCH + ch * Mx<T>::EPC) = v[c];
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ FragOf<T> frag_at(const T* p) { return *reinterpret_cast<const FragOf<T>*>(p); }
+template <typename T>
+__device__ __forceinline__ FragOf<T> frag_zero() {
+  FragOf<T> f;
+#pragma unroll
+  for (int i = 0; i < Mx<T>::EPC; ++i) f[i] = (T)0.f;
+  return f;
+}
+
+__device__ __forceinline__ int seen_keys(const XAttn& a, int b) {
+  if (a.lens == nullptr) return a.Lk;
+  const long long n = a.lens64 ? ((const long long*)a.lens)[b] : (long long)((const int*)a.lens)[b];
+  return n < 0 ? 0 : n > a.Lk ? a.Lk : (int)n;
+}
+// four consecutive mask bytes of a row, keys behind the end as zeros (one unaligned 4-byte load inside the row)
+__device__ __forceinline__ uint32_t mask4(const uint8_t* row, int key, int Lk) {
+  uint32_t m = 0;
+  if (key + 4 <= Lk) __builtin_memcpy(&m, row + key, 4);
+  else
+    for (int i = 0; i < 4; ++i)
+      if (key + i < Lk) m |= (uint32_t)row[key + i] << (8 * i);
+  return m;
+}
+__device__ __forceinline__ float group_max(float v) { v = fmaxf(v, __shfl_xor(v, 16)); return fmaxf(v, __shfl_xor(v, 32)); }
+__device__ __forceinline__ float group_sum(float v) { v += __shfl_xor(v, 16); return v + __shfl_xor(v, 32); }
+__device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
+__device__ __forceinline__ bool is_bad(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
+
+// the wave's QT x 16 rows as B operands (lane: row lane % 16, 16 bytes at piece lane / 16 of every contraction step)
+template <typename T, int DP, int QT, typename F>
+__device__ __forceinline__ void load_rows(F& f, const T* base, long long sl, long long sh, int row0, int R, const XAttn& a, int lane) {
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int r = row0 + 16 * t + (lane & 15);
+    const RowAt at = row_at(r < R ? r : R - 1, a.Lq, a.G);
+    const T* p = base + at.s * sl + at.g * sh;
+#pragma unroll
+    for (int k = 0; k < Dims<T, DP>::NK; ++k) {
+      const int c = k * Mx<T>::KC + (lane >> 4) * Mx<T>::EPC;
+      f[t][k] = r < R && c < a.D ? frag_at<T>(p + c) : frag_zero<T>();
+    }
+  }
+}
+
+struct Blk { int b, hk, split, blk; };
+__device__ __forceinline__ Blk block_of(const XAttn& a) {
+  long long i = blockIdx.x;
+  Blk w;
+  w.blk = (int)(i % a.nblk); i /= a.nblk;
+  w.split = (int)(i % a.nsplit); i /= a.nsplit;
+  w.hk = (int)(i % a.Hk);
+  w.b = (int)(i / a.Hk);
+  return w;
+}
+
+// ------------------------------------------------------------------------------------------------ forward
+template <typename T, int DP, int QT>
+__global__ __launch_bounds__(256) void k_xattn_fwd(XAttn a) {
+  using M = Mx<T>;
+  using Dm = Dims<T, DP>;
+  __shared__ __attribute__((aligned(16))) T sk[RR_XA_KT * Dm::PR];
+  __shared__ __attribute__((aligned(16))) T sv[RR_XA_KT * Dm::PX];
+  __shared__ uint32_t flag[2];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
+  const Blk w = block_of(a);
+  const int R = a.G * a.Lq, row0 = (w.blk * 4 + wave) * 16 * QT;
+  const bool busy = row0 < R;
+  const int seen = seen_keys(a, w.b);
+  const T* kp = (const T*)a.k + (long long)w.b * a.kb + (long long)w.hk * a.kh;
+  const T* vp = (const T*)a.v + (long long)w.b * a.vb + (long long)w.hk * a.vh;
+  typename M::Frag qf[QT][Dm::NK];
+  load_rows<T, DP, QT>(qf, (const T*)a.q + (long long)w.b * a.qb + (long long)w.hk * a.G * a.qh, a.ql, a.qh, row0, R, a, lane);
+  const uint8_t* mrow[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int r = row0 + 16 * t + j;
+    const RowAt at = row_at(r < R ? r : R - 1, a.Lq, a.G);
+    mrow[t] = a.mask + w.b * a.mb + (w.hk * a.G + at.g) * a.mh + at.s * a.ml;
+  }
+  const float c2 = a.scale * RR_LOG2E;
+  const int first = w.split * a.tiles_per_split * RR_XA_KT;
+  int last = first + a.tiles_per_split * RR_XA_KT;
+  last = last < seen ? last : seen;
+  f32x4 o[QT][Dm::DT];
+  float m[QT], l[QT];
+  for (int pass = 0; pass < 2; ++pass) {
+    const bool safe = pass == 1;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      m[t] = -INFINITY; l[t] = 0.f;
+#pragma unroll
+      for (int d = 0; d < Dm::DT; ++d) o[t][d] = rr_zero4();
+    }
+    for (int k0 = first; k0 < last; k0 += RR_XA_KT) {
+      __syncthreads();
+      if (safe) {
+        if (threadIdx.x < 2) flag[threadIdx.x] = 0u;
+        __syncthreads();
+      }
+      stage<T, DP, Dm::PR>(sk, [&](int r) { return kp + (long long)r * a.kl; }, k0, seen, a.D, false, flag);
+      stage<T, DP, Dm::PX>(sv, [&](int r) { return vp + (long long)r * a.vl; }, k0, seen, a.D, safe, flag);
+      __syncthreads();
+      if (!busy) continue;
+      f32x4 s[QT][4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+#pragma unroll
+        for (int t = 0; t < QT; ++t) s[t][n] = rr_zero4();
+#pragma unroll
+        for (int k = 0; k < Dm::NK; ++k) {
+          const typename M::Frag f = frag_at<T>(sk + (16 * n + j) * Dm::PR + k * M::KC + g * M::EPC);
+#pragma unroll
+          for (int t = 0; t < QT; ++t) s[t][n] = M::mma(f, qf[t][k], s[t][n]);
+        }
+      }
+      if (a.mask != nullptr || k0 + RR_XA_KT > seen) {
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const int key = k0 + 16 * n + 4 * g;
+            const uint32_t mb = a.mask != nullptr ? mask4(mrow[t], key, a.Lk) : 0x01010101u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[t][n][i] = (key + i < seen && (mb >> (8 * i) & 0xffu)) ? s[t][n][i] : -INFINITY;
+          }
+      }
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[t][n][i]);
+        const float mn = fmaxf(m[t], group_max(mx) * c2);
+        const float mu = finite_or_zero(mn);
+        const float al = __builtin_amdgcn_exp2f(m[t] - mu);
+        float sum = 0.f;
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[t][n][i] = __builtin_amdgcn_exp2f(fmaf(s[t][n][i], c2, -mu));
+            sum += s[t][n][i];
+          }
+        l[t] = fmaf(l[t], al, sum);
+        m[t] = mn;
+#pragma unroll
+        for (int d = 0; d < Dm::DT; ++d) o[t][d] *= al;
+      }
+#pragma unroll
+      for (int n = 0; n < 4; n += M::PT) {
+        typename M::Frag pf[QT];
+#pragma unroll
+        for (int t = 0; t < QT; ++t) pf[t] = M::pack(&s[t][n]);
+#pragma unroll
+        for (int d = 0; d < Dm::DT; ++d) {
+          const typename M::Frag f = M::tr(sv, Dm::PX, 16 * n, 16 * d, lane);
+#pragma unroll
+          for (int t = 0; t < QT; ++t) o[t][d] = M::mma(f, pf[t], o[t][d]);
+        }
+      }
+      if (safe && (flag[0] | flag[1])) {           // rare: what visible keys hold in the pieces that were zeroed
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+          for (int kk = 0; kk < 16; ++kk) {
+            const int key = 16 * n + kk;
+            if (!(flag[key >> 5] >> (key & 31) & 1u)) continue;
+            const T* vr = vp + (long long)(k0 + key) * a.vl;
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+              const float mine = (kk & 3) == 0 ? s[t][n][0] : (kk & 3) == 1 ? s[t][n][1] : (kk & 3) == 2 ? s[t][n][2] : s[t][n][3];
+              const float p = __shfl(mine, j + 16 * (kk >> 2));
+#pragma unroll
+              for (int d = 0; d < Dm::DT; ++d) {
+                const int c = 16 * d + 4 * g, piece = c / M::EPC * M::EPC;
+                if (p == 0.f || c >= a.D || !nonfinite4(*reinterpret_cast<const float4*>(vr + piece), kind16<T>::v)) continue;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[t][d][i] += p * (float)vr[c + i];
+              }
+            }
+          }
+      }
+    }
+    bool bad = false;
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+#pragma unroll
+      for (int d = 0; d < Dm::DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bad |= is_bad(o[t][d][i]);
+    if (!__syncthreads_or(bad && busy)) break;
+  }
+  if (!busy) return;
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int r = row0 + 16 * t + j;
+    const float lt = group_sum(l[t]);
+    if (r >= R) continue;
+    const RowAt at = row_at(r, a.Lq, a.G);
+    const int head = w.hk * a.G + at.g;
+    if (a.nsplit > 1) {                            // partials: [B * Hk * R][nsplit][DP + 2] floats
+      float* p = a.part + (((long long)(w.b * a.Hk + w.hk) * R + r) * a.nsplit + w.split) * (DP + 4);
+#pragma unroll
+      for (int d = 0; d < Dm::DT; ++d) *reinterpret_cast<f32x4*>(p + 16 * d + 4 * g) = o[t][d];
+      if (g == 0) { p[DP] = m[t]; p[DP + 1] = lt; }
+    } else {
+      const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+      T* dst = (T*)a.out + (((long long)w.b * a.Lq + at.s) * (a.Hk * a.G) + head) * a.D;
+#pragma unroll
+      for (int d = 0; d < Dm::DT; ++d) {
+        const int c = 16 * d + 4 * g;
+        if (c < a.D) {
+          typedef T V4 __attribute__((ext_vector_type(4)));
+          V4 v;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] = (T)(o[t][d][i] * inv);
+          *reinterpret_cast<V4*>(dst + c) = v;
+        }
+      }
+      if (a.lse != nullptr && g == 0)
+        a.lse[((long long)w.b * (a.Hk * a.G) + head) * a.Lq + at.s] = lt == 0.f ? -INFINITY : (m[t] + __log2f(lt)) * RR_LN2;
+    }
+  }
+}
+
+// joins the splits of a row: one wave a row, the lanes its columns
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void k_xattn_join(XAttn a) {
+  const int lane = threadIdx.x & 63;
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int R = a.G * a.Lq;
+  if (row >= (long long)a.B * a.Hk * R) return;
+  const float* p = a.part + row * a.nsplit * (DP + 4);
+  float m = -INFINITY;
+  for (int i = lane; i < a.nsplit; i += 64) m = fmaxf(m, p[i * (DP + 4) + DP]);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+  const float mu = finite_or_zero(m);
+  float acc[(DP + 63) / 64], l = 0.f;
+#pragma unroll
+  for (int c = 0; c < (DP + 63) / 64; ++c) acc[c] = 0.f;
+  for (int i = 0; i < a.nsplit; ++i) {
+    const float* pi = p + i * (DP + 4);
+    const float f = __builtin_amdgcn_exp2f(pi[DP] - mu);
+    l = fmaf(pi[DP + 1], f, l);
+#pragma unroll
+    for (int c = 0; c < (DP + 63) / 64; ++c)
+      if (lane + 64 * c < DP) acc[c] = pi[DP] == -INFINITY ? acc[c] : fmaf(pi[lane + 64 * c], f, acc[c]);
+  }
+  const int b = (int)(row / ((long long)a.Hk * R)), hk = (int)(row / R % a.Hk);
+  const RowAt at = row_at((int)(row % R), a.Lq, a.G);
+  const int head = hk * a.G + at.g;
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  T* dst = (T*)a.out + (((long long)b * a.Lq + at.s) * (a.Hk * a.G) + head) * a.D;
+#pragma unroll
+  for (int c = 0; c < (DP + 63) / 64; ++c)
+    if (lane + 64 * c < a.D) dst[lane + 64 * c] = (T)(acc[c] * inv);
+  if (a.lse != nullptr && lane == 0) a.lse[((long long)b * (a.Hk * a.G) + head) * a.Lq + at.s] = l == 0.f ? -INFINITY : (m + __log2f(l)) * RR_LN2;
+}
+
+
+// ------------------------------------------------------------------------------------------------ backward: dq (walks over the keys)
+template <typename T, int DP, int QT>
+__global__ __launch_bounds__(256) void k_xattn_dq(XAttn a) {
+  using M = Mx<T>;
+  using Dm = Dims<T, DP>;
+  __shared__ __attribute__((aligned(16))) T sk[RR_XA_KT * Dm::PX];
+  __shared__ __attribute__((aligned(16))) T sv[RR_XA_KT * Dm::PR];
+  __shared__ uint32_t flag[2];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
+  const Blk w = block_of(a);
+  const int R = a.G * a.Lq, H = a.G * a.Hk, row0 = (w.blk * 4 + wave) * 16 * QT;
+  const bool busy = row0 < R;
+  const int seen = seen_keys(a, w.b);
+  const T* kp = (const T*)a.k + (long long)w.b * a.kb + (long long)w.hk * a.kh;
+  const T* vp = (const T*)a.v + (long long)w.b * a.vb + (long long)w.hk * a.vh;
+  typename M::Frag qf[QT][Dm::NK], gf[QT][Dm::NK];
+  load_rows<T, DP, QT>(qf, (const T*)a.q + (long long)w.b * a.qb + (long long)w.hk * a.G * a.qh, a.ql, a.qh, row0, R, a, lane);
+  load_rows<T, DP, QT>(gf, (const T*)a.dout + (long long)w.b * a.gb + (long long)w.hk * a.G * a.gh, a.gl, a.gh, row0, R, a, lane);
+  const uint8_t* mrow[QT];
+  float lse2[QT], delta[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int r = row0 + 16 * t + j, rc = r < R ? r : R - 1;
+    const RowAt at = row_at(rc, a.Lq, a.G);
+    const int head = w.hk * a.G + at.g;
+    mrow[t] = a.mask + w.b * a.mb + head * a.mh + at.s * a.ml;
+    const long long li = ((long long)w.b * H + head) * a.Lq + at.s;
+    lse2[t] = busy && r < R ? a.lse[li] * RR_LOG2E : 0.f;
+    const T* op = (const T*)a.out + (((long long)w.b * a.Lq + at.s) * H + head) * a.D;
+    float d = 0.f;
+#pragma unroll
+    for (int k = 0; k < Dm::NK; ++k) {
+      const int c = k * M::KC + g * M::EPC;
+      if (r < R && c < a.D) {
+        const typename M::Frag of = frag_at<T>(op + c);
+#pragma unroll
+        for (int i = 0; i < M::EPC; ++i) d = fmaf((float)of[i], (float)gf[t][k][i], d);
+      }
+    }
+    delta[t] = group_sum(d);
+    if (w.split == 0 && g == 0 && r < R) a.delta[li] = delta[t];
+  }
+  const float c2 = a.scale * RR_LOG2E;
+  const int first = w.split * a.tiles_per_split * RR_XA_KT;
+  int last = first + a.tiles_per_split * RR_XA_KT;
+  last = last < seen ? last : seen;
+  f32x4 o[QT][Dm::DT];
+  for (int pass = 0; pass < 2; ++pass) {
+    const bool safe = pass == 1;
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+#pragma unroll
+      for (int d = 0; d < Dm::DT; ++d) o[t][d] = rr_zero4();
+    for (int k0 = first; k0 < last; k0 += RR_XA_KT) {
+      __syncthreads();
+      if (safe) {
+        if (threadIdx.x < 2) flag[threadIdx.x] = 0u;
+        __syncthreads();
+      }
+      stage<T, DP, Dm::PX>(sk, [&](int r) { return kp + (long long)r * a.kl; }, k0, seen, a.D, safe, flag);
+      stage<T, DP, Dm::PR>(sv, [&](int r) { return vp + (long long)r * a.vl; }, k0, seen, a.D, false, flag);
+      __syncthreads();
+      if (!busy) continue;
+#pragma unroll
+      for (int n = 0; n < 4; n += M::PT) {
+        f32x4 s[QT][M::PT], dp[QT][M::PT];
+#pragma unroll
+        for (int u = 0; u < M::PT; ++u) {
+#pragma unroll
+          for (int t = 0; t < QT; ++t) { s[t][u] = rr_zero4(); dp[t][u] = rr_zero4(); }
+#pragma unroll
+          for (int k = 0; k < Dm::NK; ++k) {
+            const typename M::Frag fk = frag_at<T>(sk + (16 * (n + u) + j) * Dm::PX + k * M::KC + g * M::EPC);
+            const typename M::Frag fv = frag_at<T>(sv + (16 * (n + u) + j) * Dm::PR + k * M::KC + g * M::EPC);
+#pragma unroll
+            for (int t = 0; t < QT; ++t) { s[t][u] = M::mma(fk, qf[t][k], s[t][u]); dp[t][u] = M::mma(fv, gf[t][k], dp[t][u]); }
+          }
+        }
+        typename M::Frag pf[QT];
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+#pragma unroll
+          for (int u = 0; u < M::PT; ++u) {
+            const int key = k0 + 16 * (n + u) + 4 * g;
+            const uint32_t mb = a.mask != nullptr ? mask4(mrow[t], key, a.Lk) : 0x01010101u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const bool see = key + i < seen && (mb >> (8 * i) & 0xffu);
+              float p = __builtin_amdgcn_exp2f(fmaf(s[t][u][i], c2, -lse2[t]));
+              if (safe && (flag[(key + i - k0) >> 5] >> ((key + i - k0) & 31) & 1u)) p = __builtin_nanf("");     // a visible key that holds a non-finite value
+              s[t][u][i] = see ? p * (dp[t][u][i] - delta[t]) : 0.f;
+            }
+          }
+          pf[t] = M::pack(s[t]);
+        }
+#pragma unroll
+        for (int d = 0; d < Dm::DT; ++d) {
+          const typename M::Frag f = M::tr(sk, Dm::PX, 16 * n, 16 * d, lane);
+#pragma unroll
+          for (int t = 0; t < QT; ++t) o[t][d] = M::mma(f, pf[t], o[t][d]);
+        }
+      }
+    }
+    bool bad = false;
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+#pragma unroll
+      for (int d = 0; d < Dm::DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bad |= is_bad(o[t][d][i]);
+    if (!__syncthreads_or(bad && busy)) break;
+  }
+  if (!busy) return;
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int r = row0 + 16 * t + j;
+    if (r >= R) continue;
+    const RowAt at = row_at(r, a.Lq, a.G);
+    const long long at_out = (((long long)w.b * a.Lq + at.s) * H + w.hk * a.G + at.g) * a.D;
+    float* p = a.part + (long long)w.split * a.B * a.Lq * H * a.D + at_out;
+#pragma unroll
+    for (int d = 0; d < Dm::DT; ++d) {
+      const int c = 16 * d + 4 * g;
+      if (c >= a.D) continue;
+      const f32x4 x = o[t][d] * a.scale;
+      if (a.nsplit > 1) {
+        *reinterpret_cast<f32x4*>(p + c) = x;
+      } else {
+        typedef T V4 __attribute__((ext_vector_type(4)));
+        V4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = (T)x[i];
+        *reinterpret_cast<V4*>((T*)a.dq + at_out + c) = v;
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ backward: dk, dv (walks over the rows)
+template <typename T, int DP, int KW>        // KW x 16 keys a wave
+__global__ __launch_bounds__(256) void k_xattn_dkv(XAttn a) {
+  using M = Mx<T>;
+  using Dm = Dims<T, DP>;
+  __shared__ __attribute__((aligned(16))) T sq[RR_XA_KT * Dm::PX];
+  __shared__ __attribute__((aligned(16))) T sg[RR_XA_KT * Dm::PX];
+  __shared__ float sl[RR_XA_KT], sd[RR_XA_KT];
+  __shared__ long long sm[RR_XA_KT];
+  __shared__ uint32_t flag[2];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
+  const Blk w = block_of(a);
+  const int R = a.G * a.Lq, H = a.G * a.Hk, key0 = (w.blk * 4 + wave) * 16 * KW;
+  const int seen = seen_keys(a, w.b);
+  const bool block_seen = w.blk * 64 * KW < seen;                          // (uniform in the workgroup)
+  const bool busy = key0 < seen;
+  const T* kp = (const T*)a.k + (long long)w.b * a.kb + (long long)w.hk * a.kh;
+  const T* vp = (const T*)a.v + (long long)w.b * a.vb + (long long)w.hk * a.vh;
+  const T* qp = (const T*)a.q + (long long)w.b * a.qb + (long long)w.hk * a.G * a.qh;
+  const T* gp = (const T*)a.dout + (long long)w.b * a.gb + (long long)w.hk * a.G * a.gh;
+  typename M::Frag kf[KW][Dm::NK], vf[KW][Dm::NK];
+#pragma unroll
+  for (int t = 0; t < KW; ++t) {
+    const int key = key0 + 16 * t + j;
+#pragma unroll
+    for (int k = 0; k < Dm::NK; ++k) {
+      const int c = k * M::KC + g * M::EPC;
+      const bool in = key < seen && c < a.D;
+      kf[t][k] = in ? frag_at<T>(kp + (long long)key * a.kl + c) : frag_zero<T>();
+      vf[t][k] = in ? frag_at<T>(vp + (long long)key * a.vl + c) : frag_zero<T>();
+    }
+  }
+  const float c2 = a.scale * RR_LOG2E;
+  const int first = w.split * a.tiles_per_split * RR_XA_KT;
+  int last = first + a.tiles_per_split * RR_XA_KT;
+  last = last < R ? last : R;
+  f32x4 ok[KW][Dm::DT], ov[KW][Dm::DT];
+  for (int pass = 0; pass < 2; ++pass) {
+    const bool safe = pass == 1;
+#pragma unroll
+    for (int t = 0; t < KW; ++t)
+#pragma unroll
+      for (int d = 0; d < Dm::DT; ++d) { ok[t][d] = rr_zero4(); ov[t][d] = rr_zero4(); }
+    for (int r0 = first; r0 < last && block_seen; r0 += RR_XA_KT) {
+      __syncthreads();
+      if (safe) {
+        if (threadIdx.x < 2) flag[threadIdx.x] = 0u;
+        __syncthreads();
+      }
+      stage<T, DP, Dm::PX>(sq, [&](int r) { const RowAt at = row_at(r, a.Lq, a.G); return qp + at.s * a.ql + at.g * a.qh; }, r0, R, a.D, safe, flag);
+      stage<T, DP, Dm::PX>(sg, [&](int r) { const RowAt at = row_at(r, a.Lq, a.G); return gp + at.s * a.gl + at.g * a.gh; }, r0, R, a.D, safe, flag);
+      if (threadIdx.x < RR_XA_KT) {
+        const int r = r0 + threadIdx.x;
+        const RowAt at = row_at(r < R ? r : R - 1, a.Lq, a.G);
+        const int head = w.hk * a.G + at.g;
+        const long long li = ((long long)w.b * H + head) * a.Lq + at.s;
+        sl[threadIdx.x] = r < R ? a.lse[li] * RR_LOG2E : 0.f;
+        sd[threadIdx.x] = r < R ? a.delta[li] : 0.f;
+        sm[threadIdx.x] = w.b * a.mb + head * a.mh + at.s * a.ml;
+      }
+      __syncthreads();
+      if (!busy) continue;
+#pragma unroll
+      for (int n = 0; n < 4; n += M::PT) {
+        f32x4 s[KW][M::PT], dp[KW][M::PT];
+#pragma unroll
+        for (int u = 0; u < M::PT; ++u) {
+#pragma unroll
+          for (int t = 0; t < KW; ++t) { s[t][u] = rr_zero4(); dp[t][u] = rr_zero4(); }
+#pragma unroll
+          for (int k = 0; k < Dm::NK; ++k) {
+            const typename M::Frag fq = frag_at<T>(sq + (16 * (n + u) + j) * Dm::PX + k * M::KC + g * M::EPC);
+            const typename M::Frag fg = frag_at<T>(sg + (16 * (n + u) + j) * Dm::PX + k * M::KC + g * M::EPC);
+#pragma unroll
+            for (int t = 0; t < KW; ++t) { s[t][u] = M::mma(fq, kf[t][k], s[t][u]); dp[t][u] = M::mma(fg, vf[t][k], dp[t][u]); }
+          }
+        }
+        typename M::Frag pf[KW], df[KW];
+#pragma unroll
+        for (int t = 0; t < KW; ++t) {
+          const int key = key0 + 16 * t + j;
+#pragma unroll
+          for (int u = 0; u < M::PT; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int rr = 16 * (n + u) + 4 * g + i;                     // row of the tile
+              bool see = key < seen && r0 + rr < R;
+              if (see && a.mask != nullptr) see = a.mask[sm[rr] + key] != 0;
+              float p = __builtin_amdgcn_exp2f(fmaf(s[t][u][i], c2, -sl[rr]));
+              if (safe && (flag[rr >> 5] >> (rr & 31) & 1u)) p = __builtin_nanf("");
+              const float d = p * (dp[t][u][i] - sd[rr]);
+              s[t][u][i] = see ? p : 0.f;
+              dp[t][u][i] = see ? d : 0.f;
+            }
+          pf[t] = M::pack(s[t]);
+          df[t] = M::pack(dp[t]);
+        }
+#pragma unroll
+        for (int d = 0; d < Dm::DT; ++d) {
+          const typename M::Frag fg = M::tr(sg, Dm::PX, 16 * n, 16 * d, lane);
+          const typename M::Frag fq = M::tr(sq, Dm::PX, 16 * n, 16 * d, lane);
+#pragma unroll
+          for (int t = 0; t < KW; ++t) { ov[t][d] = M::mma(fg, pf[t], ov[t][d]); ok[t][d] = M::mma(fq, df[t], ok[t][d]); }
+        }
+      }
+    }
+    bool bad = false;
+#pragma unroll
+    for (int t = 0; t < KW; ++t)
+#pragma unroll
+      for (int d = 0; d < Dm::DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bad |= is_bad(ok[t][d][i]) || is_bad(ov[t][d][i]);
+    if (!__syncthreads_or(bad && busy)) break;
+  }
+#pragma unroll
+  for (int t = 0; t < KW; ++t) {
+    const int key = key0 + 16 * t + j;
+    if (key >= a.Lk) continue;
+    const long long at_out = (((long long)w.b * a.Lk + key) * a.Hk + w.hk) * a.D;
+    const long long half = (long long)a.B * a.Lk * a.Hk * a.D;
+    float* p = a.part + (long long)w.split * 2 * half + at_out;
+#pragma unroll
+    for (int d = 0; d < Dm::DT; ++d) {
+      const int c = 16 * d + 4 * g;
+      if (c >= a.D) continue;
+      const f32x4 xk = ok[t][d] * a.scale, xv = ov[t][d];
+      if (a.nsplit > 1) {
+        *reinterpret_cast<f32x4*>(p + c) = xk;
+        *reinterpret_cast<f32x4*>(p + half + c) = xv;
+      } else {
+        typedef T V4 __attribute__((ext_vector_type(4)));
+        V4 vk, vv;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { vk[i] = (T)xk[i]; vv[i] = (T)xv[i]; }
+        *reinterpret_cast<V4*>((T*)a.dk + at_out + c) = vk;
+        *reinterpret_cast<V4*>((T*)a.dv + at_out + c) = vv;
+      }
+    }
+  }
+}
+
+// adds the splits' partial gradients in order: n values each, `stride` floats between the splits
+template <typename T>
+__global__ __launch_bounds__(256) void k_xattn_add(const float* __restrict__ part, long long stride, int nsplit, T* __restrict__ out, long long n4) {
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n4; i += (long long)gridDim.x * 256) {
+    f32x4 t = *reinterpret_cast<const f32x4*>(part + 4 * i);
+    for (int s = 1; s < nsplit; ++s) t += *reinterpret_cast<const f32x4*>(part + s * stride + 4 * i);
+    typedef T V4 __attribute__((ext_vector_type(4)));
+    V4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (T)t[e];
+    *reinterpret_cast<V4*>(out + 4 * i) = v;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+int xa_launched() { return hipGetLastError() == hipSuccess ? RR_OK : RR_ELAUNCH; }
+
+int head_pad(int D) { return D <= 16 ? 16 : D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+
+// rows (or keys) of a workgroup: 4 waves of 16 or 32
+struct Plan { int wide, nblk, nsplit, tiles_per_split; };
+Plan plan_for(long long kept, long long walked, long long outer) {
+  Plan p;
+  // 32 rows a wave read each staged tile half as often; 16 where that leaves less than a workgroup for each CU
+  p.wide = kept > 64 && outer * ((kept + 127) / 128) >= 256 ? 2 : 1;
+  p.nblk = (int)((kept + 64 * p.wide - 1) / (64 * p.wide));
+  const long long tiles = (walked + RR_XA_KT - 1) / RR_XA_KT;
+  const long long blocks = outer * p.nblk;
+  // few workgroups: the walked axis is split until about three fill each of the 256 CUs, four tiles a split at the least
+  long long split = blocks >= 512 ? 1 : (768 + blocks - 1) / blocks;
+  if (split > tiles / 4) split = tiles / 4;
+  if (split < 1) split = 1;
+  if (split > 256) split = 256;
+  p.tiles_per_split = (int)((tiles + split - 1) / split);
+  if (p.tiles_per_split < 1) p.tiles_per_split = 1;
+  p.nsplit = (int)((tiles + p.tiles_per_split - 1) / p.tiles_per_split);
+  if (p.nsplit < 1) p.nsplit = 1;
+  return p;
+}
+
+template <typename T, int DP>
+int fwd_go(XAttn& a, const Plan& p, hipStream_t st) {
+  const dim3 grid((unsigned)((long long)a.B * a.Hk * p.nsplit * p.nblk));
+  if (p.wide == 2) hipLaunchKernelGGL((k_xattn_fwd<T, DP, 2>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((k_xattn_fwd<T, DP, 1>), grid, dim3(256), 0, st, a);
+  if (p.nsplit > 1) hipLaunchKernelGGL((k_xattn_join<T, DP>), dim3((unsigned)(((long long)a.B * a.Hk * a.G * a.Lq + 3) / 4)), dim3(256), 0, st, a);
+  return xa_launched();
+}
+template <typename T, int DP>
+int bwd_go(XAttn& a, const Plan& p, const Plan& pk, hipStream_t st) {
+  const dim3 grid((unsigned)((long long)a.B * a.Hk * p.nsplit * p.nblk));
+  a.nsplit = p.nsplit; a.tiles_per_split = p.tiles_per_split; a.nblk = p.nblk;
+  if (p.wide == 2) hipLaunchKernelGGL((k_xattn_dq<T, DP, 2>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((k_xattn_dq<T, DP, 1>), grid, dim3(256), 0, st, a);
+  const long long nq4 = (long long)a.B * a.Lq * a.Hk * a.G * a.D / 4, nk4 = (long long)a.B * a.Lk * a.Hk * a.D / 4;
+  auto blocks = [](long long n) { return dim3((unsigned)(n / 256 + 1 < 4096 ? n / 256 + 1 : 4096)); };
+  if (p.nsplit > 1) hipLaunchKernelGGL((k_xattn_add<T>), blocks(nq4), dim3(256), 0, st, a.part, 4 * nq4, p.nsplit, (T*)a.dq, nq4);
+  a.nsplit = pk.nsplit; a.tiles_per_split = pk.tiles_per_split; a.nblk = pk.nblk;
+  const dim3 gk((unsigned)((long long)a.B * a.Hk * pk.nsplit * pk.nblk));
+  if (pk.wide == 2) hipLaunchKernelGGL((k_xattn_dkv<T, DP, 2>), gk, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((k_xattn_dkv<T, DP, 1>), gk, dim3(256), 0, st, a);
+  if (pk.nsplit > 1) {
+    hipLaunchKernelGGL((k_xattn_add<T>), blocks(nk4), dim3(256), 0, st, a.part, 8 * nk4, pk.nsplit, (T*)a.dk, nk4);
+    hipLaunchKernelGGL((k_xattn_add<T>), blocks(nk4), dim3(256), 0, st, a.part + 4 * nk4, 8 * nk4, pk.nsplit, (T*)a.dv, nk4);
+  }
+  return xa_launched();
+}
+
+struct Sizes { Plan q, k; size_t fwd, bwd; bool ok; };
+Sizes sizes_of(long long B, long long Lq, long long Lk, long long Hk, long long G, int D) {
+  Sizes s{};
+  const long long lim = 0x7fffffffLL;
+  // counts that index rows, keys and workgroups are 32-bit; offsets into the tensors are 64-bit
+  s.ok = B >= 1 && Lq >= 1 && Lk >= 0 && Hk >= 1 && G >= 1 && D >= 8 && D <= 128 && D % 8 == 0 && Lq <= lim && Lk <= lim - 256 && G * Lq <= lim - 256 && B <= lim && Hk <= lim &&
+         B * Hk <= lim && G * Hk <= lim;
+  if (!s.ok) return s;
+  s.q = plan_for(G * Lq, Lk, B * Hk);
+  s.k = plan_for(Lk > 0 ? Lk : 1, G * Lq, B * Hk);
+  if (B * Hk * s.q.nblk > lim / 256 || B * Hk * s.k.nblk > lim / 256 || B * Hk * G * Lq > lim) { s.ok = false; return s; }
+  const int DP = head_pad(D);
+  s.fwd = s.q.nsplit > 1 ? (size_t)(B * Hk * G * Lq) * s.q.nsplit * (DP + 4) * 4 : 0;
+  const size_t b1 = s.q.nsplit > 1 ? (size_t)s.q.nsplit * B * Lq * Hk * G * D * 4 : 0, b2 = s.k.nsplit > 1 ? (size_t)s.k.nsplit * 2 * B * Lk * Hk * D * 4 : 0;
+  s.bwd = b1 > b2 ? b1 : b2;
+  return s;
+}
+
+bool well_placed(const void* p, long long sb, long long sl, long long sh, int size) {
+  const int e = 16 / size;
+  return p != nullptr && rr_aligned16(p) && sb % e == 0 && sl % e == 0 && sh % e == 0;
+}
+
+}  // namespace
+
+typedef struct {
+  const void *q, *k, *v;
+  void* out;
+  float* lse;
+  const uint8_t* mask;
+  const void* kv_lens;
+  const void* dout;
+  float* delta;
+  void *dq, *dk, *dv;
+  void* workspace;
+  long long q_stride[3], k_stride[3], v_stride[3], mask_stride[3], dout_stride[3];
+  long long workspace_bytes;
+  int lens_int64, dtype, B, Lq, Lk, Hk, G, D;
+  float scale;
+} XAttnIO;
+
+static int xa_fill(const XAttnIO* io, XAttn& a, bool bwd) {
+  const int size = io->dtype == RR_F32 ? 4 : 2;
+  a = {};
+  if (io->dtype < 0 || io->dtype > 2 || !(io->scale > 0.f) || io->scale > 3.0e38f) return RR_EINVAL;
+  if (io->Lk > 0 && (!well_placed(io->k, io->k_stride[0], io->k_stride[1], io->k_stride[2], size) || !well_placed(io->v, io->v_stride[0], io->v_stride[1], io->v_stride[2], size)))
+    return RR_EINVAL;
+  if (!well_placed(io->q, io->q_stride[0], io->q_stride[1], io->q_stride[2], size) || io->out == nullptr || !rr_aligned16(io->out)) return RR_EINVAL;
+  if (bwd && (!well_placed(io->dout, io->dout_stride[0], io->dout_stride[1], io->dout_stride[2], size) || io->lse == nullptr || io->delta == nullptr ||
+              !rr_aligned16(io->dq) || !rr_aligned16(io->dk) || !rr_aligned16(io->dv) || io->dq == nullptr || (io->Lk > 0 && (io->dk == nullptr || io->dv == nullptr))))
+    return RR_EINVAL;
+  a.q = io->q; a.k = io->k; a.v = io->v; a.out = io->out; a.lse = io->lse; a.mask = io->mask; a.lens = io->kv_lens;
+  a.qb = io->q_stride[0]; a.ql = io->q_stride[1]; a.qh = io->q_stride[2];
+  a.kb = io->k_stride[0]; a.kl = io->k_stride[1]; a.kh = io->k_stride[2];
+  a.vb = io->v_stride[0]; a.vl = io->v_stride[1]; a.vh = io->v_stride[2];
+  a.mb = io->mask_stride[0]; a.mh = io->mask_stride[1]; a.ml = io->mask_stride[2];
+  a.gb = io->dout_stride[0]; a.gl = io->dout_stride[1]; a.gh = io->dout_stride[2];
+  a.lens64 = io->lens_int64; a.B = io->B; a.Lq = io->Lq; a.Lk = io->Lk; a.Hk = io->Hk; a.G = io->G; a.D = io->D;
+  a.scale = io->scale; a.part = (float*)io->workspace; a.dout = io->dout; a.delta = io->delta; a.dq = io->dq; a.dk = io->dk; a.dv = io->dv;
+  return RR_OK;
+}
+
+extern "C" long long rr_cross_attn_workspace(int B, int Lq, int Lk, int Hk, int G, int D, int backward) {
+  const Sizes s = sizes_of(B, Lq, Lk, Hk, G, D);
+  return s.ok ? (long long)(backward ? s.bwd : s.fwd) : -1;
+}
+
+#define RR_XA_BY_DIM(T, CALL)                                   \
+  switch (head_pad(io->D)) {                                    \
+    case 16: { constexpr int DP = 16; return CALL(T, DP); }     \
+    case 32: { constexpr int DP = 32; return CALL(T, DP); }     \
+    case 64: { constexpr int DP = 64; return CALL(T, DP); }     \
+    default: { constexpr int DP = 128; return CALL(T, DP); }    \
+  }
+
+extern "C" int rr_cross_attn(const XAttnIO* io, hipStream_t st) {
+  if (io == nullptr) return RR_EINVAL;
+  const Sizes s = sizes_of(io->B, io->Lq, io->Lk, io->Hk, io->G, io->D);
+  XAttn a;
+  if (!s.ok || xa_fill(io, a, false) != RR_OK || (s.fwd > 0 && (io->workspace == nullptr || (size_t)io->workspace_bytes < s.fwd || !rr_aligned16(io->workspace)))) return RR_EINVAL;
+  a.nsplit = s.q.nsplit; a.tiles_per_split = s.q.tiles_per_split; a.nblk = s.q.nblk;
+#define RR_CALL(T, DP) fwd_go<T, DP>(a, s.q, st)
+  if (io->dtype == RR_F32) { RR_XA_BY_DIM(float, RR_CALL) }
+  if (io->dtype == RR_F16) { RR_XA_BY_DIM(rr_f16, RR_CALL) }
+  RR_XA_BY_DIM(rr_bf16, RR_CALL)
+#undef RR_CALL
+}
+
+extern "C" int rr_cross_attn_bwd(const XAttnIO* io, hipStream_t st) {
+  if (io == nullptr || io->Lk < 1) return RR_EINVAL;
+  const Sizes s = sizes_of(io->B, io->Lq, io->Lk, io->Hk, io->G, io->D);
+  XAttn a;
+  if (!s.ok || xa_fill(io, a, true) != RR_OK || (s.bwd > 0 && (io->workspace == nullptr || (size_t)io->workspace_bytes < s.bwd || !rr_aligned16(io->workspace)))) return RR_EINVAL;
+#define RR_CALL(T, DP) bwd_go<T, DP>(a, s.q, s.k, st)
+  if (io->dtype == RR_F32) { RR_XA_BY_DIM(float, RR_CALL) }
+  if (io->dtype == RR_F16) { RR_XA_BY_DIM(rr_f16, RR_CALL) }
+  RR_XA_BY_DIM(rr_bf16, RR_CALL)
+#undef RR_CALL
+}

@@ -109,6 +109,12 @@ class MtvrpExtra(C.Structure):
     _fields_ = [(n, vp) for n in ("demand_b", "used_b", "open_route", "dist_limit", "bclass")]
 
 
+class XAttnIO(C.Structure):             # csrc/rr_xattn.hip
+    _fields_ = [(n, vp) for n in ("q", "k", "v", "out", "lse", "mask", "kv_lens", "dout", "delta", "dq", "dk", "dv", "workspace")] + \
+        [(n, C.c_longlong * 3) for n in ("q_stride", "k_stride", "v_stride", "mask_stride", "dout_stride")] + \
+        [("workspace_bytes", C.c_longlong)] + [(n, i32) for n in ("lens_int64", "dtype", "B", "Lq", "Lk", "Hk", "G", "D")] + [("scale", f32)]
+
+
 _SIGS = {
     "rr_minmax_normalize": [vp, vp, vp, vp, i32, i32, vp],
     "rr_atsp_step": [vp, vp, vp, vp, i32, i32, vp],
@@ -165,6 +171,12 @@ _SIGS = {
     "rr_mlp_wgrad": [C.POINTER(MlpWgradW), vp, vp, vp, vp, vp, vp, vp, i32, i32, C.c_longlong, vp, vp],
     "rr_mlp_wgrad16": [C.POINTER(MlpWgradW), vp, vp, vp, vp, vp, vp, vp, i32, i32, C.c_longlong, vp, vp],
     "rr_dec_attn_bwd": [C.POINTER(DecAttnIO), vp],
+    "rr_cross_attn": [C.POINTER(XAttnIO), vp],
+    "rr_cross_attn_bwd": [C.POINTER(XAttnIO), vp],
+    "rr_add_rms_norm": [i32, vp, C.c_longlong, vp, C.c_longlong, vp, i32, vp, vp, vp, vp, vp, C.c_longlong, i32, f32, vp],
+    "rr_add_rms_norm_parts": [C.c_longlong, i32],
+    "rr_add_rms_norm_bwd": [i32, vp, C.c_longlong, vp, C.c_longlong, vp, i32, vp, C.c_longlong, vp, C.c_longlong, vp, vp, vp, vp, i32,
+                            C.c_longlong, i32, vp],
 }
 
 _lib = None
@@ -185,6 +197,8 @@ def lib():
             fn.restype = i32
         _lib.rr_matnet_workspace_bytes.argtypes = [i32] * 4
         _lib.rr_matnet_workspace_bytes.restype = C.c_size_t
+        _lib.rr_cross_attn_workspace.argtypes = [i32] * 7
+        _lib.rr_cross_attn_workspace.restype = C.c_longlong
         if os.environ.get("RR_MARKERS", "0") == "1":
             _wrap_with_markers(_lib)
     return _lib
@@ -258,6 +272,29 @@ def ptr(t):
 
 def stream():
     return torch.cuda.current_stream().cuda_stream
+
+
+DTYPE_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}      # csrc/rr_types.h
+
+
+class on_device:
+    """`with on_device(t) as stream:` — launches go to the device that holds `t` and to its current stream."""
+
+    def __init__(self, t):
+        self.dev = t.device
+
+    def __enter__(self):
+        self.back = None
+        cur = torch.cuda.current_device()
+        if self.dev.index is not None and self.dev.index != cur:
+            torch.cuda.set_device(self.dev)
+            self.back = cur
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *exc):
+        if self.back is not None:
+            torch.cuda.set_device(self.back)
+        return False
 
 
 def check(rc, what):
