@@ -492,6 +492,15 @@ int rr_add_rms_norm_bwd(int dtype, const void* x, long long ldx, const void* res
                         long long lddy, const void* dh, long long lddh, const float* rstd, void* dx, void* dw, float* workspace, int parts,
                         long long rows, int E, hipStream_t stream);
 
+/* One choice a row from given random numbers (rrnco/models/decoding.py:37-63, 272-298, 311-361, with min-p and the numbers as an input): logits
+ * [R][V] of dtype by row stride, V <= 2^24; mask bytes [R][V] by row stride (0: one for all rows), 1 = may be drawn, or NULL; uniforms [R]
+ * in [0, 1).  temperature >= 0 (0: the largest logit, the lowest index among equals), top_k (0 off), top_p (0, 1 off), min_p (0 off)
+ * for all rows, or per row where row_* is not NULL.  -> index [R], logp [R] under the filtered distribution (index 0 and -inf where
+ * nothing may be drawn). */
+int rr_draw(int dtype, const void* logits, long long ld, const uint8_t* mask, long long ldm, const float* uniforms, int64_t* index, float* logp,
+            int R, int V, double temperature, int top_k, double top_p, double min_p, const float* row_temperature, const int* row_top_k,
+            const float* row_top_p, const float* row_min_p, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

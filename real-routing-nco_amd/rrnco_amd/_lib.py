@@ -171,6 +171,7 @@ _SIGS = {
     "rr_mlp_wgrad": [C.POINTER(MlpWgradW), vp, vp, vp, vp, vp, vp, vp, i32, i32, C.c_longlong, vp, vp],
     "rr_mlp_wgrad16": [C.POINTER(MlpWgradW), vp, vp, vp, vp, vp, vp, vp, i32, i32, C.c_longlong, vp, vp],
     "rr_dec_attn_bwd": [C.POINTER(DecAttnIO), vp],
+    "rr_draw": [i32, vp, C.c_longlong, vp, C.c_longlong, vp, vp, vp, i32, i32, C.c_double, i32, C.c_double, C.c_double, vp, vp, vp, vp, vp],
     "rr_cross_attn": [C.POINTER(XAttnIO), vp],
     "rr_cross_attn_bwd": [C.POINTER(XAttnIO), vp],
     "rr_add_rms_norm": [i32, vp, C.c_longlong, vp, C.c_longlong, vp, i32, vp, vp, vp, vp, vp, C.c_longlong, i32, f32, vp],

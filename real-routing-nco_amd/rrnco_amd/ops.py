@@ -6,6 +6,7 @@ import torch
 
 from .attention import cross_attention  # noqa: F401
 from .norms import add_rms_norm, add_rms_norm_fp8  # noqa: F401
+from .sampling import sample  # noqa: F401
 from .tensordict_lite import STATIC_KEYS, TensorDict
 
 

@@ -1,0 +1,203 @@
+"""rrnco_amd.ops.sample (csrc/rr_draw.hip) against the definition in 64 bits: choices have to be equal, log-probabilities within a rounding to float32.
+
+Tolerance of logp: half a step of float32 of its value (2^-24 |logp|) plus 2^-40 for what the two 64-bit evaluations and the summation order differ by."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+IDS = ["f32", "f16", "bf16"]
+
+
+def _ops():
+    from rrnco_amd import ops
+    return ops
+
+
+def reference_row(l, u, t, k, p, mp, allowed):
+    """One row by sorting, numpy float64: (index, logp, kept indices)."""
+    V = len(l)
+    ok = allowed & ~np.isnan(l) & (l != -np.inf)
+    if not ok.any():
+        return 0, -math.inf, np.array([], int)
+    ids = np.flatnonzero(ok)
+    v = l[ids]
+    top = v.max()
+    if not t > 0:
+        return int(ids[np.argmax(v)]), 0.0, ids[:0]
+    with np.errstate(invalid="ignore", over="ignore"):
+        z = np.where(v == top, 0.0, (v - top) / t)
+    w = np.exp(z)
+    kept = np.ones(len(v), bool)
+    if 0 < k < V and len(v) > k:
+        kept &= v >= np.sort(v)[::-1][k - 1]
+    if 0 < p < 1:
+        order = np.argsort(-v[kept], kind="stable")
+        vs, ws = v[kept][order], w[kept][order]
+        lim = p * ws.sum()
+        thr = top
+        for value in np.unique(vs):                                            # ascending: the smallest with less than lim strictly above
+            if ws[vs > value].sum() < lim:
+                thr = value
+                break
+        kept &= v >= thr
+    if mp > 0:
+        kept &= w >= min(mp, 1.0)
+    w = np.where(kept, w, 0.0)
+    cum = np.cumsum(w)
+    u = min(max(u, 0.0), 1 - 2.0 ** -53) if u == u else 0.0
+    over = np.flatnonzero((cum > u * cum[-1]) & (w > 0))
+    i = over[0] if len(over) else np.flatnonzero(w > 0)[-1]
+    return int(ids[i]), float(z[i] - np.log(w.sum())), ids[kept]
+
+
+def check(logits, u, mask=None, t=1.0, k=0, p=0.0, mp=0.0, rows=None):
+    idx, lp = _ops().sample(logits, u, temperature=t, top_k=k, top_p=p, min_p=mp, mask=mask)
+    R, V = logits.shape
+    x, un = logits.double().cpu().numpy(), u.double().cpu().numpy()
+    m = np.ones((R, V), bool) if mask is None else mask.expand(R, V).cpu().numpy()
+    at = lambda s, r: float(s.reshape(-1)[r]) if torch.is_tensor(s) else s         # noqa: E731
+    idx, lp = idx.cpu(), lp.cpu()
+    for r in rows if rows is not None else range(R):
+        i, want, _ = reference_row(x[r], un[r], at(t, r), int(at(k, r)), at(p, r), at(mp, r), m[r])
+        assert int(idx[r]) == i, (r, int(idx[r]), i)
+        got = float(lp[r])
+        assert got == want or abs(got - want) <= 2.0 ** -24 * abs(want) + 2.0 ** -40, (r, got, want)
+    return idx, lp
+
+
+def make(dt, R, V, seed=0, spread=3.0, masked=0.0):
+    g = torch.Generator("cuda").manual_seed(seed)
+    x = (spread * torch.randn(R, V, device="cuda", generator=g)).to(dt)
+    u = torch.rand(R, device="cuda", generator=g)
+    mask = None
+    if masked:
+        mask = torch.rand(R, V, device="cuda", generator=g) >= masked
+        mask[0] = False                                                            # a row with nothing left
+    return x, u, mask
+
+
+SIZES = [1, 2, 20, 63, 64, 65, 100, 128, 129, 257, 512, 1000, 1024, 1025, 2049, 5003, 8192, 8200, 20001, 70000]
+SETTINGS = [dict(), dict(t=0.7), dict(k=1), dict(k=5, t=1.3), dict(k=40), dict(p=0.9), dict(p=0.3, t=2.0), dict(mp=0.1), dict(k=40, p=0.9, mp=0.02, t=0.9), dict(t=0.0), dict(k=10 ** 6, p=1.0),
+            dict(p=0.999, k=3000)]
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+@pytest.mark.parametrize("V", SIZES)
+def test_choices_and_log_probabilities(dt, V):
+    R = 40 if V <= 1024 else 6
+    for n, s in enumerate(SETTINGS):
+        x, u, mask = make(dt, R, V, seed=V + n, masked=0.4 if n % 2 else 0.0)
+        check(x, u, mask, **s)
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+@pytest.mark.parametrize("V", [50, 700, 3000, 40000])
+def test_ties_and_flat_rows(dt, V):
+    """Rows of few distinct values (copies stay or go together), of one value, of two that a border separates exactly."""
+    g = torch.Generator("cuda").manual_seed(V)
+    x = torch.randint(0, 4, (8, V), device="cuda", generator=g).to(dt)
+    x[5], x[6], x[7] = 1.5, -2.0, 0.0
+    x[6, V // 3], x[7, ::2] = 4.0, -0.0
+    u = torch.rand(8, device="cuda", generator=g)
+    for s in (dict(), dict(k=3), dict(k=V // 2), dict(p=0.5), dict(p=0.9, k=V - 1), dict(mp=0.3), dict(mp=1.0), dict(t=0.0)):
+        check(x, u, **s)
+    two = torch.zeros(4, 2, device="cuda", dtype=dt)
+    check(two, torch.tensor([0.0, 0.4999, 0.5, 0.99], device="cuda"))
+    check(two, torch.tensor([0.0, 0.4999, 0.5, 0.99], device="cuda"), p=0.5)
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+@pytest.mark.parametrize("V", [30, 900, 2500, 30000])
+def test_non_finite_logits_and_random_numbers_at_the_ends(dt, V):
+    x, u, _ = make(dt, 8, V, seed=V)
+    x[0, 3], x[1, 5:9], x[2] = float("nan"), -float("inf"), -float("inf")
+    x[3, [4, 11]], x[4] = float("inf"), float("nan")
+    x[5, : V // 2] = torch.finfo(dt).min
+    x[6, 0] = -float("inf")
+    u[0], u[1], u[5], u[6], u[7] = 0.0, 1.0 - 2.0 ** -24, 0.0, 0.0, float("nan")
+    for s in (dict(), dict(k=4), dict(p=0.8), dict(mp=0.05), dict(t=0.0), dict(k=7, p=0.9, mp=0.01)):
+        idx, lp = check(x, u, **s)
+        assert int(idx[2]) == 0 and float(lp[2]) == -math.inf and int(idx[4]) == 0 and int(idx[3]) in (4, 11)
+    over = torch.tensor([1.0, 5.0, -1.0, float("inf"), -float("inf"), 1.0, 1.0, 1.0], device="cuda")
+    check(x, over, rows=[0, 1, 3, 5, 6, 7])
+
+
+@pytest.mark.parametrize("V", [100, 1001, 12000])
+def test_settings_of_each_row(V):
+    R = 24 if V < 5000 else 12
+    x, u, mask = make(torch.float32, R, V, seed=3, masked=0.3)
+    g = torch.Generator("cuda").manual_seed(9)
+    r = lambda: torch.rand(R, device="cuda", generator=g)                          # noqa: E731
+    t = 0.3 + r()
+    t[1], t[2], t[3] = 0.0, -1.0, float("nan")
+    k = (r() * 60).int()
+    k[4], k[5] = -3, 2 ** 30
+    p, mp = r(), 0.2 * r()
+    p[6], p[7], p[8], mp[9], mp[10] = 0.0, 1.0, 7.0, 3.0, -1.0
+    check(x, u, mask, t=t, k=k, p=p, mp=mp)
+    check(x, u, mask, t=t.double(), k=k.long(), p=0.8, mp=mp)
+
+
+def test_the_choices_follow_the_distribution():
+    """2^18 draws from one row of 50 keys: every frequency within 6 standard deviations of its probability."""
+    n = 1 << 18
+    x = (2 * torch.randn(50, device="cuda", generator=torch.Generator("cuda").manual_seed(1))).expand(n, 50)
+    u = torch.rand(n, device="cuda", generator=torch.Generator("cuda").manual_seed(2))
+    idx, lp = _ops().sample(x, u, top_k=20)
+    pr = torch.softmax(x[0].double().masked_fill(x[0] < x[0].topk(20).values[-1], -math.inf), 0)
+    f = torch.bincount(idx, minlength=50).double() / n
+    assert bool(((f - pr).abs() <= 6 * torch.sqrt(pr * (1 - pr) / n) + 1e-12).all()) and bool((f[pr == 0] == 0).all())
+    assert bool(((lp.double() - torch.log(pr[idx])).abs() < 1e-6).all())
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+def test_strides_masks_shapes_and_empty(dt):
+    ops = _ops()
+    for V in (90, 3001):
+        x, u, _ = make(dt, 12, 2 * V + 5, seed=V)
+        m = torch.rand(12, 2 * V + 5, device="cuda") < 0.6
+        m[:, 7] = True
+        for cut in (slice(3, 3 + V), slice(0, 2 * V, 2)):                          # rows of a wider tensor off the 16-byte grid; every second key
+            check(x[:, cut], u, m[:, cut], k=30, p=0.95)
+        check(x[:, :V], u, m[:1, :V], p=0.9)                                       # one mask for all rows
+        check(x[:1, :V].expand(12, V), u, None, k=4)
+    x = torch.randn(3, 4, 10, device="cuda").to(dt)
+    u = torch.rand(3, 4, device="cuda")
+    i, lp = ops.sample(x, u, mask=torch.ones(4, 10, dtype=torch.bool, device="cuda"))
+    assert i.shape == lp.shape == (3, 4)
+    i, lp = ops.sample(x[0, 0], u[0, 0])
+    assert i.shape == ()
+    i, lp = ops.sample(x[:0], u[:0])
+    assert i.shape == lp.shape == (0, 4)
+
+
+def test_same_choices_on_another_stream_and_in_a_graph():
+    ops = _ops()
+
+    def draw(x, u, m, long, ul):
+        return [*ops.sample(x, u, top_k=30, top_p=0.9, mask=m), *ops.sample(long, ul, top_p=0.9), *ops.sample(long, ul, top_k=50)]
+    x, u, m = make(torch.float32, 300, 500, seed=1, masked=0.5)
+    long, ul, _ = make(torch.bfloat16, 5, 50000, seed=2)
+    first = draw(x, u, m, long, ul)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        assert all(torch.equal(a, b) for a, b in zip(first, draw(x, u, m, long, ul)))
+    torch.cuda.current_stream().wait_stream(side)
+    held_in = [t.clone() for t in (x, u, m, long, ul)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = draw(*held_in)
+    for i in range(4):
+        nx, nu, nm = make(torch.float32, 300, 500, seed=40 + i, masked=0.5)
+        nl, nul, _ = make(torch.bfloat16, 5, 50000, seed=60 + i)
+        for a, b in zip(held_in, (nx, nu, nm, nl, nul)):
+            a.copy_(b)
+        graph.replay()
+        eager = draw(nx, nu, nm, nl, nul)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, eager)), i
