@@ -499,7 +499,8 @@ int rr_add_rms_norm_bwd(int dtype, const void* x, long long ldx, const void* res
  * nothing may be drawn). */
 int rr_draw(int dtype, const void* logits, long long ld, const uint8_t* mask, long long ldm, const float* uniforms, int64_t* index, float* logp,
             int R, int V, double temperature, int top_k, double top_p, double min_p, const float* row_temperature, const int* row_top_k,
-            const float* row_top_p, const float* row_min_p, hipStream_t stream);
+            const float* row_top_p, const float* row_min_p, void* workspace, long long workspace_bytes, hipStream_t stream);
+long long rr_draw_workspace(int R, int V);      /* bytes (0 for most sizes) */
 
 #ifdef __cplusplus
 }

@@ -13,9 +13,10 @@
 //
 // Up to 1 024 keys: a wave a row, its keys in registers.  The k-th largest by bisection over the bit patterns that the row's extremes
 // leave open (one ballot a register and step); what it keeps, where it fits one register a lane, moves together, in index order, so that
-// only kept keys pay for their 64-bit exponential.  Longer rows: a workgroup a row that walks the row several times (it stays in
-// the L2): a histogram over the distance from the maximum, then only the keys of the bin that holds the border are looked at.  The
-// histogram's masses are 64-bit integers in steps of 2^-45 (atomics on integers: the order does not matter).
+// only kept keys pay for their 64-bit weight.  Longer rows: a workgroup a row, its keys in registers up to 16 384: a histogram over the
+// distance from the maximum, then only the keys of the bin that holds the border are looked at.  Masses there are 64-bit whole numbers of steps
+// of 2^-45, so that atomics may add them in any order.  Few rows beyond that: a workgroup for every 16 384 keys, five launches (below).
+// Bound by the 64-bit arithmetic (some 20 instructions a weight), not by the one read of the logits.
 #include "rr_types.h"
 
 namespace {
@@ -28,17 +29,18 @@ struct Draw {
   float* logp;
   const float *pt, *pp, *pm;           // per-row temperature, top_p, min_p, or NULL: the scalars
   const int* pk;
-  double t, p, mp;
+  double t, c2, p, mp;
   long long ld, ldm;
   int k, R, V;
 };
 
-struct Par { double t, p, mp, u; int k; bool greedy; };
+struct Par { double t, c2, p, mp, u; int k; bool greedy; };
 __device__ __forceinline__ Par par_of(const Draw& a, int r) {
   Par q;
   const double t = a.pt ? (double)a.pt[r] : a.t;
   q.greedy = !(t > 0.0);                                       // 0 (and whatever is no temperature): the largest logit
   q.t = t;
+  q.c2 = a.pt ? 1.44269504088896340736 / t : a.c2;                           // weight of a key: 2^((l - max) c2)
   q.k = a.pk ? a.pk[r] : a.k;
   q.p = a.pp ? (double)a.pp[r] : a.p;
   q.mp = a.pm ? (double)a.pm[r] : a.mp;
@@ -54,31 +56,92 @@ __device__ __forceinline__ uint32_t key_of(float l, bool ok) {           // orde
   return ok && l == l && k > 0x007fffffu ? k : 0u;
 }
 __device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k); }
-__device__ __forceinline__ double z_of(uint32_t k, uint32_t top, double t) { return k == top ? 0.0 : ((double)value_of(k) - (double)value_of(top)) / t; }
+__device__ __forceinline__ double z_of(uint32_t k, uint32_t top, double c2) { return k == top ? 0.0 : ((double)value_of(k) - (double)value_of(top)) * (c2 * 0.69314718055994530942); }
+__device__ __forceinline__ double pow2_of(double f) {
+  double p = 4.4455382718708109e-10;
+  p = fma(p, f, 7.0549116208011225e-09);
+  p = fma(p, f, 1.0178086009239699e-07);
+  p = fma(p, f, 1.3215486790144307e-06);
+  p = fma(p, f, 1.5252733804059841e-05);
+  p = fma(p, f, 1.5403530393381608e-04);
+  p = fma(p, f, 1.3333558146428443e-03);
+  p = fma(p, f, 9.6181291076284769e-03);
+  p = fma(p, f, 5.5504108664821576e-02);
+  p = fma(p, f, 2.4022650695910069e-01);
+  p = fma(p, f, 6.9314718055994529e-01);
+  return fma(p, f, 1.0);
+}
+// w = 2^((l - max) c2) to 1e-14: the exponent's nearest whole number goes to ldexp, 2^f on [-1/2, 1/2] is its Taylor series (ln 2)^n / n! f^n up to
+// n = 11 (the next term is 6e-15).  About 20 instructions; the library's exp with the division by T took three times that.
+__device__ __forceinline__ double weight_of(uint32_t k, uint32_t top, double topd, double c2) {
+  double t = ((double)value_of(k) - topd) * c2;
+  t = t > -2000.0 ? t : -2000.0;                               // under the smallest number: 0, also for what an infinite maximum leaves
+  const double n = __builtin_rint(t);
+  const double w = ldexp(pow2_of(t - n), (int)n);
+  return k == top ? 1.0 : w;
+}
 
-// ---- wave helpers
+// ---- wave helpers on DPP: 16-lane rows by shifts, rows joined by broadcasts; lane 63 then holds the whole wave
+#define RR_DPP(v, old, ctrl, rows) __builtin_amdgcn_update_dpp((int)(old), (int)(v), ctrl, rows, 0xf, false)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_d(double v) {                      // 0 where there is no source lane
+  const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+  const uint32_t lo = (uint32_t)RR_DPP((uint32_t)b, 0, CTRL, ROWS), hi = (uint32_t)RR_DPP((uint32_t)(b >> 32), 0, CTRL, ROWS);
+  return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_scan_d(double v) {                // inclusive
+  v += dpp_d<0x111, 0xf>(v);
+  v += dpp_d<0x112, 0xf>(v);
+  v += dpp_d<0x114, 0xf>(v);
+  v += dpp_d<0x118, 0xf>(v);
+  v += dpp_d<0x142, 0xa>(v);
+  v += dpp_d<0x143, 0xc>(v);
+  return v;
+}
+__device__ __forceinline__ double last_lane_d(double v) {
+  const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, 63), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), 63);
+  return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum_d(double v) { return last_lane_d(wave_scan_d(v)); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t v) { const uint32_t x = (uint32_t)RR_DPP(v, 0, CTRL, ROWS); return v > x ? v : x; }
 __device__ __forceinline__ uint32_t wave_max_u(uint32_t v) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) { const uint32_t x = __shfl_xor(v, o); v = v > x ? v : x; }
-  return v;
+  v = dpp_max<0x111, 0xf>(v);
+  v = dpp_max<0x112, 0xf>(v);
+  v = dpp_max<0x114, 0xf>(v);
+  v = dpp_max<0x118, 0xf>(v);
+  v = dpp_max<0x142, 0xa>(v);
+  v = dpp_max<0x143, 0xc>(v);
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
-__device__ __forceinline__ uint32_t wave_min_u(uint32_t v) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) { const uint32_t x = __shfl_xor(v, o); v = v < x ? v : x; }
-  return v;
+__device__ __forceinline__ uint32_t wave_min_u(uint32_t v) { return ~wave_max_u(~v); }
+
+// log(x), x >= 1: the 32-bit logarithm is off by less than 1e-6 and one step x e^-y - 1 = d, log x = y + d - d^2 / 2, leaves d^3 / 3
+__device__ __forceinline__ double log_of(double x) {
+  const double y2 = (double)__log2f((float)x);
+  const double n = __builtin_rint(y2), f = n - y2;
+  const double d = fma(x, ldexp(pow2_of(f), -(int)n), -1.0);
+  return y2 * 0.69314718055994530942 + (d - 0.5 * d * d);
 }
-__device__ __forceinline__ double wave_sum_d(double v) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
-  return v;
+
+__device__ __forceinline__ double wave_total(double v) { return wave_sum_d(v); }
+__device__ __forceinline__ uint32_t wave_total(uint32_t v) {
+#define RR_ADD(CTRL, ROWS) v += (uint32_t)RR_DPP(v, 0, CTRL, ROWS)
+  RR_ADD(0x111, 0xf); RR_ADD(0x112, 0xf); RR_ADD(0x114, 0xf); RR_ADD(0x118, 0xf); RR_ADD(0x142, 0xa); RR_ADD(0x143, 0xc);
+#undef RR_ADD
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
-__device__ __forceinline__ double wave_scan_d(double v, int lane) {      // inclusive
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double x = __shfl_up(v, o);
-    if (lane >= o) v += x;
-  }
-  return v;
+__device__ __forceinline__ unsigned long long wave_total(unsigned long long v) {
+#define RR_ADD(CTRL, ROWS) v += (unsigned long long)(uint32_t)RR_DPP((uint32_t)(v >> 32), 0, CTRL, ROWS) << 32 | (uint32_t)RR_DPP((uint32_t)v, 0, CTRL, ROWS)
+  RR_ADD(0x111, 0xf); RR_ADD(0x112, 0xf); RR_ADD(0x114, 0xf); RR_ADD(0x118, 0xf); RR_ADD(0x142, 0xa); RR_ADD(0x143, 0xc);
+#undef RR_ADD
+  return (unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+__device__ __forceinline__ void wave_lds() {                             // LDS written by a lane of this wave may be read by another from here on
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 template <int E>
@@ -88,6 +151,13 @@ __device__ __forceinline__ int count_ge(const uint32_t (&key)[E], uint32_t at) {
   for (int q = 0; q < E; ++q) n += __popcll(__ballot(key[q] >= at));
   return n;
 }
+// a bit pattern between two (lo < hi, both of finite values), by value: halving patterns would spend its steps on the exponents around zero
+__device__ __forceinline__ uint32_t between(uint32_t lo, uint32_t hi, int step) {
+  const uint32_t half = lo + ((hi - lo) >> 1);
+  const uint32_t k = key_of(0.5f * value_of(lo) + 0.5f * value_of(hi), true);
+  return (step & 3) == 3 || k < lo || k >= hi ? half : k;                // (every fourth by pattern: at most 4 x 32 steps whatever the values)
+}
+
 // the k-th largest of the wave's keys (k <= their number), top = the largest
 template <int E>
 __device__ __forceinline__ uint32_t kth_largest(const uint32_t (&key)[E], int k, uint32_t top) {
@@ -96,8 +166,8 @@ __device__ __forceinline__ uint32_t kth_largest(const uint32_t (&key)[E], int k,
   for (int q = 0; q < E; ++q) low = key[q] && key[q] < low ? key[q] : low;
   low = wave_min_u(low);
   uint32_t lo = low, hi = top;                                           // count(>= lo) >= k always holds; hi: the answer is <= hi
-  while (lo < hi) {                                                      // (uniform; at most 32 halvings)
-    const uint32_t mid = lo + ((hi - lo) >> 1) + 1u;
+  for (int step = 0; lo < hi; ++step) {
+    const uint32_t mid = between(lo, hi, step) + 1u;
     const int n = count_ge(key, mid);
     if (n >= k) lo = mid; else hi = mid - 1u;
     if (n == k) {                                                        // exactly k keys from mid on: the smallest of them
@@ -110,33 +180,63 @@ __device__ __forceinline__ uint32_t kth_largest(const uint32_t (&key)[E], int k,
   return lo;
 }
 
-// keys (0: none) of one row in index order: register-major, lane-minor; idx of a register's key.  Writes the choice.
+// The threshold of top-p among a wave's keys and weights: the smallest value with less than `lim` of mass strictly above it, `above` of which is
+// outside these keys (all larger).  Weights of 64-bit floats or of whole steps.
+template <int E, typename W>
+__device__ __forceinline__ uint32_t mass_threshold(const uint32_t (&key)[E], const W (&w)[E], uint32_t top, W above, double lim, uint32_t* skey, W* sw, int lane) {
+  uint32_t low = top;
+#pragma unroll
+  for (int e = 0; e < E; ++e) low = key[e] && key[e] < low ? key[e] : low;
+  uint32_t lo = wave_min_u(low), hi = top;                               // mass(> hi) < lim holds
+  for (int step = 0; lo < hi; ++step) {
+    const uint32_t mid = between(lo, hi, step);
+    W m = 0;
+    int n = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) m += key[e] > mid ? w[e] : W(0);
+    m = above + wave_total(m);
+    if ((double)m < lim) hi = mid; else lo = mid + 1u;
+    // one value between the ends: the next key from lo on is the threshold
+#pragma unroll
+    for (int e = 0; e < E; ++e) n += __popcll(__ballot(key[e] >= lo && key[e] <= hi));
+    if (n <= 1) break;
+    if constexpr (E > 1) {
+      if (n <= 64) {                                                     // few left: one a lane, what lies above them is summed once
+        W over = 0;
+        int base = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const bool in = key[e] >= lo && key[e] <= hi;
+          const unsigned long long b = __ballot(in);
+          const int at = base + __popcll(b & ((1ull << lane) - 1ull));
+          if (in) { skey[at] = key[e]; sw[at] = w[e]; }
+          base += __popcll(b);
+          over += key[e] > hi ? w[e] : W(0);
+        }
+        wave_lds();
+        const uint32_t k1[1] = {lane < n ? skey[lane] : 0u};
+        const W w1[1] = {lane < n ? sw[lane] : W(0)};
+        wave_lds();
+        return mass_threshold<1, W>(k1, w1, wave_max_u(k1[0]), above + wave_total(over), lim, skey, sw, lane);
+      }
+    }
+  }
+  return lo;
+}
+
+// keys (0: none) of one row in index order: register-major, lane-minor; idx of a register's key; whole: the mass that top-p refers to (below 0: that of these
+// keys).  Writes the choice.
 template <int E, typename IDX>
-__device__ __forceinline__ void choose(const Draw& a, const Par& q, int r, uint32_t (&key)[E], IDX idx, uint32_t top, int lane) {
+__device__ __forceinline__ void choose(const Draw& a, const Par& q, int r, uint32_t (&key)[E], IDX idx, uint32_t top, double whole, uint32_t* skey, double* sw, int lane) {
+  const double topd = (double)value_of(top);
   double w[E], z = 0.0;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    w[e] = key[e] ? exp(z_of(key[e], top, q.t)) : 0.0;
+    w[e] = key[e] ? weight_of(key[e], top, topd, q.c2) : 0.0;
     z += w[e];
   }
   if (q.p > 0.0 && q.p < 1.0) {
-    const double lim = q.p * wave_sum_d(z);
-    uint32_t low = top;
-#pragma unroll
-    for (int e = 0; e < E; ++e) low = key[e] && key[e] < low ? key[e] : low;
-    uint32_t lo = wave_min_u(low), hi = top;                             // the smallest value with less than lim strictly above it: mass(> top) = 0
-    while (lo < hi) {
-      const uint32_t mid = lo + ((hi - lo) >> 1);
-      double m = 0.0;
-      int n = 0;
-#pragma unroll
-      for (int e = 0; e < E; ++e) m += key[e] > mid ? w[e] : 0.0;
-      if (wave_sum_d(m) < lim) hi = mid; else lo = mid + 1u;
-      // no key left between the two ends but one value: the next key from lo on is the threshold
-#pragma unroll
-      for (int e = 0; e < E; ++e) n += __popcll(__ballot(key[e] >= lo && key[e] <= hi));
-      if (n <= 1) break;
-    }
+    const uint32_t lo = mass_threshold<E, double>(key, w, top, 0.0, q.p * (whole < 0.0 ? wave_sum_d(z) : whole), skey, sw, lane);
 #pragma unroll
     for (int e = 0; e < E; ++e)
       if (key[e] < lo) { key[e] = 0u; w[e] = 0.0; }
@@ -147,36 +247,45 @@ __device__ __forceinline__ void choose(const Draw& a, const Par& q, int r, uint3
     if (q.mp > 0.0 && w[e] < q.mp) w[e] = 0.0;
     z += w[e];
   }
-  double part[E], total = 0.0;                                           // a register's mass, in index order
+  // running sums in index order: two registers are scanned at once; of more, their masses tell the register and only that one is scanned.
+  // rounding may leave the target at the very end: then the last key with a weight is taken
+  double total = 0.0, cum = 0.0, we = w[0];
+  uint32_t ke = key[0];
+  int ie = idx(0);
+  bool over = false;
   if constexpr (E == 1) {
-    part[0] = total = wave_sum_d(w[0]);
+    cum = wave_scan_d(we);
+    total = last_lane_d(cum);
+  } else if constexpr (E == 2) {
+    const double c0 = wave_scan_d(w[0]), c1 = wave_scan_d(w[1]), t0 = last_lane_d(c0), t1 = last_lane_d(c1);
+    total = t0 + t1;
+    const bool first = t0 > q.u * total || t1 == 0.0;
+    cum = first ? c0 : t0 + c1;
+    if (!first) { we = w[1]; ke = key[1]; ie = idx(1); }
   } else {
+    double part[E], before = 0.0, base = 0.0;
 #pragma unroll
     for (int e = 0; e < E; ++e) { part[e] = wave_sum_d(w[e]); total += part[e]; }
-  }
-  const double target = q.u * total;
-  // the register that the target falls in, then the lane; rounding may leave the target at the very end: the last key with a weight
-  double before = 0.0, base = 0.0, we = 0.0;
-  int reg = -1, last = -1;
+    int reg = -1, last = 0;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    if (part[e] > 0.0) last = e;
-    if (reg < 0 && before + part[e] > target) { reg = e; base = before; }
-    before += part[e];
-  }
-  const bool over = reg < 0;
-  if (over) reg = last;
-  uint32_t ke = 0u;
-  int ie = 0;
+    for (int e = 0; e < E; ++e) {
+      if (part[e] > 0.0) last = e;
+      if (reg < 0 && before + part[e] > q.u * total) { reg = e; base = before; }
+      before += part[e];
+    }
+    over = reg < 0;
+    if (over) reg = last;
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (e == reg) { we = w[e]; ke = key[e]; ie = idx(e); }
-  const double cum = base + wave_scan_d(we, lane);
-  const unsigned long long hit = __ballot(!over && we > 0.0 && cum > target), any = __ballot(we > 0.0);
+    for (int e = 1; e < E; ++e)
+      if (e == reg) { we = w[e]; ke = key[e]; ie = idx(e); }
+    cum = base + wave_scan_d(we);
+  }
+  const unsigned long long hit = __ballot(!over && we > 0.0 && cum > q.u * total), any = __ballot(we > 0.0);
   const int at = hit ? __ffsll((unsigned long long)hit) - 1 : 63 - __clzll((long long)any);
+  const float lp = (float)(z_of(ke, top, q.c2) - log_of(total));
   if (lane == at) {
     a.index[r] = ie;
-    a.logp[r] = (float)(z_of(ke, top, q.t) - log(total));
+    a.logp[r] = lp;
   }
 }
 
@@ -184,6 +293,7 @@ template <typename T, int E>
 __global__ __launch_bounds__(256) void k_draw_wave(Draw a) {
   __shared__ uint32_t skey[E > 1 ? 4 : 1][64];
   __shared__ int sidx[E > 1 ? 4 : 1][64];
+  __shared__ double sw[E > 1 ? 4 : 1][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = blockIdx.x * 4 + wave;
   if (r >= a.R) return;                                                  // (no workgroup barrier below)
   const T* row = (const T*)a.logits + (long long)r * a.ld;
@@ -228,74 +338,70 @@ __global__ __launch_bounds__(256) void k_draw_wave(Draw a) {
           if (key[e]) { skey[wave][at] = key[e]; sidx[wave][at] = lane + 64 * e; }
           base += __popcll(b);
         }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        wave_lds();
         uint32_t k1[1] = {lane < n ? skey[wave][lane] : 0u};
         const int i1 = lane < n ? sidx[wave][lane] : 0;
-        choose<1>(a, q, r, k1, [&](int) { return i1; }, top, lane);
+        choose<1>(a, q, r, k1, [&](int) { return i1; }, top, -1.0, nullptr, nullptr, lane);
         return;
       }
     }
   }
-  choose<E>(a, q, r, key, [&](int e) { return lane + 64 * e; }, top, lane);
+  choose<E>(a, q, r, key, [&](int e) { return lane + 64 * e; }, top, -1.0, skey[E > 1 ? wave : 0], sw[E > 1 ? wave : 0], lane);
 }
 
 // ------------------------------------------------------------------------------------------------ long rows
 #define RR_DRAW_BINS 1024
-#define RR_DRAW_LIST 4096
+#define RR_DRAW_LIST 2048
 #define RR_DRAW_STEP 35184372088832.0          // 2^45 steps a unit of weight
+#define RR_DRAW_NT 1024                        // the split form's workgroups, and the keys of its stretches
+#define RR_DRAW_STRETCH 16384
 
 // bin of a key: its distance from the maximum in steps of T / 32 (monotone in the key), the last bin open
 __device__ __forceinline__ int bin_of(uint32_t k, float topv, float per) {
-  const float d = (topv - value_of(k)) * per;
-  return d < (float)(RR_DRAW_BINS - 1) ? (int)d : (k && value_of(k) == topv ? 0 : RR_DRAW_BINS - 1);
+  const float v = value_of(k), d = (topv - v) * per;
+  return d < (float)(RR_DRAW_BINS - 1) ? (int)d : (v == topv ? 0 : RR_DRAW_BINS - 1);
 }
-__device__ __forceinline__ unsigned long long steps_of(double w) { return (unsigned long long)__double2ll_rn(w * RR_DRAW_STEP); }
+__device__ __forceinline__ unsigned long long steps_of(double w) {       // w <= 1: w 2^45 + 2^52 holds the whole number in its low bits
+  return __builtin_bit_cast(unsigned long long, fma(w, RR_DRAW_STEP, 4503599627370496.0)) & 0xfffffffffffffull;
+}
 
-template <typename T, int NT, bool VECTOR>
-struct Row {
-  static constexpr int VEC = VECTOR ? rr_vec_of<T>::N : 1, NW = NT / 64, PIECE = 64 * VEC;
-  const T* row;
-  const uint8_t* mask;
-  int V, lane, wave, per_wave;                                           // pieces of a wave's stretch of the row
-  __device__ __forceinline__ Row(const Draw& a, int r) {
-    row = (const T*)a.logits + (long long)r * a.ld;
-    mask = a.mask ? a.mask + (long long)r * a.ldm : nullptr;
-    V = a.V; lane = threadIdx.x & 63; wave = threadIdx.x >> 6;
-    per_wave = ((V + PIECE - 1) / PIECE + NW - 1) / NW;
-  }
-  __device__ __forceinline__ void load(int i0, uint32_t (&key)[VEC]) const {
-    float x[VEC];
-    if (i0 + VEC <= V) {
-      rr_load_n<T, VEC>(row + i0, x);
-      uint8_t m[VEC];
+// E keys a thread of NT * E consecutive ones from `base` on: piece-major, then thread, VEC keys each (index order within each level)
+template <typename T, int NT, int E, bool VECTOR>
+struct Keys {
+  static constexpr int VEC = VECTOR ? rr_vec_of<T>::N : 1, P = E / VEC, N = NT * E;
+  uint32_t key[E];
+  int base;
+  __device__ __forceinline__ int index(int e) const { return base + (e / VEC * NT + (int)threadIdx.x) * VEC + e % VEC; }
+  __device__ __forceinline__ void load(const T* row, const uint8_t* mask, int from, int V) {
+    base = from;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) m[i] = 1;
-      if (mask != nullptr) __builtin_memcpy(m, mask + i0, VEC);
+    for (int p = 0; p < P; ++p) {
+      const int i0 = base + (p * NT + (int)threadIdx.x) * VEC;
+      if (i0 + VEC <= V) {
+        float x[VEC];
+        uint8_t m[VEC];
+        rr_load_n<T, VEC>(row + i0, x);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) key[i] = key_of(x[i], m[i] != 0);
-    } else {
+        for (int i = 0; i < VEC; ++i) m[i] = 1;
+        if (mask != nullptr) __builtin_memcpy(m, mask + i0, VEC);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) key[i] = i0 + i < V ? key_of((float)row[i0 + i], mask == nullptr || mask[i0 + i] != 0) : 0u;
+        for (int i = 0; i < VEC; ++i) key[p * VEC + i] = key_of(x[i], m[i] != 0);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) key[p * VEC + i] = i0 + i < V ? key_of((float)row[i0 + i], mask == nullptr || mask[i0 + i] != 0) : 0u;
+      }
     }
   }
   template <typename F>
-  __device__ __forceinline__ void walk(F f) const {                      // f(key, index) for this lane's keys of its wave's stretch, in index order
-    for (int p = wave * per_wave; p < (wave + 1) * per_wave && p * PIECE < V; ++p) {
-      uint32_t key[VEC];
-      const int i0 = p * PIECE + lane * VEC;
-      load(i0, key);
+  __device__ __forceinline__ void each(F f) const {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) f(key[i], i0 + i);
-    }
+    for (int e = 0; e < E; ++e) f(key[e], index(e));
   }
 };
 
 template <int NT, typename V>
 __device__ __forceinline__ V block_sum(V v, V* red) {                    // every thread gets the sum, added in a fixed order
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
+  v = wave_total(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -316,14 +422,15 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {
   return t;
 }
 
-// the first bin, from the top, at which the running sum of h reaches `need` (>= for counts, and for masses where need > 0): its number and the
-// sum before it.  RR_DRAW_BINS where it is never reached.
-template <int NT, typename V, typename R>
-__device__ __forceinline__ void find_bin(const V* h, double need, R* red, int* found, V* above) {
-  constexpr int PER = RR_DRAW_BINS / NT > 0 ? RR_DRAW_BINS / NT : 1;
+// the first bin, from the top, at which the running sum of h reaches `need` (> 0): its number and the sum before it (RR_DRAW_BINS where it is never reached)
+template <int NT, typename V>
+__device__ __forceinline__ void find_bin(const V* h, double need, V* red, int* found, V* above) {
+  constexpr int PER = RR_DRAW_BINS / NT;
+  static_assert(PER >= 1, "a bin for each thread");
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b0 = threadIdx.x * PER;
   V mine = 0;
-  for (int i = 0; i < PER; ++i) mine += b0 + i < RR_DRAW_BINS ? h[b0 + i] : 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) mine += h[b0 + i];
   V run = mine;                                                          // inclusive over the wave
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -336,7 +443,7 @@ __device__ __forceinline__ void find_bin(const V* h, double need, R* red, int* f
   __syncthreads();
   V base = run - mine;
   for (int i = 0; i < wave; ++i) base += red[i];
-  for (int i = 0; i < PER && b0 + i < RR_DRAW_BINS; ++i) {
+  for (int i = 0; i < PER; ++i) {
     const V next = base + h[b0 + i];
     if ((double)base < need && (double)next >= need) { *found = b0 + i; *above = base; }      // one thread at the most: sums do not fall
     base = next;
@@ -344,179 +451,701 @@ __device__ __forceinline__ void find_bin(const V* h, double need, R* red, int* f
   __syncthreads();
 }
 
-template <typename T, int NT, bool VECTOR>
-__global__ __launch_bounds__(NT) void k_draw_row(Draw a) {
-  using Rw = Row<T, NT, VECTOR>;
-  constexpr int NW = NT / 64;
-  __shared__ unsigned long long mass[RR_DRAW_BINS];
-  __shared__ uint32_t cnt[RR_DRAW_BINS];
-  __shared__ uint32_t list[RR_DRAW_LIST];
-  __shared__ double redd[NW];
-  __shared__ unsigned long long redm[NW];
-  __shared__ uint32_t redu[NW];
-  __shared__ int found, nlist;
-  __shared__ unsigned long long above_m;
-  __shared__ uint32_t above_c;
-  const int r = blockIdx.x;
-  const Rw row(a, r);
-  const Par q = par_of(a, r);
-  uint32_t top = 0u;
-  int ntop = 0;
-  row.walk([&](uint32_t k, int) { top = k > top ? k : top; ntop += k != 0u; });
-  top = block_max<NT>(top, redu);
-  if (top == 0u) {
-    if (threadIdx.x == 0) { a.index[r] = 0; a.logp[r] = -INFINITY; }
-    return;
+template <int NT, int LIST>
+struct Scratch {
+  static constexpr int LISTED = LIST;
+  unsigned long long mass[RR_DRAW_BINS];
+  uint32_t cnt[RR_DRAW_BINS];
+  uint32_t list[LIST];
+  double part[512], redd[NT / 64];
+  unsigned long long redm[NT / 64], above_m;
+  uint32_t redu[NT / 64], above_c;
+  int found, nlist;
+};
+
+// what the thresholds leave of a key's weight
+struct Kept {
+  uint32_t top, cut;
+  double topd, c2, mp;
+  __device__ __forceinline__ double operator()(uint32_t k) const {
+    if (k < cut || k == 0u) return 0.0;
+    const double w = weight_of(k, top, topd, c2);
+    return w < mp ? 0.0 : w;
   }
-  if (q.greedy) {
-    uint32_t best = 0u;                                                  // ~index: the largest is the lowest index
-    row.walk([&](uint32_t k, int i) { if (k == top && ~(uint32_t)i > best) best = ~(uint32_t)i; });
-    best = block_max<NT>(best, redu);
-    if (threadIdx.x == 0) { a.index[r] = (int64_t)(~best); a.logp[r] = 0.f; }
-    return;
+};
+
+// the choice among the keys of one stretch: `base` is the mass before it, `total` the row's (below 0: this stretch is the row).  Each wave's mass of each
+// piece goes to LDS, every wave finds the (piece, wave) that the target falls in, that wave scans its lanes, the lane walks its VEC keys
+template <typename T, int NT, int E, bool VECTOR, typename S>
+__device__ __forceinline__ void locate(const Draw& a, const Par& q, int r, const Keys<T, NT, E, VECTOR>& ks, const Kept& kept, double base, double total, S& sh) {
+  using K = Keys<T, NT, E, VECTOR>;
+  constexpr int NW = NT / 64, N = K::P * NW, PER = (N + 63) / 64;
+  static_assert(N <= 512, "the table of parts");
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  double s[K::P];
+  __syncthreads();
+#pragma unroll
+  for (int p = 0; p < K::P; ++p) {
+    s[p] = 0.0;
+#pragma unroll
+    for (int i = 0; i < K::VEC; ++i) s[p] += kept(ks.key[p * K::VEC + i]);
+    const double t = wave_sum_d(s[p]);
+    if (lane == 0) sh.part[p * NW + wave] = t;
   }
-  const float topv = value_of(top), per = (float)(32.0 / q.t);
-  uint32_t cut = 1u;                                                     // keys from here on are kept
-  // gathers the keys >= from of one bin into `list`, the thresholds are then found among them; false where they do not fit
-  auto gather = [&](int bin, uint32_t from) {
+  __syncthreads();
+  double mine[PER], m = 0.0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) { mine[i] = lane * PER + i < N ? sh.part[lane * PER + i] : 0.0; m += mine[i]; }
+  double run = wave_scan_d(m);
+  if (total < 0.0) { total = last_lane_d(run); base = 0.0; }
+  const double target = q.u * total;
+  run = base + (run - m);
+  int hit = 0x7fffffff, last = -1;
+  double before = 0.0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (mine[i] > 0.0) last = lane * PER + i;
+    if (hit == 0x7fffffff && mine[i] > 0.0 && run + mine[i] > target) { hit = lane * PER + i; before = run; }
+    run += mine[i];
+  }
+  const unsigned long long hits = __ballot(hit != 0x7fffffff), lasts = __ballot(last >= 0);
+  if (lasts == 0ull) return;                                             // (cannot be: the stretch holds mass)
+  const bool over = hits == 0ull;                                        // rounding left the target at the very end: the last key with a weight
+  const int from = over ? 63 - __clzll((long long)lasts) : __ffsll(hits) - 1;
+  const int part = __shfl(over ? last : hit, from);
+  before = __shfl(before, from);
+  if (part % NW != wave) return;
+  const int piece = part / NW;
+  double sp = 0.0;
+#pragma unroll
+  for (int p = 0; p < K::P; ++p) sp = p == piece ? s[p] : sp;
+  const double inc = wave_scan_d(sp);
+  const unsigned long long lh = __ballot(!over && sp > 0.0 && before + inc > target), la = __ballot(sp > 0.0);
+  const int at = lh ? __ffsll(lh) - 1 : 63 - __clzll((long long)la);
+  if (lane != at) return;
+  double c = before + (inc - sp);
+  uint32_t kk = 0u;
+  int pick = 0;
+  bool done = false;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    if (e / K::VEC != piece || done) continue;
+    const double w = kept(ks.key[e]);
+    c += w;
+    if (w > 0.0) {
+      kk = ks.key[e];
+      pick = ks.index(e);
+      done = lh != 0ull && c > target;
+    }
+  }
+  a.index[r] = pick;
+  a.logp[r] = (float)(z_of(kk, kept.top, q.c2) - log_of(total));
+}
+
+// The thresholds of a row.  WALK(f) calls f(key) for all keys of the row, each by one thread of the workgroup.
+template <int NT, typename WALK, typename S>
+__device__ __forceinline__ uint32_t thresholds(const Draw& a, const Par& q, uint32_t top, uint32_t all, WALK walk, S& sh) {
+  constexpr int LIST = S::LISTED;
+  const int lane = threadIdx.x & 63;
+  const double topd = (double)value_of(top);
+  const float topv = value_of(top), per = (float)(22.180709777918249 * q.c2);      // 32 / T
+  uint32_t cut = 1u;
+  auto gather = [&](int bin, uint32_t from) {                            // the keys >= from of one bin into the list; how many they are
     __syncthreads();
-    if (threadIdx.x == 0) nlist = 0;
+    if (threadIdx.x == 0) sh.nlist = 0;
     __syncthreads();
-    row.walk([&](uint32_t k, int) {
-      if (k >= from && k && bin_of(k, topv, per) == bin) {
-        const int at = atomicAdd(&nlist, 1);
-        if (at < RR_DRAW_LIST) list[at] = k;
+    walk([&](uint32_t k) {
+      if (k >= from && bin_of(k, topv, per) == bin) {
+        const int at = atomicAdd(&sh.nlist, 1);
+        if (at < LIST) sh.list[at] = k;
       }
     });
     __syncthreads();
-    return nlist;
+    return sh.nlist;
   };
   auto each = [&](int n, int bin, uint32_t from, auto f) {               // f(key) for the bin's keys: from the list, or where they did not fit from the row
-    if (n <= RR_DRAW_LIST) {
-      for (int i = threadIdx.x; i < n; i += NT) f(list[i]);
+    if (n <= LIST) {
+      for (int i = threadIdx.x; i < n; i += NT) f(sh.list[i]);
     } else {
-      row.walk([&](uint32_t k, int) { if (k >= from && k && bin_of(k, topv, per) == bin) f(k); });
+      walk([&](uint32_t k) { if (k >= from && bin_of(k, topv, per) == bin) f(k); });
     }
   };
   auto ends = [&](int n, int bin, uint32_t from, uint32_t& lo, uint32_t& hi) {
     uint32_t h = 0u, l = 0u;                                             // l: of the complements
     each(n, bin, from, [&](uint32_t k) { h = k > h ? k : h; l = ~k > l ? ~k : l; });
-    hi = block_max<NT>(h, redu);
-    lo = ~block_max<NT>(l, redu);
+    hi = block_max<NT>(h, sh.redu);
+    lo = ~block_max<NT>(l, sh.redu);
   };
-  if (q.k > 0 && q.k < a.V) {
-    const uint32_t all = (uint32_t)block_sum<NT>((uint32_t)ntop, redu);
-    if (all > (uint32_t)q.k) {
-      for (int i = threadIdx.x; i < RR_DRAW_BINS; i += NT) cnt[i] = 0u;
+  if (q.k > 0 && all > (uint32_t)q.k) {
+    for (int i = threadIdx.x; i < RR_DRAW_BINS; i += NT) sh.cnt[i] = 0u;
+    __syncthreads();
+    walk([&](uint32_t k) { if (k) atomicAdd(&sh.cnt[bin_of(k, topv, per)], 1u); });
+    __syncthreads();
+    find_bin<NT>(sh.cnt, (double)q.k, sh.redu, &sh.found, &sh.above_c);
+    const int bin = sh.found;
+    const uint32_t need = (uint32_t)q.k - sh.above_c;                    // the need-th largest of the bin
+    const int n = gather(bin, 1u);
+    if (n <= 256) {                                                      // the first wave alone, without barriers
+      if (threadIdx.x < 64) {
+        uint32_t k4[4], t = 0u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { k4[e] = lane + 64 * e < n ? sh.list[lane + 64 * e] : 0u; t = k4[e] > t ? k4[e] : t; }
+        const uint32_t c = kth_largest(k4, (int)need, wave_max_u(t));
+        if (lane == 0) sh.above_c = c;
+      }
       __syncthreads();
-      row.walk([&](uint32_t k, int) { if (k) atomicAdd(&cnt[bin_of(k, topv, per)], 1u); });
-      __syncthreads();
-      find_bin<NT>(cnt, (double)q.k, redu, &found, &above_c);
-      const int bin = found;
-      const uint32_t need = (uint32_t)q.k - above_c;                     // the need-th largest of the bin
-      const int n = gather(bin, 1u);
+      cut = sh.above_c;
+    } else {
       uint32_t lo, hi;
       ends(n, bin, 1u, lo, hi);
       while (lo < hi) {
         const uint32_t mid = lo + ((hi - lo) >> 1) + 1u;
         uint32_t c = 0u;
         each(n, bin, 1u, [&](uint32_t k) { c += k >= mid; });
-        c = block_sum<NT>(c, redu);
+        c = block_sum<NT>(c, sh.redu);
         if (c >= need) lo = mid; else hi = mid - 1u;
       }
       cut = lo;
     }
   }
   if (q.p > 0.0 && q.p < 1.0) {
-    for (int i = threadIdx.x; i < RR_DRAW_BINS; i += NT) mass[i] = 0ull;
+    for (int i = threadIdx.x; i < RR_DRAW_BINS; i += NT) sh.mass[i] = 0ull;
     __syncthreads();
     unsigned long long m = 0ull;
-    row.walk([&](uint32_t k, int) {
+    walk([&](uint32_t k) {
       if (k >= cut) {
-        const unsigned long long w = steps_of(exp(z_of(k, top, q.t)));
+        const unsigned long long w = steps_of(weight_of(k, top, topd, q.c2));
         m += w;
-        if (w) atomicAdd(&mass[bin_of(k, topv, per)], w);
+        if (w) atomicAdd(&sh.mass[bin_of(k, topv, per)], w);
       }
     });
-    m = block_sum<NT>(m, redm);                                          // (its barriers stand between the histogram's writes and reads)
+    m = block_sum<NT>(m, sh.redm);                                       // (its barriers stand between the histogram's writes and reads)
     const double lim = q.p * (double)m;
-    find_bin<NT>(mass, lim, redm, &found, &above_m);
-    const int bin = found;
-    const unsigned long long before = above_m;
+    find_bin<NT>(sh.mass, lim, sh.redm, &sh.found, &sh.above_m);
+    const int bin = sh.found;
+    const unsigned long long before = sh.above_m;
     const int n = gather(bin, cut);
-    uint32_t lo, hi;
-    ends(n, bin, cut, lo, hi);
-    while (lo < hi) {                                                    // the smallest value with less than lim strictly above it
-      const uint32_t mid = lo + ((hi - lo) >> 1);
-      unsigned long long s = 0ull;
-      each(n, bin, cut, [&](uint32_t k) { if (k > mid) s += steps_of(exp(z_of(k, top, q.t))); });
-      s = before + block_sum<NT>(s, redm);
+    if (n <= 256) {
+      if (threadIdx.x < 64) {
+        uint32_t k4[4], t = 0u;
+        unsigned long long w4[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          k4[e] = lane + 64 * e < n ? sh.list[lane + 64 * e] : 0u;
+          w4[e] = k4[e] ? steps_of(weight_of(k4[e], top, topd, q.c2)) : 0ull;
+          t = k4[e] > t ? k4[e] : t;
+        }
+        const uint32_t c = mass_threshold<4, unsigned long long>(k4, w4, wave_max_u(t), before, lim, sh.cnt, (unsigned long long*)sh.part, lane);
+        if (lane == 0) sh.above_c = c;
+      }
+      __syncthreads();
+      cut = sh.above_c;
+    } else {
+      uint32_t lo, hi;
+      ends(n, bin, cut, lo, hi);
+      while (lo < hi) {                                                  // the smallest value with less than lim strictly above it
+        const uint32_t mid = lo + ((hi - lo) >> 1);
+        unsigned long long s = 0ull;
+        each(n, bin, cut, [&](uint32_t k) { if (k > mid) s += steps_of(weight_of(k, top, topd, q.c2)); });
+        s = before + block_sum<NT>(s, sh.redm);
+        if ((double)s < lim) hi = mid; else lo = mid + 1u;
+      }
+      cut = lo;
+    }
+  }
+  return cut;
+}
+
+// A row of any length by one workgroup.  ONE: the row's keys fit its registers; else stretch after stretch is loaded again for every walk
+template <typename T, int NT, int E, bool VECTOR, bool ONE, typename S>
+__device__ __forceinline__ void draw_row(const Draw& a, int r, S& sh) {
+  using K = Keys<T, NT, E, VECTOR>;
+  const T* row = (const T*)a.logits + (long long)r * a.ld;
+  const uint8_t* mask = a.mask ? a.mask + (long long)r * a.ldm : nullptr;
+  const Par q = par_of(a, r);
+  K ks;
+  if constexpr (ONE) ks.load(row, mask, 0, a.V);
+  auto walk_at = [&](auto f) {
+    if constexpr (ONE) ks.each(f);
+    else
+      for (int b = 0; b < a.V; b += K::N) { ks.load(row, mask, b, a.V); ks.each(f); }
+  };
+  uint32_t top = 0u, n = 0u;
+  walk_at([&](uint32_t k, int) { top = k > top ? k : top; n += k != 0u; });
+  top = block_max<NT>(top, sh.redu);
+  if (top == 0u) {
+    if (threadIdx.x == 0) { a.index[r] = 0; a.logp[r] = -INFINITY; }
+    return;
+  }
+  if (q.greedy) {
+    uint32_t best = 0u;                                                  // ~index: the largest is the lowest index
+    walk_at([&](uint32_t k, int i) { if (k == top && ~(uint32_t)i > best) best = ~(uint32_t)i; });
+    best = block_max<NT>(best, sh.redu);
+    if (threadIdx.x == 0) { a.index[r] = (int64_t)(~best); a.logp[r] = 0.f; }
+    return;
+  }
+  if (q.k > 0 && q.k < a.V) n = block_sum<NT>(n, sh.redu);
+  const uint32_t cut = thresholds<NT>(a, q, top, n, [&](auto f) { walk_at([&](uint32_t k, int) { f(k); }); }, sh);
+  const Kept kept = {top, cut, (double)value_of(top), q.c2, q.mp};
+  if constexpr (ONE) {
+    locate(a, q, r, ks, kept, 0.0, -1.0, sh);
+  } else {
+    double total = 0.0;
+    auto stretch = [&](int b) {
+      ks.load(row, mask, b, a.V);
+      double s = 0.0;
+      ks.each([&](uint32_t k, int) { s += kept(k); });
+      return block_sum<NT>(s, sh.redd);
+    };
+    for (int b = 0; b < a.V; b += K::N) total += stretch(b);
+    double before = 0.0, last_before = 0.0;
+    int at = -1, last = 0;
+    for (int b = 0; b < a.V && at < 0; b += K::N) {                      // (the same sums again: uniform)
+      const double m = stretch(b);
+      if (m > 0.0) { last = b; last_before = before; }
+      if (before + m > q.u * total) at = b;
+      else before += m;
+    }
+    if (at < 0) { at = last; before = last_before; }
+    ks.load(row, mask, at, a.V);
+    locate(a, q, r, ks, kept, before, total, sh);
+  }
+}
+template <typename T, int NT, int E, bool VECTOR, bool ONE>
+__global__ __launch_bounds__(NT) void k_draw_row(Draw a) {
+  __shared__ Scratch<NT, 1024> sh;
+  draw_row<T, NT, E, VECTOR, ONE>(a, blockIdx.x, sh);
+}
+
+// ---- few long rows: every stretch of a row has its own workgroup, five launches
+//   top      the stretches' maxima and counts
+//   measure  a histogram of the row (counts; masses too where top-p filters the whole row), or without a filter the stretches' masses
+//   border   a workgroup a row: the bin of the border
+//   gather   where all keys up to that bin are few, they go to a list with their indices, else the bin's keys do and the stretches' masses above it
+//            are summed
+//   pick     a workgroup a row: the thresholds among the list, the choice
+// A row whose list would overflow is done by `pick` alone, walking all of it.  (Letting the last workgroup of a row go on instead of a launch took
+// ten times as long: the fences that make the others' data visible across the eight L2s write them back.)
+struct Long {
+  uint32_t *tops, *counts;             // [R][C]
+  double* masses;                      // [R][C]
+  unsigned long long* mass;            // [R][bins]
+  uint32_t* cnt;                       // [R][bins]
+  uint32_t *list, *where;              // [R][RR_DRAW_LIST]
+  unsigned long long *whole, *above;   // [R] the row's mass, that above the border's bin
+  uint32_t *top, *n;                   // [R]
+  int *nlist, *mode, *bin, *greedy;      // [R]
+  int C;
+};
+enum { RR_NOTHING = 0, RR_LIST_ALL = 1, RR_LIST_BORDER = 2, RR_ALONE = 3, RR_UNFILTERED = 4, RR_GREEDY = 5 };
+struct LongScratch : Scratch<RR_DRAW_NT, RR_DRAW_LIST> {
+  uint32_t where[RR_DRAW_LIST];
+};
+
+__device__ __forceinline__ bool by_count(const Par& q, uint32_t n) { return q.k > 0 && n > (uint32_t)q.k; }
+__device__ __forceinline__ bool by_mass(const Par& q) { return q.p > 0.0 && q.p < 1.0; }
+
+template <typename T, bool VECTOR>
+using LongKeys = Keys<T, RR_DRAW_NT, RR_DRAW_STRETCH / RR_DRAW_NT, VECTOR>;
+template <typename T, bool VECTOR>
+__device__ __forceinline__ void load_stretch(LongKeys<T, VECTOR>& ks, const Draw& a, int r, int c) {
+  ks.load((const T*)a.logits + (long long)r * a.ld, a.mask ? a.mask + (long long)r * a.ldm : nullptr, c * RR_DRAW_STRETCH, a.V);
+}
+template <typename T, bool VECTOR>
+__global__ __launch_bounds__(RR_DRAW_NT) void k_draw_top(Draw a, Long l) {
+  __shared__ uint32_t red[RR_DRAW_NT / 64];
+  const int r = blockIdx.x / l.C, c = blockIdx.x % l.C;
+  LongKeys<T, VECTOR> ks;
+  load_stretch<T, VECTOR>(ks, a, r, c);
+  uint32_t top = 0u, n = 0u;
+  ks.each([&](uint32_t k, int) { top = k > top ? k : top; n += k != 0u; });
+  top = block_max<RR_DRAW_NT>(top, red);
+  n = block_sum<RR_DRAW_NT>(n, red);
+  if (threadIdx.x == 0) { l.tops[(long long)r * l.C + c] = top; l.counts[(long long)r * l.C + c] = n; }
+  if (c == 0) {
+    l.cnt[(long long)r * RR_DRAW_BINS + threadIdx.x] = 0u;
+    l.mass[(long long)r * RR_DRAW_BINS + threadIdx.x] = 0ull;
+    if (threadIdx.x == 0) { l.nlist[r] = 0; l.greedy[r] = 0x7fffffff; }
+  }
+}
+
+template <typename T, bool VECTOR>
+__global__ __launch_bounds__(RR_DRAW_NT) void k_draw_measure(Draw a, Long l) {
+  __shared__ LongScratch sh;
+  constexpr int NT = RR_DRAW_NT;
+  const int r = blockIdx.x / l.C, c = blockIdx.x % l.C, lane = threadIdx.x & 63;
+  LongKeys<T, VECTOR> ks;
+  load_stretch<T, VECTOR>(ks, a, r, c);
+  const Par q = par_of(a, r);
+  uint32_t top = 0u, n = 0u;                                             // the row's maximum and its number of keys, by each wave itself
+  for (int i = lane; i < l.C; i += 64) {
+    const uint32_t x = l.tops[(long long)r * l.C + i];
+    top = x > top ? x : top;
+    n += l.counts[(long long)r * l.C + i];
+  }
+  top = wave_max_u(top);
+  n = wave_total(n);
+  const bool counts = by_count(q, n), masses = !counts && by_mass(q);
+  const int simple = top == 0u ? RR_NOTHING : q.greedy ? RR_GREEDY : !counts && !masses ? RR_UNFILTERED : -1;
+  if (c == 0 && threadIdx.x == 0) { l.top[r] = top; l.n[r] = n; if (simple >= 0) l.mode[r] = simple; }
+  if (top == 0u) return;
+  if (q.greedy) {
+    uint32_t best = 0u;
+    ks.each([&](uint32_t k, int i) { if (k == top && ~(uint32_t)i > best) best = ~(uint32_t)i; });
+    best = block_max<NT>(best, sh.redu);
+    if (threadIdx.x == 0 && best) atomicMin(&l.greedy[r], (int)~best);
+    return;
+  }
+  const double topd = (double)value_of(top);
+  const float topv = value_of(top), per = (float)(22.180709777918249 * q.c2);
+  if (simple == RR_UNFILTERED) {
+    const Kept kept = {top, 1u, topd, q.c2, q.mp};
+    double s = 0.0;
+    ks.each([&](uint32_t k, int) { s += kept(k); });
+    s = block_sum<NT>(s, sh.redd);
+    if (threadIdx.x == 0) l.masses[(long long)r * l.C + c] = s;
+    return;
+  }
+  sh.cnt[threadIdx.x] = 0u;
+  sh.mass[threadIdx.x] = 0ull;
+  __syncthreads();
+  ks.each([&](uint32_t k, int) {
+    if (k) {
+      const int b = bin_of(k, topv, per);
+      atomicAdd(&sh.cnt[b], 1u);
+      if (masses) {
+        const unsigned long long w = steps_of(weight_of(k, top, topd, q.c2));
+        if (w) atomicAdd(&sh.mass[b], w);
+      }
+    }
+  });
+  __syncthreads();
+  const long long at = (long long)r * RR_DRAW_BINS + threadIdx.x;
+  if (sh.cnt[threadIdx.x]) atomicAdd(&l.cnt[at], sh.cnt[threadIdx.x]);
+  if (sh.mass[threadIdx.x]) atomicAdd(&l.mass[at], sh.mass[threadIdx.x]);
+}
+
+// a workgroup a row: the bin of the border, and how the row goes on
+__global__ __launch_bounds__(RR_DRAW_NT) void k_draw_border(Draw a, Long l) {
+  __shared__ Scratch<RR_DRAW_NT, 64> sh;
+  constexpr int NT = RR_DRAW_NT;
+  const int r = blockIdx.x;
+  const uint32_t n = l.n[r];
+  const Par q = par_of(a, r);
+  if (l.top[r] == 0u || q.greedy || (!by_count(q, n) && !by_mass(q))) return;
+  const bool counts = by_count(q, n), masses = !counts;
+  const long long at = (long long)r * RR_DRAW_BINS + threadIdx.x;
+  const uint32_t mine = l.cnt[at];
+  const unsigned long long mym = l.mass[at];
+  sh.cnt[threadIdx.x] = mine;
+  sh.mass[threadIdx.x] = mym;
+  const unsigned long long whole = block_sum<NT>(mym, sh.redm);
+  sh.above_m = 0ull;
+  if (counts) find_bin<NT>(sh.cnt, (double)q.k, sh.redu, &sh.found, &sh.above_c);
+  else find_bin<NT>(sh.mass, q.p * (double)whole, sh.redm, &sh.found, &sh.above_m);
+  const int bin = sh.found;
+  const uint32_t upto = block_sum<NT>((int)threadIdx.x <= bin ? mine : 0u, sh.redu), within = sh.cnt[bin];
+  if (threadIdx.x == 0) {
+    l.mode[r] = upto <= RR_DRAW_LIST ? RR_LIST_ALL : masses && within <= RR_DRAW_LIST ? RR_LIST_BORDER : RR_ALONE;
+    l.bin[r] = bin;
+    l.whole[r] = whole;
+    l.above[r] = sh.above_m;
+  }
+}
+
+// the row's choice among stretches with the masses `m(c)`: the stretch, the mass before it, the total
+template <typename F>
+__device__ __forceinline__ void pick_stretch(int C, double u, F m, int& at, double& before, double& total) {
+  total = 0.0;
+  for (int c = 0; c < C; ++c) total += m(c);
+  double run = 0.0, last_before = 0.0;
+  int last = 0;
+  at = -1;
+  for (int c = 0; c < C; ++c) {
+    const double x = m(c);
+    if (x > 0.0) { last = c; last_before = run; }
+    if (at < 0 && run + x > u * total) { at = c; before = run; }
+    run += x;
+  }
+  if (at < 0) { at = last; before = last_before; }
+}
+
+// a list in index order (a bitonic sort of sh.where, sh.list with it); `size`: the power of two >= 64 that holds it
+__device__ __forceinline__ void sort_list(LongScratch& sh, int size) {
+  for (int b = 2; b <= size; b <<= 1)
+    for (int d = b >> 1; d > 0; d >>= 1) {
+      __syncthreads();
+      if ((int)threadIdx.x < size / 2) {
+        const int i = ((int)threadIdx.x / d) * 2 * d + (int)threadIdx.x % d, j = i + d;
+        const uint32_t pi = sh.where[i], pj = sh.where[j];
+        if ((pi > pj) == ((i & b) == 0)) {
+          sh.where[i] = pj; sh.where[j] = pi;
+          const uint32_t t = sh.list[i];
+          sh.list[i] = sh.list[j]; sh.list[j] = t;
+        }
+      }
+    }
+  __syncthreads();
+}
+
+// a workgroup a row: the thresholds among the list, the choice
+template <typename T, bool VECTOR>
+__global__ __launch_bounds__(RR_DRAW_NT) void k_draw_pick(Draw a, Long l) {
+  __shared__ LongScratch sh;
+  constexpr int NT = RR_DRAW_NT;
+  const int r = blockIdx.x, mode = l.mode[r];
+  const uint32_t top = l.top[r];
+  const Par q = par_of(a, r);
+  if (mode == RR_NOTHING || mode == RR_GREEDY) {
+    if (threadIdx.x == 0) { a.index[r] = mode == RR_NOTHING ? 0 : l.greedy[r]; a.logp[r] = mode == RR_NOTHING ? -INFINITY : 0.f; }
+    return;
+  }
+  if (mode == RR_ALONE) {
+    draw_row<T, NT, RR_DRAW_STRETCH / NT, VECTOR, false>(a, r, sh);
+    return;
+  }
+  const double topd = (double)value_of(top);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const bool counted = by_count(q, l.n[r]);
+  if (mode == RR_UNFILTERED) {
+    const Kept kept = {top, 1u, topd, q.c2, q.mp};
+    int at;
+    double before, total;
+    pick_stretch(l.C, q.u, [&](int i) { return l.masses[(long long)r * l.C + i]; }, at, before, total);
+    LongKeys<T, VECTOR> ks;
+    load_stretch<T, VECTOR>(ks, a, r, at);
+    locate(a, q, r, ks, kept, before, total, sh);
+    return;
+  }
+  const int cnt = l.nlist[r];                                            // <= RR_DRAW_LIST = 2 NT
+  const uint32_t* list = l.list + (long long)r * RR_DRAW_LIST;
+  const uint32_t* where = l.where + (long long)r * RR_DRAW_LIST;
+  uint32_t key[2], pos[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int i = threadIdx.x + NT * e;
+    key[e] = i < cnt ? list[i] : 0u;
+    pos[e] = i < cnt ? where[i] : 0xffffffffu;
+  }
+  const double whole = counted ? -1.0 : (double)l.whole[r];              // what top-p refers to, in steps
+  int size = 64;
+  while (size < cnt) size <<= 1;                                         // <= RR_DRAW_LIST
+  if (mode == RR_LIST_ALL && cnt <= 256) {                               // the first wave, as a short row
+    __syncthreads();
+    if (wave < 4) { sh.list[threadIdx.x] = key[0]; sh.where[threadIdx.x] = pos[0]; }
+    sort_list(sh, size);
+    if (wave > 0) return;
+    uint32_t k4[4], p4[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { k4[e] = sh.list[lane + 64 * e]; p4[e] = sh.where[lane + 64 * e]; }
+    if (counted) {
+      const uint32_t cut = kth_largest(k4, q.k, top);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) k4[e] = k4[e] >= cut ? k4[e] : 0u;
+      const int n = count_ge(k4, 1u);
+      if (n <= 64) {
+        wave_lds();
+        int base = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const unsigned long long b = __ballot(k4[e] != 0u);
+          const int at = base + __popcll(b & ((1ull << lane) - 1ull));
+          if (k4[e]) { sh.list[at] = k4[e]; sh.where[at] = p4[e]; }
+          base += __popcll(b);
+        }
+        wave_lds();
+        uint32_t k1[1] = {lane < n ? sh.list[lane] : 0u};
+        const int i1 = lane < n ? (int)sh.where[lane] : 0;
+        choose<1>(a, q, r, k1, [&](int) { return i1; }, top, -1.0, nullptr, nullptr, lane);
+        return;
+      }
+    }
+    choose<4>(a, q, r, k4, [&](int e) { return (int)p4[e]; }, top, whole < 0.0 ? -1.0 : whole / RR_DRAW_STEP, sh.cnt, sh.part, lane);
+    return;
+  }
+  auto extremes = [&](uint32_t& lo, uint32_t& hi) {
+    uint32_t h = 0u, c = 0u;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (key[e]) { h = key[e] > h ? key[e] : h; c = ~key[e] > c ? ~key[e] : c; }
+    hi = block_max<NT>(h, sh.redu);
+    lo = ~block_max<NT>(c, sh.redu);
+  };
+  uint32_t lo, hi;
+  if (counted) {                                                         // the list holds everything from the border's bin on
+    extremes(lo, hi);
+    for (int step = 0; lo < hi; ++step) {
+      const uint32_t mid = between(lo, hi, step) + 1u;
+      const int c = (int)block_sum<NT>((uint32_t)((key[0] >= mid) + (key[1] >= mid)), sh.redu);
+      if (c >= q.k) lo = mid; else hi = mid - 1u;
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) key[e] = key[e] >= lo ? key[e] : 0u;
+  }
+  unsigned long long w[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) w[e] = key[e] ? steps_of(weight_of(key[e], top, topd, q.c2)) : 0ull;
+  uint32_t cut = 1u;
+  if (by_mass(q)) {
+    const double m = counted ? (double)block_sum<NT>(w[0] + w[1], sh.redm) : whole;
+    const unsigned long long before = mode == RR_LIST_BORDER ? l.above[r] : 0ull;
+    const double lim = q.p * m;
+    extremes(lo, hi);
+    for (int step = 0; lo < hi; ++step) {
+      const uint32_t mid = between(lo, hi, step);
+      const unsigned long long s = before + block_sum<NT>((key[0] > mid ? w[0] : 0ull) + (key[1] > mid ? w[1] : 0ull), sh.redm);
       if ((double)s < lim) hi = mid; else lo = mid + 1u;
     }
     cut = lo;
   }
-  // masses of the waves' stretches, in index order; then the stretch that holds the target, split over all threads
-  auto weight = [&](uint32_t k) {
-    if (k < cut || k == 0u) return 0.0;
-    const double w = exp(z_of(k, top, q.t));
-    return q.mp > 0.0 && w < q.mp ? 0.0 : w;
-  };
-  double s = 0.0;
-  row.walk([&](uint32_t k, int) { s += weight(k); });
-  s = wave_sum_d(s);
+  const Kept kept = {top, cut, topd, q.c2, q.mp};
+  if (mode == RR_LIST_BORDER) {                                          // a stretch's mass: its part above the bin and what the list has of it (whole steps: no order)
+    const int C = l.C;
+    int at;
+    double before, total;
+    __syncthreads();
+    sh.mass[threadIdx.x] = 0ull;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (key[e] >= cut && kept(key[e]) > 0.0) atomicAdd(&sh.mass[pos[e] / RR_DRAW_STRETCH], w[e]);
+    __syncthreads();
+    pick_stretch(C, q.u, [&](int c) { return l.masses[(long long)r * C + c] + (double)sh.mass[c] / RR_DRAW_STEP; }, at, before, total);
+    LongKeys<T, VECTOR> ks;
+    load_stretch<T, VECTOR>(ks, a, r, at);
+    locate(a, q, r, ks, kept, before, total, sh);
+    return;
+  }
+  // everything is in the list: into index order, then as one stretch, two neighbours a thread
   __syncthreads();
-  if (row.lane == 0) redd[row.wave] = s;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    sh.list[threadIdx.x + NT * e] = key[e];
+    sh.where[threadIdx.x + NT * e] = pos[e];
+  }
+  sort_list(sh, size);
+  double c[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) c[e] = 2 * (int)threadIdx.x + e < cnt ? kept(sh.list[2 * threadIdx.x + e]) : 0.0;
+  const double inc = wave_scan_d(c[0] + c[1]);
+  if (lane == 63) sh.redd[wave] = inc;
+  if (threadIdx.x == 0) { sh.found = 0x7fffffff; sh.nlist = -1; }
   __syncthreads();
   double total = 0.0, base = 0.0;
 #pragma unroll
-  for (int i = 0; i < NW; ++i) total += redd[i];
-  const double target = q.u * total;
-  int seg = -1, last = 0;
-  double run = 0.0;
-#pragma unroll
-  for (int i = 0; i < NW; ++i) {
-    if (redd[i] > 0.0) last = i;
-    if (seg < 0 && run + redd[i] > target) { seg = i; base = run; }
-    run += redd[i];
-  }
-  if (seg < 0) { seg = last; base = run - redd[last]; }
-  // consecutive keys of the stretch to consecutive threads, `per_t` each
-  const int first = seg * row.per_wave * Rw::PIECE, len = row.per_wave * Rw::PIECE, per_t = (len + NT - 1) / NT;
-  const int i0 = first + threadIdx.x * per_t;
-  const int end = first + len < a.V ? first + len : a.V;
-  auto at = [&](int i) { return key_of((float)row.row[i], row.mask == nullptr || row.mask[i] != 0); };
-  s = 0.0;
-  for (int i = i0; i < i0 + per_t && i < end; ++i) s += weight(at(i));
-  double inc = wave_scan_d(s, row.lane);
-  __syncthreads();
-  if (row.lane == 63) redd[row.wave] = inc;
-  if (threadIdx.x == 0) { found = 0x7fffffff; nlist = -1; }
-  __syncthreads();
-  for (int i = 0; i < row.wave; ++i) base += redd[i];
-  double c = base + inc - s;
-  int pick = 0x7fffffff, lastp = -1;
-  for (int i = i0; i < i0 + per_t && i < end; ++i) {
-    const double w = weight(at(i));
-    c += w;
-    if (w > 0.0) {
-      lastp = i;
-      if (c > target) { pick = i; break; }
-    }
-  }
-  if (pick != 0x7fffffff) atomicMin(&found, pick);
-  if (lastp >= 0) atomicMax(&nlist, lastp);
+  for (int i = 0; i < NT / 64; ++i) { base = i == wave ? total : base; total += sh.redd[i]; }
+  const double target = q.u * total, b0 = base + (inc - c[0] - c[1]);
+  int hit = 0x7fffffff;
+  if (c[0] > 0.0 && b0 + c[0] > target) hit = 2 * threadIdx.x;
+  else if (c[1] > 0.0 && b0 + c[0] + c[1] > target) hit = 2 * threadIdx.x + 1;
+  if (hit != 0x7fffffff) atomicMin(&sh.found, hit);
+  if (c[0] > 0.0 || c[1] > 0.0) atomicMax(&sh.nlist, 2 * (int)threadIdx.x + (c[1] > 0.0 ? 1 : 0));
   __syncthreads();
   if (threadIdx.x == 0) {
-    const int i = found != 0x7fffffff ? found : nlist;                   // (rounding may leave the target at the very end: the last key with a weight)
-    a.index[r] = i;
-    a.logp[r] = (float)(z_of(at(i), top, q.t) - log(total));
+    const int i = sh.found != 0x7fffffff ? sh.found : sh.nlist;          // (rounding may leave the target at the very end: the last key with a weight)
+    a.index[r] = (int64_t)sh.where[i];
+    a.logp[r] = (float)(z_of(sh.list[i], top, q.c2) - log_of(total));
   }
 }
 
+template <typename T, bool VECTOR>
+__global__ __launch_bounds__(RR_DRAW_NT) void k_draw_gather(Draw a, Long l) {
+  __shared__ uint32_t list[RR_DRAW_LIST], where[RR_DRAW_LIST];
+  __shared__ double red[RR_DRAW_NT / 64];
+  __shared__ int nlist, at_global;
+  constexpr int NT = RR_DRAW_NT;
+  const int r = blockIdx.x / l.C, c = blockIdx.x % l.C, mode = l.mode[r];
+  if (mode != RR_LIST_ALL && mode != RR_LIST_BORDER) return;
+  LongKeys<T, VECTOR> ks;
+  load_stretch<T, VECTOR>(ks, a, r, c);
+  const uint32_t top = l.top[r];
+  const int bin = l.bin[r];
+  const Par q = par_of(a, r);
+  const float topv = value_of(top), per = (float)(22.180709777918249 * q.c2);
+  if (threadIdx.x == 0) nlist = 0;
+  __syncthreads();
+  double s = 0.0;
+  const Kept kept = {top, 1u, (double)topv, q.c2, q.mp};
+  ks.each([&](uint32_t k, int i) {
+    if (!k) return;
+    const int b = bin_of(k, topv, per);
+    if (b > bin) return;
+    if (mode == RR_LIST_ALL || b == bin) {
+      const int to = atomicAdd(&nlist, 1);                               // (at most the row's number, which fits)
+      list[to] = k;
+      where[to] = (uint32_t)i;
+    } else s += kept(k);
+  });
+  __syncthreads();
+  const int got = nlist;
+  if (threadIdx.x == 0 && got) at_global = atomicAdd(&l.nlist[r], got);
+  __syncthreads();
+  for (int i = threadIdx.x; i < got; i += NT) {
+    l.list[(long long)r * RR_DRAW_LIST + at_global + i] = list[i];
+    l.where[(long long)r * RR_DRAW_LIST + at_global + i] = where[i];
+  }
+  if (mode == RR_LIST_BORDER) {
+    s = block_sum<NT>(s, red);
+    if (threadIdx.x == 0) l.masses[(long long)r * l.C + c] = s;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+// long rows that are too few to give each CU one go by stretches, where the row does not fit one workgroup's registers
+bool by_stretches(long long R, int V) { return V > 16384 && R <= 1024; }
+int stretches(int V) { return (V + RR_DRAW_STRETCH - 1) / RR_DRAW_STRETCH; }
+size_t long_bytes(long long R, int V) {
+  const size_t C = (size_t)stretches(V);
+  return (size_t)R * (C * 8 + RR_DRAW_BINS * 8 + 16 + C * 8 + RR_DRAW_BINS * 4 + RR_DRAW_LIST * 8 + 24);
+}
+
+template <typename T, bool VECTOR>
+int draw_long(const Draw& a, void* ws, hipStream_t st) {
+  Long l;
+  const size_t R = (size_t)a.R, C = (size_t)stretches(a.V);
+  char* p = (char*)ws;
+  auto take = [&](size_t bytes) { void* at = p; p += bytes; return at; };
+  l.masses = (double*)take(R * C * 8);
+  l.mass = (unsigned long long*)take(R * RR_DRAW_BINS * 8);
+  l.whole = (unsigned long long*)take(R * 8);
+  l.above = (unsigned long long*)take(R * 8);
+  l.tops = (uint32_t*)take(R * C * 4);
+  l.counts = (uint32_t*)take(R * C * 4);
+  l.cnt = (uint32_t*)take(R * RR_DRAW_BINS * 4);
+  l.list = (uint32_t*)take(R * RR_DRAW_LIST * 4);
+  l.where = (uint32_t*)take(R * RR_DRAW_LIST * 4);
+  l.nlist = (int*)take(R * 4);
+  l.mode = (int*)take(R * 4);
+  l.bin = (int*)take(R * 4);
+  l.greedy = (int*)take(R * 4);
+  l.top = (uint32_t*)take(R * 4);
+  l.n = (uint32_t*)take(R * 4);
+  l.C = (int)C;
+  const dim3 grid((unsigned)(R * C)), one((unsigned)R), nt(RR_DRAW_NT);
+  hipLaunchKernelGGL((k_draw_top<T, VECTOR>), grid, nt, 0, st, a, l);
+  hipLaunchKernelGGL((k_draw_measure<T, VECTOR>), grid, nt, 0, st, a, l);
+  hipLaunchKernelGGL(k_draw_border, one, nt, 0, st, a, l);
+  hipLaunchKernelGGL((k_draw_gather<T, VECTOR>), grid, nt, 0, st, a, l);
+  hipLaunchKernelGGL((k_draw_pick<T, VECTOR>), one, nt, 0, st, a, l);
+  return rr_check(hipGetLastError());
+}
+
+template <typename T, bool VECTOR>
+int draw_rows(const Draw& a, hipStream_t st) {
+  const dim3 grid((unsigned)a.R);
+  // the fewest threads whose registers hold the row (8 .. 32 keys each; 1 024 threads of 32 spill); what fits none is walked in stretches
+  if (a.V <= 2048) hipLaunchKernelGGL((k_draw_row<T, 256, 8, VECTOR, true>), grid, dim3(256), 0, st, a);
+  else if (a.V <= 4096) hipLaunchKernelGGL((k_draw_row<T, 256, 16, VECTOR, true>), grid, dim3(256), 0, st, a);
+  else if (a.V <= 8192) hipLaunchKernelGGL((k_draw_row<T, 256, 32, VECTOR, true>), grid, dim3(256), 0, st, a);
+  else if (a.V <= 16384) hipLaunchKernelGGL((k_draw_row<T, 512, 32, VECTOR, true>), grid, dim3(512), 0, st, a);
+  else hipLaunchKernelGGL((k_draw_row<T, 1024, 16, VECTOR, false>), grid, dim3(1024), 0, st, a);
+  return rr_check(hipGetLastError());
+}
+
 template <typename T>
-int draw_go(const Draw& a, hipStream_t st) {
+int draw_go(const Draw& a, void* ws, hipStream_t st) {
   const dim3 wg((unsigned)((a.R + 3) / 4));
-  // a wave a row up to 1 024 keys (16 registers of keys a lane); beyond that 256 threads a row, 1 024 where a row is long enough to feed them
+  // up to 1 024 keys a wave a row (16 registers of keys a lane)
   if (a.V <= 64) hipLaunchKernelGGL((k_draw_wave<T, 1>), wg, dim3(256), 0, st, a);
   else if (a.V <= 128) hipLaunchKernelGGL((k_draw_wave<T, 2>), wg, dim3(256), 0, st, a);
   else if (a.V <= 256) hipLaunchKernelGGL((k_draw_wave<T, 4>), wg, dim3(256), 0, st, a);
@@ -525,32 +1154,31 @@ int draw_go(const Draw& a, hipStream_t st) {
   else {
     const int e = 16 / (int)sizeof(T);
     const bool vec = a.ld % e == 0 && rr_aligned16(a.logits);
-    if (a.V <= 8192) {
-      if (vec) hipLaunchKernelGGL((k_draw_row<T, 256, true>), dim3((unsigned)a.R), dim3(256), 0, st, a);
-      else hipLaunchKernelGGL((k_draw_row<T, 256, false>), dim3((unsigned)a.R), dim3(256), 0, st, a);
-    } else {
-      if (vec) hipLaunchKernelGGL((k_draw_row<T, 1024, true>), dim3((unsigned)a.R), dim3(1024), 0, st, a);
-      else hipLaunchKernelGGL((k_draw_row<T, 1024, false>), dim3((unsigned)a.R), dim3(1024), 0, st, a);
-    }
+    if (by_stretches(a.R, a.V)) return vec ? draw_long<T, true>(a, ws, st) : draw_long<T, false>(a, ws, st);
+    return vec ? draw_rows<T, true>(a, st) : draw_rows<T, false>(a, st);
   }
   return rr_check(hipGetLastError());
 }
 
 }  // namespace
 
+extern "C" long long rr_draw_workspace(int R, int V) { return R > 0 && V > 0 && by_stretches(R, V) ? (long long)long_bytes(R, V) : 0; }
+
 extern "C" int rr_draw(int dtype, const void* logits, long long ld, const uint8_t* mask, long long ldm, const float* uniforms, int64_t* index, float* logp, int R, int V,
                        double temperature, int top_k, double top_p, double min_p, const float* row_temperature, const int* row_top_k, const float* row_top_p,
-                       const float* row_min_p, hipStream_t st) {
+                       const float* row_min_p, void* workspace, long long workspace_bytes, hipStream_t st) {
   if (R < 0 || V < 1 || V > (1 << 24) || logits == nullptr || uniforms == nullptr || index == nullptr || logp == nullptr || ld < 0 || ldm < 0) return RR_EINVAL;
   if ((row_temperature == nullptr && !(temperature >= 0.0 && temperature < 1e30)) || (row_top_p == nullptr && !(top_p >= 0.0 && top_p <= 1.0)) ||
       (row_min_p == nullptr && !(min_p >= 0.0 && min_p <= 1.0)) || (row_top_k == nullptr && top_k < 0))
     return RR_EINVAL;
   if (R == 0) return RR_OK;
-  const Draw a = {logits, mask, uniforms, index, logp, row_temperature, row_top_p, row_min_p, row_top_k, temperature, top_p, min_p, ld, ldm, top_k, R, V};
+  if (by_stretches(R, V) && (workspace == nullptr || (size_t)workspace_bytes < long_bytes(R, V) || !rr_aligned16(workspace))) return RR_EINVAL;
+  const Draw a = {logits, mask, uniforms, index, logp, row_temperature, row_top_p, row_min_p, row_top_k, temperature, 1.44269504088896340736 / temperature, top_p, min_p, ld, ldm,
+                  top_k, R, V};
   switch (dtype) {
-    case RR_F32: return draw_go<float>(a, st);
-    case RR_F16: return draw_go<rr_f16>(a, st);
-    case RR_BF16: return draw_go<rr_bf16>(a, st);
+    case RR_F32: return draw_go<float>(a, workspace, st);
+    case RR_F16: return draw_go<rr_f16>(a, workspace, st);
+    case RR_BF16: return draw_go<rr_bf16>(a, workspace, st);
   }
   return RR_EINVAL;
 }

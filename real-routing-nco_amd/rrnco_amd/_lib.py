@@ -171,7 +171,8 @@ _SIGS = {
     "rr_mlp_wgrad": [C.POINTER(MlpWgradW), vp, vp, vp, vp, vp, vp, vp, i32, i32, C.c_longlong, vp, vp],
     "rr_mlp_wgrad16": [C.POINTER(MlpWgradW), vp, vp, vp, vp, vp, vp, vp, i32, i32, C.c_longlong, vp, vp],
     "rr_dec_attn_bwd": [C.POINTER(DecAttnIO), vp],
-    "rr_draw": [i32, vp, C.c_longlong, vp, C.c_longlong, vp, vp, vp, i32, i32, C.c_double, i32, C.c_double, C.c_double, vp, vp, vp, vp, vp],
+    "rr_draw": [i32, vp, C.c_longlong, vp, C.c_longlong, vp, vp, vp, i32, i32, C.c_double, i32, C.c_double, C.c_double, vp, vp, vp, vp, vp,
+                C.c_longlong, vp],
     "rr_cross_attn": [C.POINTER(XAttnIO), vp],
     "rr_cross_attn_bwd": [C.POINTER(XAttnIO), vp],
     "rr_add_rms_norm": [i32, vp, C.c_longlong, vp, C.c_longlong, vp, i32, vp, vp, vp, vp, vp, C.c_longlong, i32, f32, vp],
@@ -200,6 +201,8 @@ def lib():
         _lib.rr_matnet_workspace_bytes.restype = C.c_size_t
         _lib.rr_cross_attn_workspace.argtypes = [i32] * 7
         _lib.rr_cross_attn_workspace.restype = C.c_longlong
+        _lib.rr_draw_workspace.argtypes = [i32] * 2
+        _lib.rr_draw_workspace.restype = C.c_longlong
         if os.environ.get("RR_MARKERS", "0") == "1":
             _wrap_with_markers(_lib)
     return _lib

@@ -63,8 +63,11 @@ def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=0.0, min_p=0.0, mas
     index, logp = torch.empty(lead, dtype=torch.int64, device=dev), torch.empty(lead, dtype=torch.float32, device=dev)
     opt = lambda s: None if s is None else s.data_ptr()                                       # noqa: E731
     if R:
+        lib = L.lib()
+        n = lib.rr_draw_workspace(R, V)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
         with L.on_device(logits) as st:
-            L.check(L.lib().rr_draw(L.DTYPE_CODE[x.dtype], x.data_ptr(), x.stride(0), opt(mask), 0 if mask is None else mask.stride(0), u.data_ptr(),
+            L.check(lib.rr_draw(L.DTYPE_CODE[x.dtype], x.data_ptr(), x.stride(0), opt(mask), 0 if mask is None else mask.stride(0), u.data_ptr(),
                                     index.data_ptr(), logp.data_ptr(), R, V, float(t), min(int(k), V), float(p), float(mp), opt(row_t), opt(row_k), opt(row_p),
-                                    opt(row_mp), st), "rr_draw")
+                                    opt(row_mp), opt(ws), n, st), "rr_draw")
     return index, logp

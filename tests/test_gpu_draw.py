@@ -38,11 +38,9 @@ def reference_row(l, u, t, k, p, mp, allowed):
         order = np.argsort(-v[kept], kind="stable")
         vs, ws = v[kept][order], w[kept][order]
         lim = p * ws.sum()
-        thr = top
-        for value in np.unique(vs):                                            # ascending: the smallest with less than lim strictly above
-            if ws[vs > value].sum() < lim:
-                thr = value
-                break
+        values, first = np.unique(-vs, return_index=True)                      # descending values, where each begins in the sorted row
+        above = np.concatenate([[0.0], np.cumsum(ws)])[first]                  # the mass strictly above each
+        thr = -values[above < lim].max()                                       # the smallest with less than lim strictly above it
         kept &= v >= thr
     if mp > 0:
         kept &= w >= min(mp, 1.0)
@@ -80,7 +78,7 @@ def make(dt, R, V, seed=0, spread=3.0, masked=0.0):
     return x, u, mask
 
 
-SIZES = [1, 2, 20, 63, 64, 65, 100, 128, 129, 257, 512, 1000, 1024, 1025, 2049, 5003, 8192, 8200, 20001, 70000]
+SIZES = [1, 2, 20, 63, 64, 65, 100, 128, 129, 257, 512, 1000, 1024, 1025, 2048, 2049, 4097, 5003, 8192, 8200, 16384, 20001, 32768, 70000]
 SETTINGS = [dict(), dict(t=0.7), dict(k=1), dict(k=5, t=1.3), dict(k=40), dict(p=0.9), dict(p=0.3, t=2.0), dict(mp=0.1), dict(k=40, p=0.9, mp=0.02, t=0.9), dict(t=0.0), dict(k=10 ** 6, p=1.0),
             dict(p=0.999, k=3000)]
 
@@ -140,6 +138,15 @@ def test_settings_of_each_row(V):
     p[6], p[7], p[8], mp[9], mp[10] = 0.0, 1.0, 7.0, 3.0, -1.0
     check(x, u, mask, t=t, k=k, p=p, mp=mp)
     check(x, u, mask, t=t.double(), k=k.long(), p=0.8, mp=mp)
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=IDS)
+@pytest.mark.parametrize("V", [1500, 6000, 16000, 40000, 131075])
+def test_wide_kept_sets(dt, V):
+    """Flat rows: the filters keep thousands of keys, the border lies in a crowded place."""
+    for n, s in enumerate((dict(p=0.9), dict(p=0.5, mp=0.3), dict(p=0.99, t=0.5), dict(k=V // 3), dict(k=V // 2, p=0.7), dict(k=1500, p=0.9))):
+        x, u, mask = make(dt, 4, V, seed=V + n, spread=0.7, masked=0.2)
+        check(x, u, mask, **s)
 
 
 def test_the_choices_follow_the_distribution():
