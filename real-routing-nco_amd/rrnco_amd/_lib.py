@@ -109,12 +109,6 @@ class MtvrpExtra(C.Structure):
     _fields_ = [(n, vp) for n in ("demand_b", "used_b", "open_route", "dist_limit", "bclass")]
 
 
-class XAttnIO(C.Structure):             # csrc/rr_xattn.hip
-    _fields_ = [(n, vp) for n in ("q", "k", "v", "out", "lse", "mask", "kv_lens", "dout", "delta", "dq", "dk", "dv", "workspace")] + \
-        [(n, C.c_longlong * 3) for n in ("q_stride", "k_stride", "v_stride", "mask_stride", "dout_stride")] + \
-        [("workspace_bytes", C.c_longlong)] + [(n, i32) for n in ("lens_int64", "dtype", "B", "Lq", "Lk", "Hk", "G", "D")] + [("scale", f32)]
-
-
 _SIGS = {
     "rr_minmax_normalize": [vp, vp, vp, vp, i32, i32, vp],
     "rr_atsp_step": [vp, vp, vp, vp, i32, i32, vp],
@@ -173,8 +167,8 @@ _SIGS = {
     "rr_dec_attn_bwd": [C.POINTER(DecAttnIO), vp],
     "rr_draw": [i32, vp, C.c_longlong, vp, C.c_longlong, vp, vp, vp, i32, i32, C.c_double, i32, C.c_double, C.c_double, vp, vp, vp, vp, vp,
                 C.c_longlong, vp],
-    "rr_cross_attn": [C.POINTER(XAttnIO), vp],
-    "rr_cross_attn_bwd": [C.POINTER(XAttnIO), vp],
+    "rr_cross_attn": [vp, vp],
+    "rr_cross_attn_bwd": [vp, vp],
     "rr_add_rms_norm": [i32, vp, C.c_longlong, vp, C.c_longlong, vp, i32, vp, vp, vp, vp, vp, C.c_longlong, i32, f32, vp],
     "rr_add_rms_norm_parts": [C.c_longlong, i32],
     "rr_add_rms_norm_bwd": [i32, vp, C.c_longlong, vp, C.c_longlong, vp, i32, vp, C.c_longlong, vp, C.c_longlong, vp, vp, vp, vp, i32,
@@ -278,27 +272,20 @@ def stream():
     return torch.cuda.current_stream().cuda_stream
 
 
-DTYPE_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}      # csrc/rr_types.h
+_native = None
 
 
-class on_device:
-    """`with on_device(t) as stream:` — launches go to the device that holds `t` and to its current stream."""
-
-    def __init__(self, t):
-        self.dev = t.device
-
-    def __enter__(self):
-        self.back = None
-        cur = torch.cuda.current_device()
-        if self.dev.index is not None and self.dev.index != cur:
-            torch.cuda.set_device(self.dev)
-            self.back = cur
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *exc):
-        if self.back is not None:
-            torch.cuda.set_device(self.back)
-        return False
+def native():
+    """The torch side of the decoder operators (csrc/rr_torch.cpp), loaded once; raises if it has not been built."""
+    global _native
+    if _native is None:
+        lib()
+        try:
+            from . import _native as module
+        except ImportError as e:
+            raise ImportError(f"rrnco_amd: torch module not built: {os.path.join(_HERE, '_native.so')} (make -C real-routing-nco_amd/csrc). There is no CPU fallback.") from e
+        _native = module
+    return _native
 
 
 def check(rc, what):
