@@ -477,7 +477,7 @@ typedef struct {
   int lens_int64, dtype, B, Lq, Lk, Hk, G, D;
   float scale;
 } XAttnIO;
-long long rr_cross_attn_workspace(int B, int Lq, int Lk, int Hk, int G, int D, int backward);
+long long rr_cross_attn_workspace(int dtype, int B, int Lq, int Lk, int Hk, int G, int D, int backward);
 int rr_cross_attn(const XAttnIO* io, hipStream_t stream);
 int rr_cross_attn_bwd(const XAttnIO* io, hipStream_t stream);
 

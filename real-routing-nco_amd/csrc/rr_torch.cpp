@@ -156,7 +156,7 @@ void attention_call(const Tensor& q_, const Tensor& k_, const Tensor& v_, const 
     io.dk = ptr(dk);
     io.dv = ptr(dv);
   }
-  const long long n = rr_cross_attn_workspace(io.B, io.Lq, io.Lk, io.Hk, io.G, io.D, back);
+  const long long n = rr_cross_attn_workspace(io.dtype, io.B, io.Lq, io.Lk, io.Hk, io.G, io.D, back);
   TORCH_CHECK_VALUE(n >= 0, "cross_attention: more rows, keys or heads than 32-bit counts hold");
   if (n > 0) {
     ws = at::empty({(int64_t)n}, q.options().dtype(at::kByte));

@@ -147,28 +147,39 @@ __device__ __forceinline__ RowAt row_at(int r, int Lq, int G) {
   return {g, r - g * Lq};
 }
 
-// rows [row0, row0 + 64) of a key-side tensor into LDS (zeros behind the last row and the head dim).
-// safe: pieces that hold a non-finite value become zeros and their row's bit is set in `flag`
-template <typename T, int DP, int PITCH, typename PTR>
-__device__ __forceinline__ void stage(T* lds, PTR rowptr, int row0, int valid, int D, bool safe, uint32_t* flag) {
+// rows [row0, row0 + 64) of a tensor, 16-byte pieces over the 256 threads, on their way through registers into LDS (zeros behind the last row and the
+// head dim): the loads of the next tile are in flight while the present one is computed
+template <typename T, int DP>
+struct Piece {
   using Dm = Dims<T, DP>;
-  constexpr int N = RR_XA_KT * Dm::CPR / 256;
+  static constexpr int N = RR_XA_KT * Dm::CPR / 256;
   float4 v[N];
+  template <typename PTR>
+  __device__ __forceinline__ void load(PTR rowptr, int row0, int valid, int D) {
 #pragma unroll
-  for (int c = 0; c < N; ++c) {
-    const int i = threadIdx.x + 256 * c, row = i / Dm::CPR, ch = i % Dm::CPR;
-    v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (row0 + row < valid && ch * Mx<T>::EPC < D) v[c] = *reinterpret_cast<const float4*>(rowptr(row0 + row) + ch * Mx<T>::EPC);
-  }
-#pragma unroll
-  for (int c = 0; c < N; ++c) {
-    const int i = threadIdx.x + 256 * c, row = i / Dm::CPR, ch = i % Dm::CPR;
-    if (safe && nonfinite4(v[c], kind16<T>::v)) {
+    for (int c = 0; c < N; ++c) {
+      const int i = threadIdx.x + 256 * c, row = i / Dm::CPR, ch = i % Dm::CPR;
       v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-      atomicOr(&flag[row >> 5], 1u << (row & 31));
+      if (row0 + row < valid && ch * Mx<T>::EPC < D) v[c] = *reinterpret_cast<const float4*>(rowptr(row0 + row) + ch * Mx<T>::EPC);
     }
-    *reinterpret_cast<float4*>(lds + row * PITCH + ch * Mx<T>::EPC) = v[c];
   }
+  // safe: pieces that hold a non-finite value become zeros and their row's bit is set in `flag`
+  template <int PITCH>
+  __device__ __forceinline__ void store(T* lds, bool safe, uint32_t* flag) {
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      const int i = threadIdx.x + 256 * c, row = i / Dm::CPR, ch = i % Dm::CPR;
+      if (safe && nonfinite4(v[c], kind16<T>::v)) {
+        v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+        atomicOr(&flag[row >> 5], 1u << (row & 31));
+      }
+      *reinterpret_cast<float4*>(lds + row * PITCH + ch * Mx<T>::EPC) = v[c];
+    }
+  }
+};
+__device__ __forceinline__ void clear_flag(uint32_t* flag) {             // (by the whole workgroup)
+  if (threadIdx.x < 2) flag[threadIdx.x] = 0u;
+  __syncthreads();
 }
 
 template <typename T>
@@ -186,14 +197,30 @@ __device__ __forceinline__ int seen_keys(const XAttn& a, int b) {
   const long long n = a.lens64 ? ((const long long*)a.lens)[b] : (long long)((const int*)a.lens)[b];
   return n < 0 ? 0 : n > a.Lk ? a.Lk : (int)n;
 }
-// four consecutive mask bytes of a row, keys behind the end as zeros (one unaligned 4-byte load inside the row)
+// four consecutive mask bytes of a row from `key` on, zeros behind the end: one unaligned 4-byte load that ends inside the row
 __device__ __forceinline__ uint32_t mask4(const uint8_t* row, int key, int Lk) {
   uint32_t m = 0;
-  if (key + 4 <= Lk) __builtin_memcpy(&m, row + key, 4);
-  else
-    for (int i = 0; i < 4; ++i)
-      if (key + i < Lk) m |= (uint32_t)row[key + i] << (8 * i);
-  return m;
+  if (Lk >= 4) {                                                         // (uniform)
+    const int from = key < Lk - 4 ? key : Lk - 4, off = key - from;
+    __builtin_memcpy(&m, row + from, 4);
+    return off < 4 ? m >> (8 * off) : 0u;
+  }
+  for (int i = 0; i < Lk; ++i) m |= (uint32_t)row[i] << (8 * i);
+  return key < 4 ? m >> (8 * key) : 0u;
+}
+__device__ __forceinline__ uint32_t first_bytes(uint32_t b, int n) {     // the first n of four bytes
+  return n >= 4 ? b : n <= 0 ? 0u : b & ((1u << (8 * n)) - 1u);
+}
+// x where the byte of its place is set, y elsewhere (selects without branches: the four values stay in their registers)
+__device__ __forceinline__ void keep4(f32x4& x, uint32_t bytes, float y) {
+  const float a = x[0], b = x[1], c = x[2], d = x[3];
+  const f32x4 r = {bytes & 0xffu ? a : y, bytes & 0xff00u ? b : y, bytes & 0xff0000u ? c : y, bytes & 0xff000000u ? d : y};
+  x = r;
+}
+// the flags of four consecutive rows of a tile as bytes
+__device__ __forceinline__ uint32_t flag4(const uint32_t* flag, int row) {
+  const uint32_t f = flag[row >> 5] >> (row & 31);
+  return (f & 1u) | (f & 2u) << 7 | (f & 4u) << 14 | (f & 8u) << 21;
 }
 __device__ __forceinline__ float group_max(float v) { v = fmaxf(v, __shfl_xor(v, 16)); return fmaxf(v, __shfl_xor(v, 32)); }
 __device__ __forceinline__ float group_sum(float v) { v += __shfl_xor(v, 16); return v + __shfl_xor(v, 32); }
@@ -228,13 +255,16 @@ __device__ __forceinline__ Blk block_of(const XAttn& a) {
 }
 
 // ------------------------------------------------------------------------------------------------ forward
+// registers: two waves a SIMD, except where 128-wide float32 rows need more
+template <typename T, int DP> struct Waves { static constexpr int N = sizeof(T) == 4 && DP == 128 ? 1 : 2; };
+
 template <typename T, int DP, int QT>
-__global__ __launch_bounds__(256) void k_xattn_fwd(XAttn a) {
+__global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_fwd(XAttn a) {
   using M = Mx<T>;
   using Dm = Dims<T, DP>;
-  __shared__ __attribute__((aligned(16))) T sk[RR_XA_KT * Dm::PR];
-  __shared__ __attribute__((aligned(16))) T sv[RR_XA_KT * Dm::PX];
-  __shared__ uint32_t flag[2];
+  __shared__ __attribute__((aligned(16))) T sk[2][RR_XA_KT * Dm::PR];
+  __shared__ __attribute__((aligned(16))) T sv[2][RR_XA_KT * Dm::PX];
+  __shared__ uint32_t flag[2][2];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
   const Blk w = block_of(a);
   const int R = a.G * a.Lq, row0 = (w.blk * 4 + wave) * 16 * QT;
@@ -242,6 +272,16 @@ __global__ __launch_bounds__(256) void k_xattn_fwd(XAttn a) {
   const int seen = seen_keys(a, w.b);
   const T* kp = (const T*)a.k + (long long)w.b * a.kb + (long long)w.hk * a.kh;
   const T* vp = (const T*)a.v + (long long)w.b * a.vb + (long long)w.hk * a.vh;
+  auto krow = [&](int r) { return kp + (long long)r * a.kl; };
+  auto vrow = [&](int r) { return vp + (long long)r * a.vl; };
+  const int first = w.split * a.tiles_per_split * RR_XA_KT;
+  int last = first + a.tiles_per_split * RR_XA_KT;
+  last = last < seen ? last : seen;
+  Piece<T, DP> pk, pv;
+  if (first < last) {
+    pk.load(krow, first, seen, a.D);
+    pv.load(vrow, first, seen, a.D);
+  }
   typename M::Frag qf[QT][Dm::NK];
   load_rows<T, DP, QT>(qf, (const T*)a.q + (long long)w.b * a.qb + (long long)w.hk * a.G * a.qh, a.ql, a.qh, row0, R, a, lane);
   const uint8_t* mrow[QT];
@@ -252,9 +292,6 @@ __global__ __launch_bounds__(256) void k_xattn_fwd(XAttn a) {
     mrow[t] = a.mask + w.b * a.mb + (w.hk * a.G + at.g) * a.mh + at.s * a.ml;
   }
   const float c2 = a.scale * RR_LOG2E;
-  const int first = w.split * a.tiles_per_split * RR_XA_KT;
-  int last = first + a.tiles_per_split * RR_XA_KT;
-  last = last < seen ? last : seen;
   f32x4 o[QT][Dm::DT];
   float m[QT], l[QT];
   for (int pass = 0; pass < 2; ++pass) {
@@ -265,95 +302,134 @@ __global__ __launch_bounds__(256) void k_xattn_fwd(XAttn a) {
 #pragma unroll
       for (int d = 0; d < Dm::DT; ++d) o[t][d] = rr_zero4();
     }
-    for (int k0 = first; k0 < last; k0 += RR_XA_KT) {
-      __syncthreads();
-      if (safe) {
-        if (threadIdx.x < 2) flag[threadIdx.x] = 0u;
-        __syncthreads();
+    if (safe) {
+      clear_flag(flag[0]);
+      pk.load(krow, first, seen, a.D);
+      pv.load(vrow, first, seen, a.D);
+    }
+    if (first < last) {
+      pk.template store<Dm::PR>(sk[0], false, flag[0]);
+      pv.template store<Dm::PX>(sv[0], safe, flag[0]);
+    }
+    __syncthreads();
+    int at = 0;
+    for (int k0 = first; k0 < last; k0 += RR_XA_KT, at ^= 1) {
+      const bool more = k0 + RR_XA_KT < last;
+      if (more) {
+        pk.load(krow, k0 + RR_XA_KT, seen, a.D);
+        pv.load(vrow, k0 + RR_XA_KT, seen, a.D);
       }
-      stage<T, DP, Dm::PR>(sk, [&](int r) { return kp + (long long)r * a.kl; }, k0, seen, a.D, false, flag);
-      stage<T, DP, Dm::PX>(sv, [&](int r) { return vp + (long long)r * a.vl; }, k0, seen, a.D, safe, flag);
-      __syncthreads();
-      if (!busy) continue;
-      f32x4 s[QT][4];
+      if (busy) {
+        const T *tk = sk[at], *tv = sv[at];
+        uint32_t mb[QT][4];
+        if (a.mask != nullptr) {
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
+          for (int t = 0; t < QT; ++t)
 #pragma unroll
-        for (int t = 0; t < QT; ++t) s[t][n] = rr_zero4();
-#pragma unroll
-        for (int k = 0; k < Dm::NK; ++k) {
-          const typename M::Frag f = frag_at<T>(sk + (16 * n + j) * Dm::PR + k * M::KC + g * M::EPC);
-#pragma unroll
-          for (int t = 0; t < QT; ++t) s[t][n] = M::mma(f, qf[t][k], s[t][n]);
+            for (int n = 0; n < 4; ++n) mb[t][n] = mask4(mrow[t], k0 + 16 * n + 4 * g, a.Lk);
         }
-      }
-      if (a.mask != nullptr || k0 + RR_XA_KT > seen) {
+        const int parts = (seen - k0 + 15) >> 4;           // 16-key tiles that hold a key; whole tiles take the straight path
+        f32x4 s[QT][4];
 #pragma unroll
-        for (int t = 0; t < QT; ++t)
+        for (int n = 0; n < 4; ++n) {
 #pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const int key = k0 + 16 * n + 4 * g;
-            const uint32_t mb = a.mask != nullptr ? mask4(mrow[t], key, a.Lk) : 0x01010101u;
+          for (int t = 0; t < QT; ++t) s[t][n] = rr_zero4();
+          if (n < parts) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[t][n][i] = (key + i < seen && (mb >> (8 * i) & 0xffu)) ? s[t][n][i] : -INFINITY;
-          }
-      }
+            for (int k = 0; k < Dm::NK; ++k) {
+              const typename M::Frag f = frag_at<T>(tk + (16 * n + j) * Dm::PR + k * M::KC + g * M::EPC);
 #pragma unroll
-      for (int t = 0; t < QT; ++t) {
-        float mx = -INFINITY;
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[t][n][i]);
-        const float mn = fmaxf(m[t], group_max(mx) * c2);
-        const float mu = finite_or_zero(mn);
-        const float al = __builtin_amdgcn_exp2f(m[t] - mu);
-        float sum = 0.f;
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            s[t][n][i] = __builtin_amdgcn_exp2f(fmaf(s[t][n][i], c2, -mu));
-            sum += s[t][n][i];
-          }
-        l[t] = fmaf(l[t], al, sum);
-        m[t] = mn;
-#pragma unroll
-        for (int d = 0; d < Dm::DT; ++d) o[t][d] *= al;
-      }
-#pragma unroll
-      for (int n = 0; n < 4; n += M::PT) {
-        typename M::Frag pf[QT];
-#pragma unroll
-        for (int t = 0; t < QT; ++t) pf[t] = M::pack(&s[t][n]);
-#pragma unroll
-        for (int d = 0; d < Dm::DT; ++d) {
-          const typename M::Frag f = M::tr(sv, Dm::PX, 16 * n, 16 * d, lane);
-#pragma unroll
-          for (int t = 0; t < QT; ++t) o[t][d] = M::mma(f, pf[t], o[t][d]);
-        }
-      }
-      if (safe && (flag[0] | flag[1])) {           // rare: what visible keys hold in the pieces that were zeroed
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-          for (int kk = 0; kk < 16; ++kk) {
-            const int key = 16 * n + kk;
-            if (!(flag[key >> 5] >> (key & 31) & 1u)) continue;
-            const T* vr = vp + (long long)(k0 + key) * a.vl;
-#pragma unroll
-            for (int t = 0; t < QT; ++t) {
-              const float mine = (kk & 3) == 0 ? s[t][n][0] : (kk & 3) == 1 ? s[t][n][1] : (kk & 3) == 2 ? s[t][n][2] : s[t][n][3];
-              const float p = __shfl(mine, j + 16 * (kk >> 2));
-#pragma unroll
-              for (int d = 0; d < Dm::DT; ++d) {
-                const int c = 16 * d + 4 * g, piece = c / M::EPC * M::EPC;
-                if (p == 0.f || c >= a.D || !nonfinite4(*reinterpret_cast<const float4*>(vr + piece), kind16<T>::v)) continue;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[t][d][i] += p * (float)vr[c + i];
-              }
+              for (int t = 0; t < QT; ++t) s[t][n] = M::mma(f, qf[t][k], s[t][n]);
             }
           }
+        }
+        if (a.mask != nullptr || parts < 4 || k0 + RR_XA_KT > seen) {
+#pragma unroll
+          for (int t = 0; t < QT; ++t)
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              keep4(s[t][n], first_bytes(a.mask != nullptr ? mb[t][n] : 0x01010101u, seen - (k0 + 16 * n + 4 * g)), -INFINITY);
+            }
+        }
+        // the running maximum moves only when a score passes it by 2^8: weights up to that are as exact as those up to one, and a tile
+        // that does not move it needs no exchange between the lanes of a row and no rescaling
+        float mx[QT];
+        bool move = false;
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+          mx[t] = s[t][0][0];
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx[t] = fmaxf(mx[t], s[t][n][i]);
+          move |= mx[t] * c2 > m[t] + 8.0f;
+        }
+        if (__any(move)) {
+#pragma unroll
+          for (int t = 0; t < QT; ++t) {
+            const float mn = fmaxf(m[t], group_max(mx[t]) * c2);
+            const float al = __builtin_amdgcn_exp2f(m[t] - finite_or_zero(mn));
+            l[t] *= al;
+            m[t] = mn;
+#pragma unroll
+            for (int d = 0; d < Dm::DT; ++d) o[t][d] *= al;
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+          const float mu = finite_or_zero(m[t]);
+          float sum = 0.f;
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              s[t][n][i] = __builtin_amdgcn_exp2f(fmaf(s[t][n][i], c2, -mu));
+              sum += s[t][n][i];
+            }
+          l[t] += sum;
+        }
+#pragma unroll
+        for (int n = 0; n < 4; n += M::PT) {
+          if (n >= parts) break;
+          typename M::Frag pf[QT];
+#pragma unroll
+          for (int t = 0; t < QT; ++t) pf[t] = M::pack(&s[t][n]);
+#pragma unroll
+          for (int d = 0; d < Dm::DT; ++d) {
+            const typename M::Frag f = M::tr(tv, Dm::PX, 16 * n, 16 * d, lane);
+#pragma unroll
+            for (int t = 0; t < QT; ++t) o[t][d] = M::mma(f, pf[t], o[t][d]);
+          }
+        }
+        const uint32_t* fl = flag[at];
+        if (safe && (fl[0] | fl[1])) {               // rare: what visible keys hold in the pieces that were zeroed
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+            for (int kk = 0; kk < 16; ++kk) {
+              const int key = 16 * n + kk;
+              if (!(fl[key >> 5] >> (key & 31) & 1u)) continue;
+              const T* vr = vrow(k0 + key);
+#pragma unroll
+              for (int t = 0; t < QT; ++t) {
+                const float mine = (kk & 3) == 0 ? s[t][n][0] : (kk & 3) == 1 ? s[t][n][1] : (kk & 3) == 2 ? s[t][n][2] : s[t][n][3];
+                const float p = __shfl(mine, j + 16 * (kk >> 2));
+#pragma unroll
+                for (int d = 0; d < Dm::DT; ++d) {
+                  const int c = 16 * d + 4 * g, piece = c / M::EPC * M::EPC;
+                  if (p == 0.f || c >= a.D || !nonfinite4(*reinterpret_cast<const float4*>(vr + piece), kind16<T>::v)) continue;
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) o[t][d][i] += p * (float)vr[c + i];
+                }
+              }
+            }
+        }
       }
+      if (more) {
+        if (safe) clear_flag(flag[at ^ 1]);
+        pk.template store<Dm::PR>(sk[at ^ 1], false, flag[at ^ 1]);
+        pv.template store<Dm::PX>(sv[at ^ 1], safe, flag[at ^ 1]);
+      }
+      __syncthreads();
     }
     bool bad = false;
 #pragma unroll
@@ -435,12 +511,12 @@ __global__ __launch_bounds__(256) void k_xattn_join(XAttn a) {
 
 // ------------------------------------------------------------------------------------------------ backward: dq (walks over the keys)
 template <typename T, int DP, int QT>
-__global__ __launch_bounds__(256) void k_xattn_dq(XAttn a) {
+__global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_dq(XAttn a) {
   using M = Mx<T>;
   using Dm = Dims<T, DP>;
-  __shared__ __attribute__((aligned(16))) T sk[RR_XA_KT * Dm::PX];
-  __shared__ __attribute__((aligned(16))) T sv[RR_XA_KT * Dm::PR];
-  __shared__ uint32_t flag[2];
+  __shared__ __attribute__((aligned(16))) T sk[2][RR_XA_KT * Dm::PX];
+  __shared__ __attribute__((aligned(16))) T sv[2][RR_XA_KT * Dm::PR];
+  __shared__ uint32_t flag[2][2];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
   const Blk w = block_of(a);
   const int R = a.G * a.Lq, H = a.G * a.Hk, row0 = (w.blk * 4 + wave) * 16 * QT;
@@ -448,6 +524,16 @@ __global__ __launch_bounds__(256) void k_xattn_dq(XAttn a) {
   const int seen = seen_keys(a, w.b);
   const T* kp = (const T*)a.k + (long long)w.b * a.kb + (long long)w.hk * a.kh;
   const T* vp = (const T*)a.v + (long long)w.b * a.vb + (long long)w.hk * a.vh;
+  auto krow = [&](int r) { return kp + (long long)r * a.kl; };
+  auto vrow = [&](int r) { return vp + (long long)r * a.vl; };
+  const int first = w.split * a.tiles_per_split * RR_XA_KT;
+  int last = first + a.tiles_per_split * RR_XA_KT;
+  last = last < seen ? last : seen;
+  Piece<T, DP> pk, pv;
+  if (first < last) {
+    pk.load(krow, first, seen, a.D);
+    pv.load(vrow, first, seen, a.D);
+  }
   typename M::Frag qf[QT][Dm::NK], gf[QT][Dm::NK];
   load_rows<T, DP, QT>(qf, (const T*)a.q + (long long)w.b * a.qb + (long long)w.hk * a.G * a.qh, a.ql, a.qh, row0, R, a, lane);
   load_rows<T, DP, QT>(gf, (const T*)a.dout + (long long)w.b * a.gb + (long long)w.hk * a.G * a.gh, a.gl, a.gh, row0, R, a, lane);
@@ -476,9 +562,6 @@ __global__ __launch_bounds__(256) void k_xattn_dq(XAttn a) {
     if (w.split == 0 && g == 0 && r < R) a.delta[li] = delta[t];
   }
   const float c2 = a.scale * RR_LOG2E;
-  const int first = w.split * a.tiles_per_split * RR_XA_KT;
-  int last = first + a.tiles_per_split * RR_XA_KT;
-  last = last < seen ? last : seen;
   f32x4 o[QT][Dm::DT];
   for (int pass = 0; pass < 2; ++pass) {
     const bool safe = pass == 1;
@@ -486,55 +569,84 @@ __global__ __launch_bounds__(256) void k_xattn_dq(XAttn a) {
     for (int t = 0; t < QT; ++t)
 #pragma unroll
       for (int d = 0; d < Dm::DT; ++d) o[t][d] = rr_zero4();
-    for (int k0 = first; k0 < last; k0 += RR_XA_KT) {
-      __syncthreads();
-      if (safe) {
-        if (threadIdx.x < 2) flag[threadIdx.x] = 0u;
-        __syncthreads();
+    if (safe) {
+      clear_flag(flag[0]);
+      pk.load(krow, first, seen, a.D);
+      pv.load(vrow, first, seen, a.D);
+    }
+    if (first < last) {
+      pk.template store<Dm::PX>(sk[0], safe, flag[0]);
+      pv.template store<Dm::PR>(sv[0], false, flag[0]);
+    }
+    __syncthreads();
+    int at = 0;
+    for (int k0 = first; k0 < last; k0 += RR_XA_KT, at ^= 1) {
+      const bool more = k0 + RR_XA_KT < last;
+      if (more) {
+        pk.load(krow, k0 + RR_XA_KT, seen, a.D);
+        pv.load(vrow, k0 + RR_XA_KT, seen, a.D);
       }
-      stage<T, DP, Dm::PX>(sk, [&](int r) { return kp + (long long)r * a.kl; }, k0, seen, a.D, safe, flag);
-      stage<T, DP, Dm::PR>(sv, [&](int r) { return vp + (long long)r * a.vl; }, k0, seen, a.D, false, flag);
-      __syncthreads();
-      if (!busy) continue;
+      if (busy) {
+        const T *tk = sk[at], *tv = sv[at];
+        const uint32_t* fl = flag[at];
+        const bool some = a.mask != nullptr || k0 + RR_XA_KT > seen || safe;      // (uniform) not every pair of the tile may be seen
+        uint32_t mb[QT][4];
+        if (a.mask != nullptr) {
 #pragma unroll
-      for (int n = 0; n < 4; n += M::PT) {
-        f32x4 s[QT][M::PT], dp[QT][M::PT];
+          for (int t = 0; t < QT; ++t)
 #pragma unroll
-        for (int u = 0; u < M::PT; ++u) {
-#pragma unroll
-          for (int t = 0; t < QT; ++t) { s[t][u] = rr_zero4(); dp[t][u] = rr_zero4(); }
-#pragma unroll
-          for (int k = 0; k < Dm::NK; ++k) {
-            const typename M::Frag fk = frag_at<T>(sk + (16 * (n + u) + j) * Dm::PX + k * M::KC + g * M::EPC);
-            const typename M::Frag fv = frag_at<T>(sv + (16 * (n + u) + j) * Dm::PR + k * M::KC + g * M::EPC);
-#pragma unroll
-            for (int t = 0; t < QT; ++t) { s[t][u] = M::mma(fk, qf[t][k], s[t][u]); dp[t][u] = M::mma(fv, gf[t][k], dp[t][u]); }
-          }
+            for (int n = 0; n < 4; ++n) mb[t][n] = mask4(mrow[t], k0 + 16 * n + 4 * g, a.Lk);
         }
-        typename M::Frag pf[QT];
 #pragma unroll
-        for (int t = 0; t < QT; ++t) {
+        for (int n = 0; n < 4; n += M::PT) {
+          if (k0 + 16 * n >= seen) break;
+          f32x4 s[QT][M::PT], dp[QT][M::PT];
 #pragma unroll
           for (int u = 0; u < M::PT; ++u) {
-            const int key = k0 + 16 * (n + u) + 4 * g;
-            const uint32_t mb = a.mask != nullptr ? mask4(mrow[t], key, a.Lk) : 0x01010101u;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const bool see = key + i < seen && (mb >> (8 * i) & 0xffu);
-              float p = __builtin_amdgcn_exp2f(fmaf(s[t][u][i], c2, -lse2[t]));
-              if (safe && (flag[(key + i - k0) >> 5] >> ((key + i - k0) & 31) & 1u)) p = __builtin_nanf("");     // a visible key that holds a non-finite value
-              s[t][u][i] = see ? p * (dp[t][u][i] - delta[t]) : 0.f;
+            for (int t = 0; t < QT; ++t) { s[t][u] = rr_zero4(); dp[t][u] = rr_zero4(); }
+#pragma unroll
+            for (int k = 0; k < Dm::NK; ++k) {
+              const typename M::Frag fk = frag_at<T>(tk + (16 * (n + u) + j) * Dm::PX + k * M::KC + g * M::EPC);
+              const typename M::Frag fv = frag_at<T>(tv + (16 * (n + u) + j) * Dm::PR + k * M::KC + g * M::EPC);
+#pragma unroll
+              for (int t = 0; t < QT; ++t) { s[t][u] = M::mma(fk, qf[t][k], s[t][u]); dp[t][u] = M::mma(fv, gf[t][k], dp[t][u]); }
             }
           }
-          pf[t] = M::pack(s[t]);
-        }
+          typename M::Frag pf[QT];
 #pragma unroll
-        for (int d = 0; d < Dm::DT; ++d) {
-          const typename M::Frag f = M::tr(sk, Dm::PX, 16 * n, 16 * d, lane);
+          for (int t = 0; t < QT; ++t) {
 #pragma unroll
-          for (int t = 0; t < QT; ++t) o[t][d] = M::mma(f, pf[t], o[t][d]);
+            for (int u = 0; u < M::PT; ++u)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[t][u][i], c2, -lse2[t]));
+                s[t][u][i] = p * (dp[t][u][i] - delta[t]);
+              }
+            if (some) {
+#pragma unroll
+              for (int u = 0; u < M::PT; ++u) {
+                const int key = 16 * (n + u) + 4 * g;
+                if (safe) keep4(s[t][u], ~(flag4(fl, key) * 0xffu), __builtin_nanf(""));      // a visible key that holds a non-finite value
+                keep4(s[t][u], first_bytes(a.mask != nullptr ? mb[t][n + u] : 0x01010101u, seen - (k0 + key)), 0.f);
+              }
+            }
+            pf[t] = M::pack(s[t]);
+          }
+#pragma unroll
+          for (int d = 0; d < Dm::DT; ++d) {
+            const typename M::Frag f = M::tr(tk, Dm::PX, 16 * n, 16 * d, lane);
+#pragma unroll
+            for (int t = 0; t < QT; ++t) o[t][d] = M::mma(f, pf[t], o[t][d]);
+          }
         }
       }
+      if (more) {
+        if (safe) clear_flag(flag[at ^ 1]);
+        pk.template store<Dm::PX>(sk[at ^ 1], safe, flag[at ^ 1]);
+        pv.template store<Dm::PR>(sv[at ^ 1], false, flag[at ^ 1]);
+      }
+      __syncthreads();
     }
     bool bad = false;
 #pragma unroll
@@ -573,24 +685,66 @@ __global__ __launch_bounds__(256) void k_xattn_dq(XAttn a) {
 
 // ------------------------------------------------------------------------------------------------ backward: dk, dv (walks over the rows)
 template <typename T, int DP, int KW>        // KW x 16 keys a wave
-__global__ __launch_bounds__(256) void k_xattn_dkv(XAttn a) {
+__global__ __launch_bounds__(256, (DP == 128 && (sizeof(T) == 4 || KW == 2) ? 1 : 2)) void k_xattn_dkv(XAttn a) {
   using M = Mx<T>;
   using Dm = Dims<T, DP>;
-  __shared__ __attribute__((aligned(16))) T sq[RR_XA_KT * Dm::PX];
-  __shared__ __attribute__((aligned(16))) T sg[RR_XA_KT * Dm::PX];
-  __shared__ float sl[RR_XA_KT], sd[RR_XA_KT];
-  __shared__ long long sm[RR_XA_KT];
-  __shared__ uint32_t flag[2];
+  constexpr int MP = RR_XA_KT + 4;           // a key's mask bytes of the tile's rows: a lane reads those of its four rows at once
+  __shared__ __attribute__((aligned(16))) T sq[2][RR_XA_KT * Dm::PX];
+  __shared__ __attribute__((aligned(16))) T sg[2][RR_XA_KT * Dm::PX];
+  __shared__ __attribute__((aligned(16))) float sl[2][RR_XA_KT], sd[2][RR_XA_KT];
+  __shared__ __attribute__((aligned(16))) uint8_t sm[2][64 * KW * MP];
+  __shared__ uint32_t flag[2][2];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
   const Blk w = block_of(a);
-  const int R = a.G * a.Lq, H = a.G * a.Hk, key0 = (w.blk * 4 + wave) * 16 * KW;
+  const int R = a.G * a.Lq, H = a.G * a.Hk, block0 = w.blk * 64 * KW, key0 = block0 + wave * 16 * KW;
   const int seen = seen_keys(a, w.b);
-  const bool block_seen = w.blk * 64 * KW < seen;                          // (uniform in the workgroup)
   const bool busy = key0 < seen;
   const T* kp = (const T*)a.k + (long long)w.b * a.kb + (long long)w.hk * a.kh;
   const T* vp = (const T*)a.v + (long long)w.b * a.vb + (long long)w.hk * a.vh;
   const T* qp = (const T*)a.q + (long long)w.b * a.qb + (long long)w.hk * a.G * a.qh;
   const T* gp = (const T*)a.dout + (long long)w.b * a.gb + (long long)w.hk * a.G * a.gh;
+  auto qrow = [&](int r) { const RowAt at = row_at(r, a.Lq, a.G); return qp + at.s * a.ql + at.g * a.qh; };
+  auto grow = [&](int r) { const RowAt at = row_at(r, a.Lq, a.G); return gp + at.s * a.gl + at.g * a.gh; };
+  const float c2 = a.scale * RR_LOG2E;
+  const int first = w.split * a.tiles_per_split * RR_XA_KT;
+  int last = first + a.tiles_per_split * RR_XA_KT;
+  last = block0 < seen ? (last < R ? last : R) : first;                  // (a workgroup behind the last key only writes zeros)
+  Piece<T, DP> pq, pg;
+  float nl = 0.f, nd = 0.f;                                              // the tile's lse (in powers of two) and delta, a row a thread
+  uint32_t nm[4 * KW];                                                   // its mask: four keys' bytes of a row, 4 KW times a thread
+  auto load_tile = [&](int r0) {
+    pq.load(qrow, r0, R, a.D);
+    pg.load(grow, r0, R, a.D);
+    if (threadIdx.x < RR_XA_KT) {
+      const int r = r0 + threadIdx.x;
+      const RowAt at = row_at(r < R ? r : R - 1, a.Lq, a.G);
+      const long long li = ((long long)w.b * H + w.hk * a.G + at.g) * a.Lq + at.s;
+      nl = a.lse[li] * RR_LOG2E;
+      nd = a.delta[li];
+    }
+    if (a.mask != nullptr) {
+#pragma unroll
+      for (int c = 0; c < 4 * KW; ++c) {
+        const int i = threadIdx.x + 256 * c, r = r0 + i / (16 * KW), key = block0 + i % (16 * KW) * 4;
+        const RowAt at = row_at(r < R ? r : R - 1, a.Lq, a.G);
+        nm[c] = mask4(a.mask + w.b * a.mb + (w.hk * a.G + at.g) * a.mh + at.s * a.ml, key, a.Lk);
+      }
+    }
+  };
+  auto store_tile = [&](int at, bool safe) {
+    pq.template store<Dm::PX>(sq[at], safe, flag[at]);
+    pg.template store<Dm::PX>(sg[at], safe, flag[at]);
+    if (threadIdx.x < RR_XA_KT) { sl[at][threadIdx.x] = nl; sd[at][threadIdx.x] = nd; }
+    if (a.mask != nullptr) {
+#pragma unroll
+      for (int c = 0; c < 4 * KW; ++c) {
+        const int i = threadIdx.x + 256 * c, r = i / (16 * KW), key = i % (16 * KW) * 4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sm[at][(key + e) * MP + r] = (uint8_t)(nm[c] >> (8 * e));
+      }
+    }
+  };
+  if (first < last) load_tile(first);
   typename M::Frag kf[KW][Dm::NK], vf[KW][Dm::NK];
 #pragma unroll
   for (int t = 0; t < KW; ++t) {
@@ -603,10 +757,6 @@ __global__ __launch_bounds__(256) void k_xattn_dkv(XAttn a) {
       vf[t][k] = in ? frag_at<T>(vp + (long long)key * a.vl + c) : frag_zero<T>();
     }
   }
-  const float c2 = a.scale * RR_LOG2E;
-  const int first = w.split * a.tiles_per_split * RR_XA_KT;
-  int last = first + a.tiles_per_split * RR_XA_KT;
-  last = last < R ? last : R;
   f32x4 ok[KW][Dm::DT], ov[KW][Dm::DT];
   for (int pass = 0; pass < 2; ++pass) {
     const bool safe = pass == 1;
@@ -614,68 +764,86 @@ __global__ __launch_bounds__(256) void k_xattn_dkv(XAttn a) {
     for (int t = 0; t < KW; ++t)
 #pragma unroll
       for (int d = 0; d < Dm::DT; ++d) { ok[t][d] = rr_zero4(); ov[t][d] = rr_zero4(); }
-    for (int r0 = first; r0 < last && block_seen; r0 += RR_XA_KT) {
-      __syncthreads();
-      if (safe) {
-        if (threadIdx.x < 2) flag[threadIdx.x] = 0u;
-        __syncthreads();
-      }
-      stage<T, DP, Dm::PX>(sq, [&](int r) { const RowAt at = row_at(r, a.Lq, a.G); return qp + at.s * a.ql + at.g * a.qh; }, r0, R, a.D, safe, flag);
-      stage<T, DP, Dm::PX>(sg, [&](int r) { const RowAt at = row_at(r, a.Lq, a.G); return gp + at.s * a.gl + at.g * a.gh; }, r0, R, a.D, safe, flag);
-      if (threadIdx.x < RR_XA_KT) {
-        const int r = r0 + threadIdx.x;
-        const RowAt at = row_at(r < R ? r : R - 1, a.Lq, a.G);
-        const int head = w.hk * a.G + at.g;
-        const long long li = ((long long)w.b * H + head) * a.Lq + at.s;
-        sl[threadIdx.x] = r < R ? a.lse[li] * RR_LOG2E : 0.f;
-        sd[threadIdx.x] = r < R ? a.delta[li] : 0.f;
-        sm[threadIdx.x] = w.b * a.mb + head * a.mh + at.s * a.ml;
-      }
-      __syncthreads();
-      if (!busy) continue;
+    if (safe) {
+      clear_flag(flag[0]);
+      load_tile(first);
+    }
+    if (first < last) store_tile(0, safe);
+    __syncthreads();
+    int at = 0;
+    for (int r0 = first; r0 < last; r0 += RR_XA_KT, at ^= 1) {
+      const bool more = r0 + RR_XA_KT < last;
+      if (more) load_tile(r0 + RR_XA_KT);
+      if (busy) {
+        const T *tq = sq[at], *tg = sg[at];
+        const uint32_t* fl = flag[at];
+        const bool some = a.mask != nullptr || r0 + RR_XA_KT > R || block0 + 64 * KW > seen || safe;      // (uniform)
 #pragma unroll
-      for (int n = 0; n < 4; n += M::PT) {
-        f32x4 s[KW][M::PT], dp[KW][M::PT];
+        for (int n = 0; n < 4; n += M::PT) {
+          if (r0 + 16 * n >= R) break;
+          f32x4 s[KW][M::PT], dp[KW][M::PT];
 #pragma unroll
-        for (int u = 0; u < M::PT; ++u) {
+          for (int u = 0; u < M::PT; ++u) {
 #pragma unroll
-          for (int t = 0; t < KW; ++t) { s[t][u] = rr_zero4(); dp[t][u] = rr_zero4(); }
+            for (int t = 0; t < KW; ++t) { s[t][u] = rr_zero4(); dp[t][u] = rr_zero4(); }
 #pragma unroll
-          for (int k = 0; k < Dm::NK; ++k) {
-            const typename M::Frag fq = frag_at<T>(sq + (16 * (n + u) + j) * Dm::PX + k * M::KC + g * M::EPC);
-            const typename M::Frag fg = frag_at<T>(sg + (16 * (n + u) + j) * Dm::PX + k * M::KC + g * M::EPC);
+            for (int k = 0; k < Dm::NK; ++k) {
+              const typename M::Frag fq = frag_at<T>(tq + (16 * (n + u) + j) * Dm::PX + k * M::KC + g * M::EPC);
+              const typename M::Frag fg = frag_at<T>(tg + (16 * (n + u) + j) * Dm::PX + k * M::KC + g * M::EPC);
 #pragma unroll
-            for (int t = 0; t < KW; ++t) { s[t][u] = M::mma(fq, kf[t][k], s[t][u]); dp[t][u] = M::mma(fg, vf[t][k], dp[t][u]); }
+              for (int t = 0; t < KW; ++t) { s[t][u] = M::mma(fq, kf[t][k], s[t][u]); dp[t][u] = M::mma(fg, vf[t][k], dp[t][u]); }
+            }
+          }
+          f32x4 ls[M::PT], de[M::PT];
+#pragma unroll
+          for (int u = 0; u < M::PT; ++u) {
+            ls[u] = *reinterpret_cast<const f32x4*>(&sl[at][16 * (n + u) + 4 * g]);
+            de[u] = *reinterpret_cast<const f32x4*>(&sd[at][16 * (n + u) + 4 * g]);
+          }
+          typename M::Frag pf[KW], df[KW];
+#pragma unroll
+          for (int t = 0; t < KW; ++t) {
+#pragma unroll
+            for (int u = 0; u < M::PT; ++u)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[t][u][i], c2, -ls[u][i]));
+                dp[t][u][i] = p * (dp[t][u][i] - de[u][i]);
+                s[t][u][i] = p;
+              }
+            if (some) {
+              const int key = key0 + 16 * t + j;
+#pragma unroll
+              for (int u = 0; u < M::PT; ++u) {
+                const int rr = 16 * (n + u) + 4 * g;                     // rows of the tile
+                uint32_t b = a.mask != nullptr ? *reinterpret_cast<const uint32_t*>(&sm[at][(key - block0) * MP + rr]) : 0x01010101u;
+                b = key < seen ? first_bytes(b, R - (r0 + rr)) : 0u;
+                if (safe) {                                              // a row that holds a non-finite value
+                  const uint32_t fine = ~(flag4(fl, rr) * 0xffu);
+                  keep4(s[t][u], fine, __builtin_nanf(""));
+                  keep4(dp[t][u], fine, __builtin_nanf(""));
+                }
+                keep4(s[t][u], b, 0.f);
+                keep4(dp[t][u], b, 0.f);
+              }
+            }
+            pf[t] = M::pack(s[t]);
+            df[t] = M::pack(dp[t]);
+          }
+#pragma unroll
+          for (int d = 0; d < Dm::DT; ++d) {
+            const typename M::Frag fg = M::tr(tg, Dm::PX, 16 * n, 16 * d, lane);
+            const typename M::Frag fq = M::tr(tq, Dm::PX, 16 * n, 16 * d, lane);
+#pragma unroll
+            for (int t = 0; t < KW; ++t) { ov[t][d] = M::mma(fg, pf[t], ov[t][d]); ok[t][d] = M::mma(fq, df[t], ok[t][d]); }
           }
         }
-        typename M::Frag pf[KW], df[KW];
-#pragma unroll
-        for (int t = 0; t < KW; ++t) {
-          const int key = key0 + 16 * t + j;
-#pragma unroll
-          for (int u = 0; u < M::PT; ++u)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int rr = 16 * (n + u) + 4 * g + i;                     // row of the tile
-              bool see = key < seen && r0 + rr < R;
-              if (see && a.mask != nullptr) see = a.mask[sm[rr] + key] != 0;
-              float p = __builtin_amdgcn_exp2f(fmaf(s[t][u][i], c2, -sl[rr]));
-              if (safe && (flag[rr >> 5] >> (rr & 31) & 1u)) p = __builtin_nanf("");
-              const float d = p * (dp[t][u][i] - sd[rr]);
-              s[t][u][i] = see ? p : 0.f;
-              dp[t][u][i] = see ? d : 0.f;
-            }
-          pf[t] = M::pack(s[t]);
-          df[t] = M::pack(dp[t]);
-        }
-#pragma unroll
-        for (int d = 0; d < Dm::DT; ++d) {
-          const typename M::Frag fg = M::tr(sg, Dm::PX, 16 * n, 16 * d, lane);
-          const typename M::Frag fq = M::tr(sq, Dm::PX, 16 * n, 16 * d, lane);
-#pragma unroll
-          for (int t = 0; t < KW; ++t) { ov[t][d] = M::mma(fg, pf[t], ov[t][d]); ok[t][d] = M::mma(fq, df[t], ok[t][d]); }
-        }
       }
+      if (more) {
+        if (safe) clear_flag(flag[at ^ 1]);
+        store_tile(at ^ 1, safe);
+      }
+      __syncthreads();
     }
     bool bad = false;
 #pragma unroll
@@ -734,10 +902,11 @@ int head_pad(int D) { return D <= 16 ? 16 : D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
 // rows (or keys) of a workgroup: 4 waves of 16 or 32
 struct Plan { int wide, nblk, nsplit, tiles_per_split; };
-Plan plan_for(long long kept, long long walked, long long outer) {
+Plan plan_for(long long kept, long long walked, long long outer, bool f32) {
   Plan p;
-  // 32 rows a wave read each staged tile half as often; 16 where that leaves less than a workgroup for each CU
-  p.wide = kept > 64 && outer * ((kept + 127) / 128) >= 256 ? 2 : 1;
+  // 16-bit types: with 16 rows a wave the reads of the staged tiles take LDS twice as long as the products take the matrix pipe, with 32 as long.
+  // float32 products are eight times slower: 16 rows, more waves
+  p.wide = !f32 && kept > 64 ? 2 : 1;
   p.nblk = (int)((kept + 64 * p.wide - 1) / (64 * p.wide));
   const long long tiles = (walked + RR_XA_KT - 1) / RR_XA_KT;
   const long long blocks = outer * p.nblk;
@@ -756,8 +925,10 @@ Plan plan_for(long long kept, long long walked, long long outer) {
 template <typename T, int DP>
 int fwd_go(XAttn& a, const Plan& p, hipStream_t st) {
   const dim3 grid((unsigned)((long long)a.B * a.Hk * p.nsplit * p.nblk));
-  if (p.wide == 2) hipLaunchKernelGGL((k_xattn_fwd<T, DP, 2>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((k_xattn_fwd<T, DP, 1>), grid, dim3(256), 0, st, a);
+  if constexpr (sizeof(T) == 2) {
+    if (p.wide == 2) hipLaunchKernelGGL((k_xattn_fwd<T, DP, 2>), grid, dim3(256), 0, st, a);
+  }
+  if (p.wide == 1) hipLaunchKernelGGL((k_xattn_fwd<T, DP, 1>), grid, dim3(256), 0, st, a);
   if (p.nsplit > 1) hipLaunchKernelGGL((k_xattn_join<T, DP>), dim3((unsigned)(((long long)a.B * a.Hk * a.G * a.Lq + 3) / 4)), dim3(256), 0, st, a);
   return xa_launched();
 }
@@ -765,15 +936,19 @@ template <typename T, int DP>
 int bwd_go(XAttn& a, const Plan& p, const Plan& pk, hipStream_t st) {
   const dim3 grid((unsigned)((long long)a.B * a.Hk * p.nsplit * p.nblk));
   a.nsplit = p.nsplit; a.tiles_per_split = p.tiles_per_split; a.nblk = p.nblk;
-  if (p.wide == 2) hipLaunchKernelGGL((k_xattn_dq<T, DP, 2>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((k_xattn_dq<T, DP, 1>), grid, dim3(256), 0, st, a);
+  if constexpr (sizeof(T) == 2) {
+    if (p.wide == 2) hipLaunchKernelGGL((k_xattn_dq<T, DP, 2>), grid, dim3(256), 0, st, a);
+  }
+  if (p.wide == 1) hipLaunchKernelGGL((k_xattn_dq<T, DP, 1>), grid, dim3(256), 0, st, a);
   const long long nq4 = (long long)a.B * a.Lq * a.Hk * a.G * a.D / 4, nk4 = (long long)a.B * a.Lk * a.Hk * a.D / 4;
   auto blocks = [](long long n) { return dim3((unsigned)(n / 256 + 1 < 4096 ? n / 256 + 1 : 4096)); };
   if (p.nsplit > 1) hipLaunchKernelGGL((k_xattn_add<T>), blocks(nq4), dim3(256), 0, st, a.part, 4 * nq4, p.nsplit, (T*)a.dq, nq4);
   a.nsplit = pk.nsplit; a.tiles_per_split = pk.tiles_per_split; a.nblk = pk.nblk;
   const dim3 gk((unsigned)((long long)a.B * a.Hk * pk.nsplit * pk.nblk));
-  if (pk.wide == 2) hipLaunchKernelGGL((k_xattn_dkv<T, DP, 2>), gk, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((k_xattn_dkv<T, DP, 1>), gk, dim3(256), 0, st, a);
+  if constexpr (sizeof(T) == 2) {
+    if (pk.wide == 2) hipLaunchKernelGGL((k_xattn_dkv<T, DP, 2>), gk, dim3(256), 0, st, a);
+  }
+  if (pk.wide == 1) hipLaunchKernelGGL((k_xattn_dkv<T, DP, 1>), gk, dim3(256), 0, st, a);
   if (pk.nsplit > 1) {
     hipLaunchKernelGGL((k_xattn_add<T>), blocks(nk4), dim3(256), 0, st, a.part, 8 * nk4, pk.nsplit, (T*)a.dk, nk4);
     hipLaunchKernelGGL((k_xattn_add<T>), blocks(nk4), dim3(256), 0, st, a.part + 4 * nk4, 8 * nk4, pk.nsplit, (T*)a.dv, nk4);
@@ -782,15 +957,15 @@ int bwd_go(XAttn& a, const Plan& p, const Plan& pk, hipStream_t st) {
 }
 
 struct Sizes { Plan q, k; size_t fwd, bwd; bool ok; };
-Sizes sizes_of(long long B, long long Lq, long long Lk, long long Hk, long long G, int D) {
+Sizes sizes_of(long long B, long long Lq, long long Lk, long long Hk, long long G, int D, int dtype) {
   Sizes s{};
   const long long lim = 0x7fffffffLL;
   // counts that index rows, keys and workgroups are 32-bit; offsets into the tensors are 64-bit
   s.ok = B >= 1 && Lq >= 1 && Lk >= 0 && Hk >= 1 && G >= 1 && D >= 8 && D <= 128 && D % 8 == 0 && Lq <= lim && Lk <= lim - 256 && G * Lq <= lim - 256 && B <= lim && Hk <= lim &&
          B * Hk <= lim && G * Hk <= lim;
   if (!s.ok) return s;
-  s.q = plan_for(G * Lq, Lk, B * Hk);
-  s.k = plan_for(Lk > 0 ? Lk : 1, G * Lq, B * Hk);
+  s.q = plan_for(G * Lq, Lk, B * Hk, dtype == RR_F32);
+  s.k = plan_for(Lk > 0 ? Lk : 1, G * Lq, B * Hk, dtype == RR_F32);
   if (B * Hk * s.q.nblk > lim / 256 || B * Hk * s.k.nblk > lim / 256 || B * Hk * G * Lq > lim) { s.ok = false; return s; }
   const int DP = head_pad(D);
   s.fwd = s.q.nsplit > 1 ? (size_t)(B * Hk * G * Lq) * s.q.nsplit * (DP + 4) * 4 : 0;
@@ -843,8 +1018,8 @@ static int xa_fill(const XAttnIO* io, XAttn& a, bool bwd) {
   return RR_OK;
 }
 
-extern "C" long long rr_cross_attn_workspace(int B, int Lq, int Lk, int Hk, int G, int D, int backward) {
-  const Sizes s = sizes_of(B, Lq, Lk, Hk, G, D);
+extern "C" long long rr_cross_attn_workspace(int dtype, int B, int Lq, int Lk, int Hk, int G, int D, int backward) {
+  const Sizes s = sizes_of(B, Lq, Lk, Hk, G, D, dtype);
   return s.ok ? (long long)(backward ? s.bwd : s.fwd) : -1;
 }
 
@@ -858,7 +1033,7 @@ extern "C" long long rr_cross_attn_workspace(int B, int Lq, int Lk, int Hk, int 
 
 extern "C" int rr_cross_attn(const XAttnIO* io, hipStream_t st) {
   if (io == nullptr) return RR_EINVAL;
-  const Sizes s = sizes_of(io->B, io->Lq, io->Lk, io->Hk, io->G, io->D);
+  const Sizes s = sizes_of(io->B, io->Lq, io->Lk, io->Hk, io->G, io->D, io->dtype);
   XAttn a;
   if (!s.ok || xa_fill(io, a, false) != RR_OK || (s.fwd > 0 && (io->workspace == nullptr || (size_t)io->workspace_bytes < s.fwd || !rr_aligned16(io->workspace)))) return RR_EINVAL;
   a.nsplit = s.q.nsplit; a.tiles_per_split = s.q.tiles_per_split; a.nblk = s.q.nblk;
@@ -871,7 +1046,7 @@ extern "C" int rr_cross_attn(const XAttnIO* io, hipStream_t st) {
 
 extern "C" int rr_cross_attn_bwd(const XAttnIO* io, hipStream_t st) {
   if (io == nullptr || io->Lk < 1) return RR_EINVAL;
-  const Sizes s = sizes_of(io->B, io->Lq, io->Lk, io->Hk, io->G, io->D);
+  const Sizes s = sizes_of(io->B, io->Lq, io->Lk, io->Hk, io->G, io->D, io->dtype);
   XAttn a;
   if (!s.ok || xa_fill(io, a, true) != RR_OK || (s.bwd > 0 && (io->workspace == nullptr || (size_t)io->workspace_bytes < s.bwd || !rr_aligned16(io->workspace)))) return RR_EINVAL;
 #define RR_CALL(T, DP) bwd_go<T, DP>(a, s.q, s.k, st)

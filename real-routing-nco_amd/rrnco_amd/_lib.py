@@ -193,7 +193,7 @@ def lib():
             fn.restype = i32
         _lib.rr_matnet_workspace_bytes.argtypes = [i32] * 4
         _lib.rr_matnet_workspace_bytes.restype = C.c_size_t
-        _lib.rr_cross_attn_workspace.argtypes = [i32] * 7
+        _lib.rr_cross_attn_workspace.argtypes = [i32] * 8
         _lib.rr_cross_attn_workspace.restype = C.c_longlong
         _lib.rr_draw_workspace.argtypes = [i32] * 2
         _lib.rr_draw_workspace.restype = C.c_longlong
