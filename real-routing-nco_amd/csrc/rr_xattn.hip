@@ -245,7 +245,10 @@ __device__ __forceinline__ void load_rows(F& f, const T* base, long long sl, lon
 
 struct Blk { int b, hk, split, blk; };
 __device__ __forceinline__ Blk block_of(const XAttn& a) {
-  long long i = blockIdx.x;
+  // workgroups go to the eight XCDs in turn: each gets one stretch of the work, so that the heads of an instance, which share its cache lines and
+  // its mask, meet in one L2
+  const unsigned n = gridDim.x, x = blockIdx.x & 7u, q = n >> 3, r = n & 7u;
+  long long i = x * q + (x < r ? x : r) + (blockIdx.x >> 3);
   Blk w;
   w.blk = (int)(i % a.nblk); i /= a.nblk;
   w.split = (int)(i % a.nsplit); i /= a.nsplit;
@@ -473,41 +476,41 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_fwd(XAttn a) {
   }
 }
 
-// joins the splits of a row: one wave a row, the lanes its columns
+// joins the splits of a row: DP / 4 lanes a row, four columns each
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void k_xattn_join(XAttn a) {
-  const int lane = threadIdx.x & 63;
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  constexpr int LPR = DP / 4;
+  const int c = threadIdx.x % LPR * 4;
+  const long long row = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
   const int R = a.G * a.Lq;
   if (row >= (long long)a.B * a.Hk * R) return;
   const float* p = a.part + row * a.nsplit * (DP + 4);
   float m = -INFINITY;
-  for (int i = lane; i < a.nsplit; i += 64) m = fmaxf(m, p[i * (DP + 4) + DP]);
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+  for (int i = 0; i < a.nsplit; ++i) m = fmaxf(m, p[i * (DP + 4) + DP]);
   const float mu = finite_or_zero(m);
-  float acc[(DP + 63) / 64], l = 0.f;
-#pragma unroll
-  for (int c = 0; c < (DP + 63) / 64; ++c) acc[c] = 0.f;
+  f32x4 acc = rr_zero4();
+  float l = 0.f;
+#pragma unroll 4
   for (int i = 0; i < a.nsplit; ++i) {
     const float* pi = p + i * (DP + 4);
-    const float f = __builtin_amdgcn_exp2f(pi[DP] - mu);
-    l = fmaf(pi[DP + 1], f, l);
+    const float mi = pi[DP], li = pi[DP + 1], f = __builtin_amdgcn_exp2f(mi - mu);
+    const f32x4 v = *reinterpret_cast<const f32x4*>(pi + c);
+    l = fmaf(li, f, l);
 #pragma unroll
-    for (int c = 0; c < (DP + 63) / 64; ++c)
-      if (lane + 64 * c < DP) acc[c] = pi[DP] == -INFINITY ? acc[c] : fmaf(pi[lane + 64 * c], f, acc[c]);
+    for (int e = 0; e < 4; ++e) acc[e] = mi == -INFINITY ? acc[e] : fmaf(v[e], f, acc[e]);
   }
   const int b = (int)(row / ((long long)a.Hk * R)), hk = (int)(row / R % a.Hk);
   const RowAt at = row_at((int)(row % R), a.Lq, a.G);
   const int head = hk * a.G + at.g;
   const float inv = l == 0.f ? 0.f : 1.0f / l;
   T* dst = (T*)a.out + (((long long)b * a.Lq + at.s) * (a.Hk * a.G) + head) * a.D;
-#pragma unroll
-  for (int c = 0; c < (DP + 63) / 64; ++c)
-    if (lane + 64 * c < a.D) dst[lane + 64 * c] = (T)(acc[c] * inv);
-  if (a.lse != nullptr && lane == 0) a.lse[((long long)b * (a.Hk * a.G) + head) * a.Lq + at.s] = l == 0.f ? -INFINITY : (m + __log2f(l)) * RR_LN2;
+  if (c < a.D) {
+    typedef T V4 __attribute__((ext_vector_type(4)));
+    const V4 v = {(T)(acc[0] * inv), (T)(acc[1] * inv), (T)(acc[2] * inv), (T)(acc[3] * inv)};
+    *reinterpret_cast<V4*>(dst + c) = v;
+  }
+  if (a.lse != nullptr && c == 0) a.lse[((long long)b * (a.Hk * a.G) + head) * a.Lq + at.s] = l == 0.f ? -INFINITY : (m + __log2f(l)) * RR_LN2;
 }
-
 
 // ------------------------------------------------------------------------------------------------ backward: dq (walks over the keys)
 template <typename T, int DP, int QT>
@@ -910,8 +913,10 @@ Plan plan_for(long long kept, long long walked, long long outer, bool f32) {
   p.nblk = (int)((kept + 64 * p.wide - 1) / (64 * p.wide));
   const long long tiles = (walked + RR_XA_KT - 1) / RR_XA_KT;
   const long long blocks = outer * p.nblk;
-  // few workgroups: the walked axis is split until about three fill each of the 256 CUs, four tiles a split at the least
-  long long split = blocks >= 512 ? 1 : (768 + blocks - 1) / blocks;
+  // fewer workgroups than CUs: the walked axis is split, four tiles a split at the least.  A workgroup of many rows writes much for the joining
+  // launch: two for each CU; one of few rows hardly any: eight, which also evens out ragged lengths
+  const long long target = kept > 64 ? 512 : 2048;
+  long long split = blocks >= (kept > 64 ? 256 : 512) ? 1 : (target + blocks - 1) / blocks;
   if (split > tiles / 4) split = tiles / 4;
   if (split < 1) split = 1;
   if (split > 256) split = 256;
@@ -929,7 +934,7 @@ int fwd_go(XAttn& a, const Plan& p, hipStream_t st) {
     if (p.wide == 2) hipLaunchKernelGGL((k_xattn_fwd<T, DP, 2>), grid, dim3(256), 0, st, a);
   }
   if (p.wide == 1) hipLaunchKernelGGL((k_xattn_fwd<T, DP, 1>), grid, dim3(256), 0, st, a);
-  if (p.nsplit > 1) hipLaunchKernelGGL((k_xattn_join<T, DP>), dim3((unsigned)(((long long)a.B * a.Hk * a.G * a.Lq + 3) / 4)), dim3(256), 0, st, a);
+  if (p.nsplit > 1) hipLaunchKernelGGL((k_xattn_join<T, DP>), dim3((unsigned)(((long long)a.B * a.Hk * a.G * a.Lq + 1024 / DP - 1) / (1024 / DP))), dim3(256), 0, st, a);
   return xa_launched();
 }
 template <typename T, int DP>
