@@ -17,6 +17,8 @@
 // Non-finite values where nothing may look (a masked key whose value is NaN): 0 * NaN would spoil the products, so a workgroup
 // whose accumulators end non-finite walks its tiles once more with the non-finite 16-byte pieces replaced by zeros and their
 // contribution to the rows that do see them put back: a masked key never shows, a visible one does.
+#include <type_traits>
+
 #include "rr_types.h"
 
 namespace {
@@ -154,13 +156,19 @@ struct Piece {
   using Dm = Dims<T, DP>;
   static constexpr int N = RR_XA_KT * Dm::CPR / 256;
   float4 v[N];
-  template <typename PTR>
-  __device__ __forceinline__ void load(PTR rowptr, int row0, int valid, int D) {
+  // base: the tile's first row, ld: elements from row to row; rows: how many exist from there on.  A thread's pieces lie 256 / CPR rows apart.
+  __device__ __forceinline__ void load(const T* base, long long ld, int rows, int D) {
+    const int row = threadIdx.x / Dm::CPR, col = threadIdx.x % Dm::CPR * Mx<T>::EPC;
+    const long long off = row * ld + col;
+    if (rows >= RR_XA_KT && D == Dm::KD) {                               // (uniform: a whole tile needs no conditions)
 #pragma unroll
-    for (int c = 0; c < N; ++c) {
-      const int i = threadIdx.x + 256 * c, row = i / Dm::CPR, ch = i % Dm::CPR;
-      v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (row0 + row < valid && ch * Mx<T>::EPC < D) v[c] = *reinterpret_cast<const float4*>(rowptr(row0 + row) + ch * Mx<T>::EPC);
+      for (int c = 0; c < N; ++c) v[c] = *reinterpret_cast<const float4*>(base + c * (256 / Dm::CPR) * ld + off);
+    } else {
+#pragma unroll
+      for (int c = 0; c < N; ++c) {
+        v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (row + c * (256 / Dm::CPR) < rows && col < D) v[c] = *reinterpret_cast<const float4*>(base + c * (256 / Dm::CPR) * ld + off);
+      }
     }
   }
   // safe: pieces that hold a non-finite value become zeros and their row's bit is set in `flag`
@@ -259,12 +267,18 @@ __device__ __forceinline__ Blk block_of(const XAttn& a) {
 
 // ------------------------------------------------------------------------------------------------ forward
 // registers: two waves a SIMD, except where 128-wide float32 rows need more
+// Variants near the register limit keep the reads of one 16-key step behind those of the step before (hoisted further, they spill)
+template <bool TIGHT>
+__device__ __forceinline__ void in_order() {
+  if constexpr (TIGHT) __builtin_amdgcn_sched_barrier(0);
+}
 template <typename T, int DP> struct Waves { static constexpr int N = sizeof(T) == 4 && DP == 128 ? 1 : 2; };
 
 template <typename T, int DP, int QT>
 __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_fwd(XAttn a) {
   using M = Mx<T>;
   using Dm = Dims<T, DP>;
+  constexpr bool TIGHT = DP == 128 && QT == 2, SKIP = sizeof(T) == 4;
   __shared__ __attribute__((aligned(16))) T sk[2][RR_XA_KT * Dm::PR];
   __shared__ __attribute__((aligned(16))) T sv[2][RR_XA_KT * Dm::PX];
   __shared__ uint32_t flag[2][2];
@@ -282,8 +296,8 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_fwd(XAttn a) {
   last = last < seen ? last : seen;
   Piece<T, DP> pk, pv;
   if (first < last) {
-    pk.load(krow, first, seen, a.D);
-    pv.load(vrow, first, seen, a.D);
+    pk.load(krow(first), a.kl, seen - first, a.D);
+    pv.load(vrow(first), a.vl, seen - first, a.D);
   }
   typename M::Frag qf[QT][Dm::NK];
   load_rows<T, DP, QT>(qf, (const T*)a.q + (long long)w.b * a.qb + (long long)w.hk * a.G * a.qh, a.ql, a.qh, row0, R, a, lane);
@@ -297,140 +311,144 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_fwd(XAttn a) {
   const float c2 = a.scale * RR_LOG2E;
   f32x4 o[QT][Dm::DT];
   float m[QT], l[QT];
-  for (int pass = 0; pass < 2; ++pass) {
-    const bool safe = pass == 1;
+  // one staged tile; `safe`: second walk.  float32 skips 16-key tiles behind the last key; 16-bit types compute them and drop the scores: branches between the
+  // tiles keep the reads of the next one from being issued early, which costs more than the products
+  auto tile = [&](auto safe, int k0, int at) {
+    const T *tk = sk[at], *tv = sv[at];
+    uint32_t mb[QT][4];
+    if (a.mask != nullptr) {
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) mb[t][n] = mask4(mrow[t], k0 + 16 * n + 4 * g, a.Lk);
+    }
+    const int parts = SKIP ? (seen - k0 + 15) >> 4 : 4;
+    f32x4 s[QT][4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+#pragma unroll
+      for (int t = 0; t < QT; ++t) s[t][n] = rr_zero4();
+      if (!SKIP || n < parts) {
+#pragma unroll
+        for (int k = 0; k < Dm::NK; ++k) {
+          const typename M::Frag f = frag_at<T>(tk + (16 * n + j) * Dm::PR + k * M::KC + g * M::EPC);
+#pragma unroll
+          for (int t = 0; t < QT; ++t) s[t][n] = M::mma(f, qf[t][k], s[t][n]);
+        }
+      }
+      in_order<TIGHT>();
+    }
+    if (a.mask != nullptr || k0 + RR_XA_KT > seen) {
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          keep4(s[t][n], first_bytes(a.mask != nullptr ? mb[t][n] : 0x01010101u, seen - (k0 + 16 * n + 4 * g)), -INFINITY);
+        }
+    }
+    // the running maximum moves only when a score passes it by 2^8: weights up to that are as exact as those up to one, and a tile
+    // that does not move it needs no exchange between the lanes of a row and no rescaling
+    float mx[QT];
+    bool move = false;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      mx[t] = s[t][0][0];
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx[t] = fmaxf(mx[t], s[t][n][i]);
+      move |= mx[t] * c2 > m[t] + 8.0f;
+    }
+    if (__any(move)) {
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        const float mn = fmaxf(m[t], group_max(mx[t]) * c2);
+        const float al = __builtin_amdgcn_exp2f(m[t] - finite_or_zero(mn));
+        l[t] *= al;
+        m[t] = mn;
+#pragma unroll
+        for (int d = 0; d < Dm::DT; ++d) o[t][d] *= al;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      const float mu = finite_or_zero(m[t]);
+      float sum = 0.f;
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[t][n][i] = __builtin_amdgcn_exp2f(fmaf(s[t][n][i], c2, -mu));
+          sum += s[t][n][i];
+        }
+      l[t] += sum;
+    }
+#pragma unroll
+    for (int n = 0; n < 4; n += M::PT) {
+      if (SKIP && n >= parts) break;
+      typename M::Frag pf[QT];
+#pragma unroll
+      for (int t = 0; t < QT; ++t) pf[t] = M::pack(&s[t][n]);
+#pragma unroll
+      for (int d = 0; d < Dm::DT; ++d) {
+        const typename M::Frag f = M::tr(tv, Dm::PX, 16 * n, 16 * d, lane);
+#pragma unroll
+        for (int t = 0; t < QT; ++t) o[t][d] = M::mma(f, pf[t], o[t][d]);
+        if ((d & 3) == 3) in_order<TIGHT>();
+      }
+    }
+    const uint32_t* fl = flag[at];
+    if constexpr (safe()) if (fl[0] | fl[1]) {               // rare: what visible keys hold in the pieces that were zeroed
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+        for (int kk = 0; kk < 16; ++kk) {
+          const int key = 16 * n + kk;
+          if (!(fl[key >> 5] >> (key & 31) & 1u)) continue;
+          const T* vr = vrow(k0 + key);
+#pragma unroll
+          for (int t = 0; t < QT; ++t) {
+            const float mine = (kk & 3) == 0 ? s[t][n][0] : (kk & 3) == 1 ? s[t][n][1] : (kk & 3) == 2 ? s[t][n][2] : s[t][n][3];
+            const float p = __shfl(mine, j + 16 * (kk >> 2));
+#pragma unroll
+            for (int d = 0; d < Dm::DT; ++d) {
+              const int c = 16 * d + 4 * g, piece = c / M::EPC * M::EPC;
+              if (p == 0.f || c >= a.D || !nonfinite4(*reinterpret_cast<const float4*>(vr + piece), kind16<T>::v)) continue;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) o[t][d][i] += p * (float)vr[c + i];
+            }
+          }
+        }
+    }
+  };
+  auto walk = [&](auto safe) {
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
       m[t] = -INFINITY; l[t] = 0.f;
 #pragma unroll
       for (int d = 0; d < Dm::DT; ++d) o[t][d] = rr_zero4();
     }
-    if (safe) {
+    if constexpr (safe()) {
       clear_flag(flag[0]);
-      pk.load(krow, first, seen, a.D);
-      pv.load(vrow, first, seen, a.D);
+      pk.load(krow(first), a.kl, seen - first, a.D);
+      pv.load(vrow(first), a.vl, seen - first, a.D);
     }
     if (first < last) {
       pk.template store<Dm::PR>(sk[0], false, flag[0]);
-      pv.template store<Dm::PX>(sv[0], safe, flag[0]);
+      pv.template store<Dm::PX>(sv[0], safe(), flag[0]);
     }
     __syncthreads();
     int at = 0;
     for (int k0 = first; k0 < last; k0 += RR_XA_KT, at ^= 1) {
       const bool more = k0 + RR_XA_KT < last;
       if (more) {
-        pk.load(krow, k0 + RR_XA_KT, seen, a.D);
-        pv.load(vrow, k0 + RR_XA_KT, seen, a.D);
+        pk.load(krow(k0 + RR_XA_KT), a.kl, seen - k0 - RR_XA_KT, a.D);
+        pv.load(vrow(k0 + RR_XA_KT), a.vl, seen - k0 - RR_XA_KT, a.D);
       }
-      if (busy) {
-        const T *tk = sk[at], *tv = sv[at];
-        uint32_t mb[QT][4];
-        if (a.mask != nullptr) {
-#pragma unroll
-          for (int t = 0; t < QT; ++t)
-#pragma unroll
-            for (int n = 0; n < 4; ++n) mb[t][n] = mask4(mrow[t], k0 + 16 * n + 4 * g, a.Lk);
-        }
-        const int parts = (seen - k0 + 15) >> 4;           // 16-key tiles that hold a key; whole tiles take the straight path
-        f32x4 s[QT][4];
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-#pragma unroll
-          for (int t = 0; t < QT; ++t) s[t][n] = rr_zero4();
-          if (n < parts) {
-#pragma unroll
-            for (int k = 0; k < Dm::NK; ++k) {
-              const typename M::Frag f = frag_at<T>(tk + (16 * n + j) * Dm::PR + k * M::KC + g * M::EPC);
-#pragma unroll
-              for (int t = 0; t < QT; ++t) s[t][n] = M::mma(f, qf[t][k], s[t][n]);
-            }
-          }
-        }
-        if (a.mask != nullptr || parts < 4 || k0 + RR_XA_KT > seen) {
-#pragma unroll
-          for (int t = 0; t < QT; ++t)
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-              keep4(s[t][n], first_bytes(a.mask != nullptr ? mb[t][n] : 0x01010101u, seen - (k0 + 16 * n + 4 * g)), -INFINITY);
-            }
-        }
-        // the running maximum moves only when a score passes it by 2^8: weights up to that are as exact as those up to one, and a tile
-        // that does not move it needs no exchange between the lanes of a row and no rescaling
-        float mx[QT];
-        bool move = false;
-#pragma unroll
-        for (int t = 0; t < QT; ++t) {
-          mx[t] = s[t][0][0];
-#pragma unroll
-          for (int n = 0; n < 4; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) mx[t] = fmaxf(mx[t], s[t][n][i]);
-          move |= mx[t] * c2 > m[t] + 8.0f;
-        }
-        if (__any(move)) {
-#pragma unroll
-          for (int t = 0; t < QT; ++t) {
-            const float mn = fmaxf(m[t], group_max(mx[t]) * c2);
-            const float al = __builtin_amdgcn_exp2f(m[t] - finite_or_zero(mn));
-            l[t] *= al;
-            m[t] = mn;
-#pragma unroll
-            for (int d = 0; d < Dm::DT; ++d) o[t][d] *= al;
-          }
-        }
-#pragma unroll
-        for (int t = 0; t < QT; ++t) {
-          const float mu = finite_or_zero(m[t]);
-          float sum = 0.f;
-#pragma unroll
-          for (int n = 0; n < 4; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              s[t][n][i] = __builtin_amdgcn_exp2f(fmaf(s[t][n][i], c2, -mu));
-              sum += s[t][n][i];
-            }
-          l[t] += sum;
-        }
-#pragma unroll
-        for (int n = 0; n < 4; n += M::PT) {
-          if (n >= parts) break;
-          typename M::Frag pf[QT];
-#pragma unroll
-          for (int t = 0; t < QT; ++t) pf[t] = M::pack(&s[t][n]);
-#pragma unroll
-          for (int d = 0; d < Dm::DT; ++d) {
-            const typename M::Frag f = M::tr(tv, Dm::PX, 16 * n, 16 * d, lane);
-#pragma unroll
-            for (int t = 0; t < QT; ++t) o[t][d] = M::mma(f, pf[t], o[t][d]);
-          }
-        }
-        const uint32_t* fl = flag[at];
-        if (safe && (fl[0] | fl[1])) {               // rare: what visible keys hold in the pieces that were zeroed
-#pragma unroll
-          for (int n = 0; n < 4; ++n)
-            for (int kk = 0; kk < 16; ++kk) {
-              const int key = 16 * n + kk;
-              if (!(fl[key >> 5] >> (key & 31) & 1u)) continue;
-              const T* vr = vrow(k0 + key);
-#pragma unroll
-              for (int t = 0; t < QT; ++t) {
-                const float mine = (kk & 3) == 0 ? s[t][n][0] : (kk & 3) == 1 ? s[t][n][1] : (kk & 3) == 2 ? s[t][n][2] : s[t][n][3];
-                const float p = __shfl(mine, j + 16 * (kk >> 2));
-#pragma unroll
-                for (int d = 0; d < Dm::DT; ++d) {
-                  const int c = 16 * d + 4 * g, piece = c / M::EPC * M::EPC;
-                  if (p == 0.f || c >= a.D || !nonfinite4(*reinterpret_cast<const float4*>(vr + piece), kind16<T>::v)) continue;
-#pragma unroll
-                  for (int i = 0; i < 4; ++i) o[t][d][i] += p * (float)vr[c + i];
-                }
-              }
-            }
-        }
-      }
+      if (busy) tile(safe, k0, at);
       if (more) {
-        if (safe) clear_flag(flag[at ^ 1]);
+        if constexpr (safe()) clear_flag(flag[at ^ 1]);
         pk.template store<Dm::PR>(sk[at ^ 1], false, flag[at ^ 1]);
-        pv.template store<Dm::PX>(sv[at ^ 1], safe, flag[at ^ 1]);
+        pv.template store<Dm::PX>(sv[at ^ 1], safe(), flag[at ^ 1]);
       }
       __syncthreads();
     }
@@ -441,8 +459,9 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_fwd(XAttn a) {
       for (int d = 0; d < Dm::DT; ++d)
 #pragma unroll
         for (int i = 0; i < 4; ++i) bad |= is_bad(o[t][d][i]);
-    if (!__syncthreads_or(bad && busy)) break;
-  }
+    return __syncthreads_or(bad && busy);
+  };
+  if (walk(std::false_type{})) walk(std::true_type{});
   if (!busy) return;
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
@@ -517,6 +536,7 @@ template <typename T, int DP, int QT>
 __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_dq(XAttn a) {
   using M = Mx<T>;
   using Dm = Dims<T, DP>;
+  constexpr bool TIGHT = DP == 128 && QT == 2, SKIP = sizeof(T) == 4;
   __shared__ __attribute__((aligned(16))) T sk[2][RR_XA_KT * Dm::PX];
   __shared__ __attribute__((aligned(16))) T sv[2][RR_XA_KT * Dm::PR];
   __shared__ uint32_t flag[2][2];
@@ -534,8 +554,8 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_dq(XAttn a) {
   last = last < seen ? last : seen;
   Piece<T, DP> pk, pv;
   if (first < last) {
-    pk.load(krow, first, seen, a.D);
-    pv.load(vrow, first, seen, a.D);
+    pk.load(krow(first), a.kl, seen - first, a.D);
+    pv.load(vrow(first), a.vl, seen - first, a.D);
   }
   typename M::Frag qf[QT][Dm::NK], gf[QT][Dm::NK];
   load_rows<T, DP, QT>(qf, (const T*)a.q + (long long)w.b * a.qb + (long long)w.hk * a.G * a.qh, a.ql, a.qh, row0, R, a, lane);
@@ -566,19 +586,76 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_dq(XAttn a) {
   }
   const float c2 = a.scale * RR_LOG2E;
   f32x4 o[QT][Dm::DT];
-  for (int pass = 0; pass < 2; ++pass) {
-    const bool safe = pass == 1;
+  // keys behind the last one are staged as zeros: whatever their weight, they add nothing (unless it overflows, which the second walk sorts out)
+  auto tile = [&](auto safe, int k0, int at) {
+    const T *tk = sk[at], *tv = sv[at];
+    const uint32_t* fl = flag[at];
+    const bool some = a.mask != nullptr || safe();      // (uniform) not every pair of the tile may be seen
+    uint32_t mb[QT][4];
+    if (a.mask != nullptr) {
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) mb[t][n] = mask4(mrow[t], k0 + 16 * n + 4 * g, a.Lk);
+    }
+#pragma unroll
+    for (int n = 0; n < 4; n += M::PT) {
+      if (SKIP && k0 + 16 * n >= seen) break;
+      f32x4 s[QT][M::PT], dp[QT][M::PT];
+#pragma unroll
+      for (int u = 0; u < M::PT; ++u) {
+#pragma unroll
+        for (int t = 0; t < QT; ++t) { s[t][u] = rr_zero4(); dp[t][u] = rr_zero4(); }
+#pragma unroll
+        for (int k = 0; k < Dm::NK; ++k) {
+          const typename M::Frag fk = frag_at<T>(tk + (16 * (n + u) + j) * Dm::PX + k * M::KC + g * M::EPC);
+          const typename M::Frag fv = frag_at<T>(tv + (16 * (n + u) + j) * Dm::PR + k * M::KC + g * M::EPC);
+#pragma unroll
+          for (int t = 0; t < QT; ++t) { s[t][u] = M::mma(fk, qf[t][k], s[t][u]); dp[t][u] = M::mma(fv, gf[t][k], dp[t][u]); }
+        }
+        in_order<TIGHT>();
+      }
+      typename M::Frag pf[QT];
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+#pragma unroll
+        for (int u = 0; u < M::PT; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(s[t][u][i], c2, -lse2[t]));
+            s[t][u][i] = p * (dp[t][u][i] - delta[t]);
+          }
+        if (some) {
+#pragma unroll
+          for (int u = 0; u < M::PT; ++u) {
+            const int key = 16 * (n + u) + 4 * g;
+            if constexpr (safe()) keep4(s[t][u], ~(flag4(fl, key) * 0xffu), __builtin_nanf(""));      // a visible key that holds a non-finite value
+            keep4(s[t][u], first_bytes(a.mask != nullptr ? mb[t][n + u] : 0x01010101u, seen - (k0 + key)), 0.f);
+          }
+        }
+        pf[t] = M::pack(s[t]);
+      }
+#pragma unroll
+      for (int d = 0; d < Dm::DT; ++d) {
+        const typename M::Frag f = M::tr(tk, Dm::PX, 16 * n, 16 * d, lane);
+#pragma unroll
+        for (int t = 0; t < QT; ++t) o[t][d] = M::mma(f, pf[t], o[t][d]);
+        if ((d & 3) == 3) in_order<TIGHT>();
+      }
+    }
+  };
+  auto walk = [&](auto safe) {
 #pragma unroll
     for (int t = 0; t < QT; ++t)
 #pragma unroll
       for (int d = 0; d < Dm::DT; ++d) o[t][d] = rr_zero4();
-    if (safe) {
+    if constexpr (safe()) {
       clear_flag(flag[0]);
-      pk.load(krow, first, seen, a.D);
-      pv.load(vrow, first, seen, a.D);
+      pk.load(krow(first), a.kl, seen - first, a.D);
+      pv.load(vrow(first), a.vl, seen - first, a.D);
     }
     if (first < last) {
-      pk.template store<Dm::PX>(sk[0], safe, flag[0]);
+      pk.template store<Dm::PX>(sk[0], safe(), flag[0]);
       pv.template store<Dm::PR>(sv[0], false, flag[0]);
     }
     __syncthreads();
@@ -586,67 +663,13 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_dq(XAttn a) {
     for (int k0 = first; k0 < last; k0 += RR_XA_KT, at ^= 1) {
       const bool more = k0 + RR_XA_KT < last;
       if (more) {
-        pk.load(krow, k0 + RR_XA_KT, seen, a.D);
-        pv.load(vrow, k0 + RR_XA_KT, seen, a.D);
+        pk.load(krow(k0 + RR_XA_KT), a.kl, seen - k0 - RR_XA_KT, a.D);
+        pv.load(vrow(k0 + RR_XA_KT), a.vl, seen - k0 - RR_XA_KT, a.D);
       }
-      if (busy) {
-        const T *tk = sk[at], *tv = sv[at];
-        const uint32_t* fl = flag[at];
-        const bool some = a.mask != nullptr || k0 + RR_XA_KT > seen || safe;      // (uniform) not every pair of the tile may be seen
-        uint32_t mb[QT][4];
-        if (a.mask != nullptr) {
-#pragma unroll
-          for (int t = 0; t < QT; ++t)
-#pragma unroll
-            for (int n = 0; n < 4; ++n) mb[t][n] = mask4(mrow[t], k0 + 16 * n + 4 * g, a.Lk);
-        }
-#pragma unroll
-        for (int n = 0; n < 4; n += M::PT) {
-          if (k0 + 16 * n >= seen) break;
-          f32x4 s[QT][M::PT], dp[QT][M::PT];
-#pragma unroll
-          for (int u = 0; u < M::PT; ++u) {
-#pragma unroll
-            for (int t = 0; t < QT; ++t) { s[t][u] = rr_zero4(); dp[t][u] = rr_zero4(); }
-#pragma unroll
-            for (int k = 0; k < Dm::NK; ++k) {
-              const typename M::Frag fk = frag_at<T>(tk + (16 * (n + u) + j) * Dm::PX + k * M::KC + g * M::EPC);
-              const typename M::Frag fv = frag_at<T>(tv + (16 * (n + u) + j) * Dm::PR + k * M::KC + g * M::EPC);
-#pragma unroll
-              for (int t = 0; t < QT; ++t) { s[t][u] = M::mma(fk, qf[t][k], s[t][u]); dp[t][u] = M::mma(fv, gf[t][k], dp[t][u]); }
-            }
-          }
-          typename M::Frag pf[QT];
-#pragma unroll
-          for (int t = 0; t < QT; ++t) {
-#pragma unroll
-            for (int u = 0; u < M::PT; ++u)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(s[t][u][i], c2, -lse2[t]));
-                s[t][u][i] = p * (dp[t][u][i] - delta[t]);
-              }
-            if (some) {
-#pragma unroll
-              for (int u = 0; u < M::PT; ++u) {
-                const int key = 16 * (n + u) + 4 * g;
-                if (safe) keep4(s[t][u], ~(flag4(fl, key) * 0xffu), __builtin_nanf(""));      // a visible key that holds a non-finite value
-                keep4(s[t][u], first_bytes(a.mask != nullptr ? mb[t][n + u] : 0x01010101u, seen - (k0 + key)), 0.f);
-              }
-            }
-            pf[t] = M::pack(s[t]);
-          }
-#pragma unroll
-          for (int d = 0; d < Dm::DT; ++d) {
-            const typename M::Frag f = M::tr(tk, Dm::PX, 16 * n, 16 * d, lane);
-#pragma unroll
-            for (int t = 0; t < QT; ++t) o[t][d] = M::mma(f, pf[t], o[t][d]);
-          }
-        }
-      }
+      if (busy) tile(safe, k0, at);
       if (more) {
-        if (safe) clear_flag(flag[at ^ 1]);
-        pk.template store<Dm::PX>(sk[at ^ 1], safe, flag[at ^ 1]);
+        if constexpr (safe()) clear_flag(flag[at ^ 1]);
+        pk.template store<Dm::PX>(sk[at ^ 1], safe(), flag[at ^ 1]);
         pv.template store<Dm::PR>(sv[at ^ 1], false, flag[at ^ 1]);
       }
       __syncthreads();
@@ -658,8 +681,9 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_dq(XAttn a) {
       for (int d = 0; d < Dm::DT; ++d)
 #pragma unroll
         for (int i = 0; i < 4; ++i) bad |= is_bad(o[t][d][i]);
-    if (!__syncthreads_or(bad && busy)) break;
-  }
+    return __syncthreads_or(bad && busy);
+  };
+  if (walk(std::false_type{})) walk(std::true_type{});
   if (!busy) return;
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
@@ -691,6 +715,7 @@ template <typename T, int DP, int KW>        // KW x 16 keys a wave
 __global__ __launch_bounds__(256, (DP == 128 && (sizeof(T) == 4 || KW == 2) ? 1 : 2)) void k_xattn_dkv(XAttn a) {
   using M = Mx<T>;
   using Dm = Dims<T, DP>;
+  constexpr bool TIGHT = DP >= 64 && KW == 2, SKIP = sizeof(T) == 4;
   constexpr int MP = RR_XA_KT + 4;           // a key's mask bytes of the tile's rows: a lane reads those of its four rows at once
   __shared__ __attribute__((aligned(16))) T sq[2][RR_XA_KT * Dm::PX];
   __shared__ __attribute__((aligned(16))) T sg[2][RR_XA_KT * Dm::PX];
@@ -699,38 +724,37 @@ __global__ __launch_bounds__(256, (DP == 128 && (sizeof(T) == 4 || KW == 2) ? 1 
   __shared__ uint32_t flag[2][2];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
   const Blk w = block_of(a);
-  const int R = a.G * a.Lq, H = a.G * a.Hk, block0 = w.blk * 64 * KW, key0 = block0 + wave * 16 * KW;
+  const int H = a.G * a.Hk, per_head = (a.Lq + RR_XA_KT - 1) / RR_XA_KT, block0 = w.blk * 64 * KW, key0 = block0 + wave * 16 * KW;
   const int seen = seen_keys(a, w.b);
   const bool busy = key0 < seen;
   const T* kp = (const T*)a.k + (long long)w.b * a.kb + (long long)w.hk * a.kh;
   const T* vp = (const T*)a.v + (long long)w.b * a.vb + (long long)w.hk * a.vh;
   const T* qp = (const T*)a.q + (long long)w.b * a.qb + (long long)w.hk * a.G * a.qh;
   const T* gp = (const T*)a.dout + (long long)w.b * a.gb + (long long)w.hk * a.G * a.gh;
-  auto qrow = [&](int r) { const RowAt at = row_at(r, a.Lq, a.G); return qp + at.s * a.ql + at.g * a.qh; };
-  auto grow = [&](int r) { const RowAt at = row_at(r, a.Lq, a.G); return gp + at.s * a.gl + at.g * a.gh; };
   const float c2 = a.scale * RR_LOG2E;
-  const int first = w.split * a.tiles_per_split * RR_XA_KT;
-  int last = first + a.tiles_per_split * RR_XA_KT;
-  last = block0 < seen ? (last < R ? last : R) : first;                  // (a workgroup behind the last key only writes zeros)
+  // the walked tiles: 64 positions of one head of the group each, head after head
+  const int first = w.split * a.tiles_per_split;
+  int last = first + a.tiles_per_split;
+  last = block0 < seen ? (last < a.G * per_head ? last : a.G * per_head) : first;      // (a workgroup behind the last key only writes zeros)
   Piece<T, DP> pq, pg;
   float nl = 0.f, nd = 0.f;                                              // the tile's lse (in powers of two) and delta, a row a thread
   uint32_t nm[4 * KW];                                                   // its mask: four keys' bytes of a row, 4 KW times a thread
-  auto load_tile = [&](int r0) {
-    pq.load(qrow, r0, R, a.D);
-    pg.load(grow, r0, R, a.D);
+  auto load_tile = [&](int tile) {
+    const int h = tile / per_head, s0 = (tile - h * per_head) * RR_XA_KT, rows = a.Lq - s0, head = w.hk * a.G + h;
+    pq.load(qp + h * a.qh + s0 * a.ql, a.ql, rows, a.D);
+    pg.load(gp + h * a.gh + s0 * a.gl, a.gl, rows, a.D);
     if (threadIdx.x < RR_XA_KT) {
-      const int r = r0 + threadIdx.x;
-      const RowAt at = row_at(r < R ? r : R - 1, a.Lq, a.G);
-      const long long li = ((long long)w.b * H + w.hk * a.G + at.g) * a.Lq + at.s;
-      nl = a.lse[li] * RR_LOG2E;
-      nd = a.delta[li];
+      const long long li = ((long long)w.b * H + head) * a.Lq + s0 + ((int)threadIdx.x < rows ? (int)threadIdx.x : rows - 1);
+      nl = (int)threadIdx.x < rows ? a.lse[li] * RR_LOG2E : INFINITY;
+      nd = (int)threadIdx.x < rows ? a.delta[li] : 0.f;
     }
     if (a.mask != nullptr) {
+      const uint8_t* mp = a.mask + w.b * a.mb + head * a.mh + s0 * a.ml;
+      const int key = block0 + threadIdx.x % (16 * KW) * 4;
 #pragma unroll
       for (int c = 0; c < 4 * KW; ++c) {
-        const int i = threadIdx.x + 256 * c, r = r0 + i / (16 * KW), key = block0 + i % (16 * KW) * 4;
-        const RowAt at = row_at(r < R ? r : R - 1, a.Lq, a.G);
-        nm[c] = mask4(a.mask + w.b * a.mb + (w.hk * a.G + at.g) * a.mh + at.s * a.ml, key, a.Lk);
+        const int r = threadIdx.x / (16 * KW) + c * (256 / (16 * KW));
+        nm[c] = mask4(mp + (r < rows ? r : rows - 1) * a.ml, key, a.Lk);
       }
     }
   };
@@ -741,7 +765,7 @@ __global__ __launch_bounds__(256, (DP == 128 && (sizeof(T) == 4 || KW == 2) ? 1 
     if (a.mask != nullptr) {
 #pragma unroll
       for (int c = 0; c < 4 * KW; ++c) {
-        const int i = threadIdx.x + 256 * c, r = i / (16 * KW), key = i % (16 * KW) * 4;
+        const int r = threadIdx.x / (16 * KW) + c * (256 / (16 * KW)), key = threadIdx.x % (16 * KW) * 4;
 #pragma unroll
         for (int e = 0; e < 4; ++e) sm[at][(key + e) * MP + r] = (uint8_t)(nm[c] >> (8 * e));
       }
@@ -761,90 +785,94 @@ __global__ __launch_bounds__(256, (DP == 128 && (sizeof(T) == 4 || KW == 2) ? 1 
     }
   }
   f32x4 ok[KW][Dm::DT], ov[KW][Dm::DT];
-  for (int pass = 0; pass < 2; ++pass) {
-    const bool safe = pass == 1;
+  // one staged tile of rows.  Rows behind the last one are zeros with an lse of infinity: their weights are zero.  Keys behind the last one hold zeros; what
+  // they collect is not written
+  auto tile = [&](auto safe, int rows, int at) {
+    const T *tq = sq[at], *tg = sg[at];
+    const uint32_t* fl = flag[at];
+    const bool some = a.mask != nullptr || safe();      // (uniform)
+#pragma unroll
+    for (int n = 0; n < 4; n += M::PT) {
+      if (SKIP && 16 * n >= rows) break;
+      f32x4 s[KW][M::PT], dp[KW][M::PT];
+#pragma unroll
+      for (int u = 0; u < M::PT; ++u) {
+#pragma unroll
+        for (int t = 0; t < KW; ++t) { s[t][u] = rr_zero4(); dp[t][u] = rr_zero4(); }
+#pragma unroll
+        for (int k = 0; k < Dm::NK; ++k) {
+          const typename M::Frag fq = frag_at<T>(tq + (16 * (n + u) + j) * Dm::PX + k * M::KC + g * M::EPC);
+          const typename M::Frag fg = frag_at<T>(tg + (16 * (n + u) + j) * Dm::PX + k * M::KC + g * M::EPC);
+#pragma unroll
+          for (int t = 0; t < KW; ++t) { s[t][u] = M::mma(fq, kf[t][k], s[t][u]); dp[t][u] = M::mma(fg, vf[t][k], dp[t][u]); }
+        }
+        in_order<TIGHT>();
+      }
+      f32x4 ls[M::PT], de[M::PT];
+#pragma unroll
+      for (int u = 0; u < M::PT; ++u) {
+        ls[u] = *reinterpret_cast<const f32x4*>(&sl[at][16 * (n + u) + 4 * g]);
+        de[u] = *reinterpret_cast<const f32x4*>(&sd[at][16 * (n + u) + 4 * g]);
+      }
+      typename M::Frag pf[KW], df[KW];
+#pragma unroll
+      for (int t = 0; t < KW; ++t) {
+#pragma unroll
+        for (int u = 0; u < M::PT; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(s[t][u][i], c2, -ls[u][i]));
+            dp[t][u][i] = p * (dp[t][u][i] - de[u][i]);
+            s[t][u][i] = p;
+          }
+        if (some) {
+          const int key = key0 + 16 * t + j;
+#pragma unroll
+          for (int u = 0; u < M::PT; ++u) {
+            const int rr = 16 * (n + u) + 4 * g;                     // rows of the tile
+            uint32_t b = a.mask != nullptr ? *reinterpret_cast<const uint32_t*>(&sm[at][(key - block0) * MP + rr]) : 0x01010101u;
+            b = key < seen ? first_bytes(b, rows - rr) : 0u;
+            if constexpr (safe()) {                                              // a row that holds a non-finite value
+              const uint32_t fine = ~(flag4(fl, rr) * 0xffu);
+              keep4(s[t][u], fine, __builtin_nanf(""));
+              keep4(dp[t][u], fine, __builtin_nanf(""));
+            }
+            keep4(s[t][u], b, 0.f);
+            keep4(dp[t][u], b, 0.f);
+          }
+        }
+        pf[t] = M::pack(s[t]);
+        df[t] = M::pack(dp[t]);
+      }
+#pragma unroll
+      for (int d = 0; d < Dm::DT; ++d) {
+        const typename M::Frag fg = M::tr(tg, Dm::PX, 16 * n, 16 * d, lane);
+        const typename M::Frag fq = M::tr(tq, Dm::PX, 16 * n, 16 * d, lane);
+#pragma unroll
+        for (int t = 0; t < KW; ++t) { ov[t][d] = M::mma(fg, pf[t], ov[t][d]); ok[t][d] = M::mma(fq, df[t], ok[t][d]); }
+        if ((d & 1) == 1) in_order<TIGHT>();
+      }
+    }
+  };
+  auto walk = [&](auto safe) {
 #pragma unroll
     for (int t = 0; t < KW; ++t)
 #pragma unroll
       for (int d = 0; d < Dm::DT; ++d) { ok[t][d] = rr_zero4(); ov[t][d] = rr_zero4(); }
-    if (safe) {
+    if constexpr (safe()) {
       clear_flag(flag[0]);
       load_tile(first);
     }
-    if (first < last) store_tile(0, safe);
+    if (first < last) store_tile(0, safe());
     __syncthreads();
     int at = 0;
-    for (int r0 = first; r0 < last; r0 += RR_XA_KT, at ^= 1) {
-      const bool more = r0 + RR_XA_KT < last;
-      if (more) load_tile(r0 + RR_XA_KT);
-      if (busy) {
-        const T *tq = sq[at], *tg = sg[at];
-        const uint32_t* fl = flag[at];
-        const bool some = a.mask != nullptr || r0 + RR_XA_KT > R || block0 + 64 * KW > seen || safe;      // (uniform)
-#pragma unroll
-        for (int n = 0; n < 4; n += M::PT) {
-          if (r0 + 16 * n >= R) break;
-          f32x4 s[KW][M::PT], dp[KW][M::PT];
-#pragma unroll
-          for (int u = 0; u < M::PT; ++u) {
-#pragma unroll
-            for (int t = 0; t < KW; ++t) { s[t][u] = rr_zero4(); dp[t][u] = rr_zero4(); }
-#pragma unroll
-            for (int k = 0; k < Dm::NK; ++k) {
-              const typename M::Frag fq = frag_at<T>(tq + (16 * (n + u) + j) * Dm::PX + k * M::KC + g * M::EPC);
-              const typename M::Frag fg = frag_at<T>(tg + (16 * (n + u) + j) * Dm::PX + k * M::KC + g * M::EPC);
-#pragma unroll
-              for (int t = 0; t < KW; ++t) { s[t][u] = M::mma(fq, kf[t][k], s[t][u]); dp[t][u] = M::mma(fg, vf[t][k], dp[t][u]); }
-            }
-          }
-          f32x4 ls[M::PT], de[M::PT];
-#pragma unroll
-          for (int u = 0; u < M::PT; ++u) {
-            ls[u] = *reinterpret_cast<const f32x4*>(&sl[at][16 * (n + u) + 4 * g]);
-            de[u] = *reinterpret_cast<const f32x4*>(&sd[at][16 * (n + u) + 4 * g]);
-          }
-          typename M::Frag pf[KW], df[KW];
-#pragma unroll
-          for (int t = 0; t < KW; ++t) {
-#pragma unroll
-            for (int u = 0; u < M::PT; ++u)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(s[t][u][i], c2, -ls[u][i]));
-                dp[t][u][i] = p * (dp[t][u][i] - de[u][i]);
-                s[t][u][i] = p;
-              }
-            if (some) {
-              const int key = key0 + 16 * t + j;
-#pragma unroll
-              for (int u = 0; u < M::PT; ++u) {
-                const int rr = 16 * (n + u) + 4 * g;                     // rows of the tile
-                uint32_t b = a.mask != nullptr ? *reinterpret_cast<const uint32_t*>(&sm[at][(key - block0) * MP + rr]) : 0x01010101u;
-                b = key < seen ? first_bytes(b, R - (r0 + rr)) : 0u;
-                if (safe) {                                              // a row that holds a non-finite value
-                  const uint32_t fine = ~(flag4(fl, rr) * 0xffu);
-                  keep4(s[t][u], fine, __builtin_nanf(""));
-                  keep4(dp[t][u], fine, __builtin_nanf(""));
-                }
-                keep4(s[t][u], b, 0.f);
-                keep4(dp[t][u], b, 0.f);
-              }
-            }
-            pf[t] = M::pack(s[t]);
-            df[t] = M::pack(dp[t]);
-          }
-#pragma unroll
-          for (int d = 0; d < Dm::DT; ++d) {
-            const typename M::Frag fg = M::tr(tg, Dm::PX, 16 * n, 16 * d, lane);
-            const typename M::Frag fq = M::tr(tq, Dm::PX, 16 * n, 16 * d, lane);
-#pragma unroll
-            for (int t = 0; t < KW; ++t) { ov[t][d] = M::mma(fg, pf[t], ov[t][d]); ok[t][d] = M::mma(fq, df[t], ok[t][d]); }
-          }
-        }
-      }
+    for (int i = first; i < last; ++i, at ^= 1) {
+      const bool more = i + 1 < last;
+      if (more) load_tile(i + 1);
+      if (busy) tile(safe, a.Lq - i % per_head * RR_XA_KT, at);
       if (more) {
-        if (safe) clear_flag(flag[at ^ 1]);
-        store_tile(at ^ 1, safe);
+        if constexpr (safe()) clear_flag(flag[at ^ 1]);
+        store_tile(at ^ 1, safe());
       }
       __syncthreads();
     }
@@ -854,9 +882,10 @@ __global__ __launch_bounds__(256, (DP == 128 && (sizeof(T) == 4 || KW == 2) ? 1 
 #pragma unroll
       for (int d = 0; d < Dm::DT; ++d)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) bad |= is_bad(ok[t][d][i]) || is_bad(ov[t][d][i]);
-    if (!__syncthreads_or(bad && busy)) break;
-  }
+        for (int i = 0; i < 4; ++i) bad |= key0 + 16 * t + j < seen && (is_bad(ok[t][d][i]) || is_bad(ov[t][d][i]));
+    return __syncthreads_or(bad && busy);
+  };
+  if (walk(std::false_type{})) walk(std::true_type{});
 #pragma unroll
   for (int t = 0; t < KW; ++t) {
     const int key = key0 + 16 * t + j;
@@ -868,7 +897,7 @@ __global__ __launch_bounds__(256, (DP == 128 && (sizeof(T) == 4 || KW == 2) ? 1 
     for (int d = 0; d < Dm::DT; ++d) {
       const int c = 16 * d + 4 * g;
       if (c >= a.D) continue;
-      const f32x4 xk = ok[t][d] * a.scale, xv = ov[t][d];
+      const f32x4 zero = rr_zero4(), xk = key < seen ? ok[t][d] * a.scale : zero, xv = key < seen ? ov[t][d] : zero;
       if (a.nsplit > 1) {
         *reinterpret_cast<f32x4*>(p + c) = xk;
         *reinterpret_cast<f32x4*>(p + half + c) = xv;
@@ -966,11 +995,11 @@ Sizes sizes_of(long long B, long long Lq, long long Lk, long long Hk, long long 
   Sizes s{};
   const long long lim = 0x7fffffffLL;
   // counts that index rows, keys and workgroups are 32-bit; offsets into the tensors are 64-bit
-  s.ok = B >= 1 && Lq >= 1 && Lk >= 0 && Hk >= 1 && G >= 1 && D >= 8 && D <= 128 && D % 8 == 0 && Lq <= lim && Lk <= lim - 256 && G * Lq <= lim - 256 && B <= lim && Hk <= lim &&
+  s.ok = B >= 1 && Lq >= 1 && Lk >= 0 && Hk >= 1 && G >= 1 && D >= 8 && D <= 128 && D % 8 == 0 && Lq <= lim && Lk <= lim - 256 && G * (Lq + 64) <= lim - 256 && B <= lim && Hk <= lim &&
          B * Hk <= lim && G * Hk <= lim;
   if (!s.ok) return s;
   s.q = plan_for(G * Lq, Lk, B * Hk, dtype == RR_F32);
-  s.k = plan_for(Lk > 0 ? Lk : 1, G * Lq, B * Hk, dtype == RR_F32);
+  s.k = plan_for(Lk > 0 ? Lk : 1, G * ((Lq + RR_XA_KT - 1) / RR_XA_KT) * RR_XA_KT, B * Hk, dtype == RR_F32);
   if (B * Hk * s.q.nblk > lim / 256 || B * Hk * s.k.nblk > lim / 256 || B * Hk * G * Lq > lim) { s.ok = false; return s; }
   const int DP = head_pad(D);
   s.fwd = s.q.nsplit > 1 ? (size_t)(B * Hk * G * Lq) * s.q.nsplit * (DP + 4) * 4 : 0;
