@@ -32,21 +32,30 @@ __device__ __forceinline__ float team_sum(float v, float* red) {          // red
   return v;
 }
 
-template <int N>
-__device__ __forceinline__ void load_w(const void* w, int w_is_f32, int dtype, long c, bool vec, float (&x)[N]) {
-  if (w == nullptr) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = 1.f;
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    x[i] = (w_is_f32 || dtype == RR_F32) ? ((const float*)w)[c + i] : dtype == RR_F16 ? (float)((const rr_f16*)w)[c + i] : (float)((const rr_bf16*)w)[c + i];
-}
 template <typename T> struct code;
 template <> struct code<float> { static constexpr int v = RR_F32; };
 template <> struct code<rr_f16> { static constexpr int v = RR_F16; };
 template <> struct code<rr_bf16> { static constexpr int v = RR_BF16; };
+
+// N weights from column c on, of the inputs' type or float32 (aligned like the rows where N > 1), ones without a weight
+template <typename T, int N>
+__device__ __forceinline__ void load_w(const void* w, int w32, int c, float (&x)[N]) {
+  if (w == nullptr) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = 1.f;
+  } else if (w32 || code<T>::v == RR_F32) {
+    if constexpr (N == 1) x[0] = ((const float*)w)[c];
+    else {
+#pragma unroll
+      for (int i = 0; i < N; i += 4) {
+        const float4 v = *reinterpret_cast<const float4*>((const float*)w + c + i);
+        x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
+      }
+    }
+  } else {
+    rr_load_n<T, N>((const T*)w + c, x);
+  }
+}
 
 // ------------------------------------------------------------------------------------------------ forward
 template <typename T, int VEC, int TPR, int NC, bool FP8>
@@ -89,7 +98,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_fwd(const T* __re
       const int col = (c * TPR + lane) * VEC;
       if (live && col < E) {
         float g[VEC];
-        load_w<VEC>(w, w32, code<T>::v, col, VEC > 1, g);
+        load_w<T, VEC>(w, w32, col, g);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) g[i] = v[c][i] * s * g[i];
         rr_store_n<T, VEC>(y + row * (long)E + col, g);
@@ -108,7 +117,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_fwd(const T* __re
       a[c] = 0.f;
       if (live && col < E) {
         float g[VEC];
-        load_w<VEC>(w, w32, code<T>::v, col, VEC > 1, g);
+        load_w<T, VEC>(w, w32, col, g);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) { v[c][i] = v[c][i] * s * g[i]; a[c] = fmaxf(a[c], fabsf(v[c][i])); }
         if constexpr (VEC == 1) atomicMax(&gmax[team * 128 + col / 128], __float_as_uint(a[c]));
@@ -127,10 +136,11 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_fwd(const T* __re
         const float am = VEC == 1 ? __uint_as_float(gmax[team * 128 + col / 128]) : a[c];
         const float sc = am == 0.f ? 1.f : am / 448.0f;
         if (col % 128 == 0) qs[row * G + col / 128] = sc;
+        const float inv = 1.0f / sc;                                       // one quotient a group; y * inv is off by a step of float32 at the most
         float z[VEC < 4 ? 4 : VEC];
 #pragma unroll
         for (int i = 0; i < (VEC < 4 ? 4 : VEC); ++i) {
-          const float e = i < VEC ? v[c][i < VEC ? i : 0] / sc : 0.f;
+          const float e = i < VEC ? v[c][i < VEC ? i : 0] * inv : 0.f;
           z[i] = e != e ? e : fminf(fmaxf(e, -448.f), 448.f);             // the quotient may pass 448 by a rounding
         }
         int p0 = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
@@ -164,7 +174,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_bwd(const T* __re
     const int col = (c * TPR + lane) * VEC;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) { gw[c][i] = 0.f; acc[c][i] = 0.f; }
-    if (col < E) load_w<VEC>(w, w32, code<T>::v, col, VEC > 1, gw[c]);
+    if (col < E) load_w<T, VEC>(w, w32, col, gw[c]);
   }
   for (long r0 = (long)blockIdx.x * TEAMS; r0 < rows; r0 += (long)gridDim.x * TEAMS) {     // (uniform in the workgroup: the barriers inside are met)
     const long row = r0 + team;
@@ -235,19 +245,23 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_bwd(const T* __re
   }
 }
 
-// dw[c] = sum of the P partial rows: 64 columns a workgroup, its 16 waves take every 16th row each, joined in order
+// dw[c] = sum of the P partial rows: 16 columns a workgroup, 64 lanes of rows each, joined in order through LDS
 __global__ __launch_bounds__(1024) void k_rms_dw(const float* __restrict__ dwp, int P, int E, void* __restrict__ dw, int dtype) {
-  __shared__ float part[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
+  __shared__ float part[64][17];
+  const int lane = threadIdx.x & 15, row = threadIdx.x >> 4, c = blockIdx.x * 16 + lane;
   float t = 0.f;
-  if (c < E)
-    for (int p = wave; p < P; p += 16) t += dwp[(long)p * E + c];
-  part[wave][lane] = t;
-  __syncthreads();
-  if (wave == 0 && c < E) {
-    t = 0.f;
+  if (c < E) {
+#pragma unroll 4
+    for (int p = row; p < P; p += 64) t += dwp[(long)p * E + c];
+  }
+  part[row][lane] = t;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) t += part[i][lane];
+  for (int h = 32; h > 0; h >>= 1) {
+    __syncthreads();
+    if (row < h) part[row][lane] += part[row + h][lane];
+  }
+  if (row == 0 && c < E) {
+    t = part[0][lane];
     if (dtype == RR_F32) ((float*)dw)[c] = t;
     else if (dtype == RR_F16) ((rr_f16*)dw)[c] = (rr_f16)t;
     else ((rr_bf16*)dw)[c] = (rr_bf16)t;
@@ -270,7 +284,7 @@ template <typename T>
 int norm_fwd(const void* x, long ldx, const void* res, long ldr, const void* w, int w32, void* y, void* h, float* rstd, uint8_t* q, float* qs, long rows, int E,
              float eps, hipStream_t st) {
   constexpr int N = rr_vec_of<T>::N;
-  const bool vec = E % N == 0 && ldx % N == 0 && ldr % N == 0 && rr_aligned16(x) && rr_aligned16(res) && rr_aligned16(y) && rr_aligned16(h) && rr_aligned16(q);
+  const bool vec = E % N == 0 && ldx % N == 0 && ldr % N == 0 && rr_aligned16(x) && rr_aligned16(res) && rr_aligned16(y) && rr_aligned16(h) && rr_aligned16(q) && rr_aligned16(w);
 #define RR_GO8(T_, V, TPR, NC) \
   hipLaunchKernelGGL((k_rms_fwd<T_, V, TPR, NC, true>), dim3((unsigned)((rows + (TPR > 256 ? 1 : 256 / TPR) - 1) / (TPR > 256 ? 1 : 256 / TPR))), \
                      dim3(TPR > 256 ? TPR : 256), 0, st, (const T*)x, ldx, (const T*)res, ldr, w, w32, (T*)y, (T*)h, rstd, q, qs, rows, E, eps)
@@ -290,12 +304,12 @@ int norm_bwd(const void* x, long ldx, const void* res, long ldr, const void* w, 
              void* dx, void* dw, float* dwp, int parts, long rows, int E, hipStream_t st) {
   constexpr int N = rr_vec_of<T>::N;
   const bool vec = E % N == 0 && ldx % N == 0 && ldr % N == 0 && lddy % N == 0 && lddh % N == 0 && rr_aligned16(x) && rr_aligned16(res) && rr_aligned16(dy) &&
-                   rr_aligned16(dh) && rr_aligned16(dx);
+                   rr_aligned16(dh) && rr_aligned16(dx) && rr_aligned16(w);
 #define RR_GOB(T_, V, TPR, NC) \
   hipLaunchKernelGGL((k_rms_bwd<T_, V, TPR, NC>), dim3((unsigned)parts), dim3(TPR > 256 ? TPR : 256), 0, st, (const T*)x, ldx, (const T*)res, ldr, w, w32, \
                      (const T*)dy, lddy, (const T*)dh, lddh, rstd, (T*)dx, dw != nullptr ? dwp : (float*)nullptr, rows, E)
   if (vec) RR_NORM_DISPATCH(T, N, RR_GOB); else RR_NORM_DISPATCH(T, 1, RR_GOB);
-  if (dw != nullptr) hipLaunchKernelGGL(k_rms_dw, dim3((E + 63) / 64), dim3(1024), 0, st, dwp, parts, E, dw, w32 ? RR_F32 : code<T>::v);
+  if (dw != nullptr) hipLaunchKernelGGL(k_rms_dw, dim3((E + 15) / 16), dim3(1024), 0, st, dwp, parts, E, dw, w32 ? RR_F32 : code<T>::v);
   return rms_launched(hipGetLastError());
 }
 
@@ -317,8 +331,8 @@ extern "C" int rr_add_rms_norm(int dtype, const void* x, long long ldx, const vo
 
 extern "C" int rr_add_rms_norm_parts(long long rows, int E) {      // workgroups of the backward = partial rows of dw (floats [parts][E])
   const long long per = E <= 4096 ? 4 : 1;                         // about four teams a workgroup and four rows a team at the least
-  const long long want = (rows + 4 * per - 1) / (4 * per);
-  return (int)(want < 1 ? 1 : want > 1024 ? 1024 : want);
+  const long long want = (rows + 4 * per - 1) / (4 * per), most = E <= 2048 ? 1024 : 512;      // (512 partial rows of 4 096: 8 MB)
+  return (int)(want < 1 ? 1 : want > most ? most : want);
 }
 
 extern "C" int rr_add_rms_norm_bwd(int dtype, const void* x, long long ldx, const void* res, long long ldr, const void* w, int w_is_f32, const void* dy, long long lddy,
