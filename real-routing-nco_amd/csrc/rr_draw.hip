@@ -294,7 +294,7 @@ __global__ __launch_bounds__(256) void k_draw_wave(Draw a) {
   __shared__ uint32_t skey[E > 1 ? 4 : 1][64];
   __shared__ int sidx[E > 1 ? 4 : 1][64];
   __shared__ double sw[E > 1 ? 4 : 1][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = blockIdx.x * 4 + wave;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = blockIdx.x * 4 + wave;      // (the row's addresses in scalar registers)
   if (r >= a.R) return;                                                  // (no workgroup barrier below)
   const T* row = (const T*)a.logits + (long long)r * a.ld;
   uint32_t key[E];
@@ -347,6 +347,84 @@ __global__ __launch_bounds__(256) void k_draw_wave(Draw a) {
     }
   }
   choose<E>(a, q, r, key, [&](int e) { return lane + 64 * e; }, top, -1.0, skey[E > 1 ? wave : 0], sw[E > 1 ? wave : 0], lane);
+}
+
+// ---- short rows without top-k and top-p: 16 lanes a row, E consecutive keys a lane; four rows share every exchange between lanes
+template <int CTRL>
+__device__ __forceinline__ uint32_t ror_max(uint32_t v) { const uint32_t x = (uint32_t)RR_DPP(v, 0, CTRL, 0xf); return v > x ? v : x; }
+
+template <typename T, int E, bool VECTOR>
+__global__ __launch_bounds__(256) void k_draw_group(Draw a) {
+  constexpr int VEC = VECTOR ? rr_vec_of<T>::N : 1;
+  static_assert(E % VEC == 0, "whole pieces");
+  const int lane = threadIdx.x & 15, r = blockIdx.x * 16 + (threadIdx.x >> 4);
+  const bool live = r < a.R;
+  const int rc = live ? r : a.R - 1;                                     // (a row behind the last one repeats it and writes nothing)
+  const T* row = (const T*)a.logits + (long long)rc * a.ld;
+  const uint8_t* mask = a.mask != nullptr ? a.mask + (long long)rc * a.ldm : nullptr;
+  const int i0 = lane * E;
+  uint32_t key[E], top = 0u;
+#pragma unroll
+  for (int p = 0; p < E; p += VEC) {
+    float x[VEC];
+    uint8_t m[VEC];
+    const bool in = i0 + p < a.V;                                        // (pieces are whole: V is a multiple of VEC)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) { x[i] = 0.f; m[i] = 1; }
+    if (in) {
+      rr_load_n<T, VEC>(row + i0 + p, x);
+      if (mask != nullptr) __builtin_memcpy(m, mask + i0 + p, VEC);
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) { key[p + i] = key_of(x[i], in && m[i] != 0); top = key[p + i] > top ? key[p + i] : top; }
+  }
+  top = ror_max<0x128>(top);                                             // row_ror 8, 4, 2, 1: every lane of a row gets its maximum
+  top = ror_max<0x124>(top);
+  top = ror_max<0x122>(top);
+  top = ror_max<0x121>(top);
+  const Par q = par_of(a, rc);
+  const double topd = (double)value_of(top);
+  double w[E], s = 0.0;
+  int first = 0x7fffffff;
+#pragma unroll
+  for (int e = E - 1; e >= 0; --e) first = key[e] == top && top ? i0 + e : first;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    w[e] = key[e] ? weight_of(key[e], top, topd, q.c2) : 0.0;
+    if (w[e] < q.mp) w[e] = 0.0;
+    if (q.greedy) w[e] = i0 + e == first ? 1.0 : 0.0;                    // (one a lane; the lowest lane's wins below)
+    s += w[e];
+  }
+  double inc = s;
+  inc += dpp_d<0x111, 0xf>(inc);
+  inc += dpp_d<0x112, 0xf>(inc);
+  inc += dpp_d<0x114, 0xf>(inc);
+  inc += dpp_d<0x118, 0xf>(inc);
+  const double total = __shfl(inc, (threadIdx.x & 48) | 15);
+  const double target = q.greedy ? 0.0 : q.u * total;
+  const int shift = threadIdx.x & 48;
+  const unsigned hits = (unsigned)(__ballot(s > 0.0 && inc > target) >> shift) & 0xffffu, any = (unsigned)(__ballot(s > 0.0) >> shift) & 0xffffu;
+  if (!live) return;
+  if (any == 0u) {                                                       // nothing may be drawn
+    if (lane == 0) { a.index[r] = 0; a.logp[r] = -INFINITY; }
+    return;
+  }
+  const int at = hits ? __ffs(hits) - 1 : 31 - __clz(any);               // (rounding may leave the target at the very end: the last key with a weight)
+  if (lane != at) return;
+  double c = inc - s;
+  uint32_t k = 0u;
+  int pick = 0;
+  bool done = false;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    c += w[e];
+    const bool take = w[e] > 0.0 && !done;
+    k = take ? key[e] : k;
+    pick = take ? i0 + e : pick;
+    done = done || (take && hits != 0u && c > target);
+  }
+  a.index[r] = pick;
+  a.logp[r] = q.greedy ? 0.f : (float)(z_of(k, top, q.c2) - log_of(total));
 }
 
 // ------------------------------------------------------------------------------------------------ long rows
@@ -1144,7 +1222,19 @@ int draw_rows(const Draw& a, hipStream_t st) {
 
 template <typename T>
 int draw_go(const Draw& a, void* ws, hipStream_t st) {
-  const dim3 wg((unsigned)((a.R + 3) / 4));
+  const dim3 wg((unsigned)((a.R + 3) / 4)), wg16((unsigned)((a.R + 15) / 16));
+  // without top-k and top-p rows of up to 128 keys take 16 lanes: the scans, the logarithm and the choice are paid once for four rows
+  // (51 200 x 100 float32: 27 us with a wave a row)
+  if (a.V <= 128 && a.pk == nullptr && a.pp == nullptr && (a.k <= 0 || a.k >= a.V) && !(a.p > 0.0 && a.p < 1.0)) {
+    constexpr int N = rr_vec_of<T>::N;
+    const bool vec = a.V % N == 0 && a.ld % N == 0 && rr_aligned16(a.logits);
+    if (vec && a.V <= 16 * N) hipLaunchKernelGGL((k_draw_group<T, N, true>), wg16, dim3(256), 0, st, a);
+    else if (vec) hipLaunchKernelGGL((k_draw_group<T, 8, true>), wg16, dim3(256), 0, st, a);
+    else if (a.V <= 32) hipLaunchKernelGGL((k_draw_group<T, 2, false>), wg16, dim3(256), 0, st, a);
+    else if (a.V <= 64) hipLaunchKernelGGL((k_draw_group<T, 4, false>), wg16, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_draw_group<T, 8, false>), wg16, dim3(256), 0, st, a);
+    return rr_check(hipGetLastError());
+  }
   // up to 1 024 keys a wave a row (16 registers of keys a lane)
   if (a.V <= 64) hipLaunchKernelGGL((k_draw_wave<T, 1>), wg, dim3(256), 0, st, a);
   else if (a.V <= 128) hipLaunchKernelGGL((k_draw_wave<T, 2>), wg, dim3(256), 0, st, a);
