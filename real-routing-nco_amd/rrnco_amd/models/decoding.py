@@ -6,6 +6,7 @@ import torch
 
 from .. import _lib as L
 from ..ops import batchify
+from ..sampling import sample
 
 
 def get_decoding_strategy(decoding_strategy, **config):
@@ -23,7 +24,7 @@ class DecodingStrategy:
 
     def __init__(self, temperature=1.0, top_p=0.0, top_k=0, mask_logits=True, tanh_clipping=0, num_samples=None,
                  multisample=False, num_starts=None, multistart=False, select_start_nodes_fn=None,
-                 improvement_method_mode=False, select_best=False, store_all_logp=False, seed=None, **kwargs):
+                 improvement_method_mode=False, select_best=False, store_all_logp=False, seed=None, min_p=0.0, uniforms=None, **kwargs):
         if improvement_method_mode:
             raise NotImplementedError("improvement_method_mode is outside the MI355X hot path")
         self.select_best = bool(select_best)
@@ -44,7 +45,37 @@ class DecodingStrategy:
         # the sampling noise is a pure function of (seed, rollout, step, key): without an explicit seed, draw a fresh one from
         # torch's generator, as the reference's torch.multinomial advances it (decoding.py:282-298)
         self.seed = int(torch.randint(0, 2 ** 62, (1,)).item()) if seed is None else int(seed)
+        # min_p and given random numbers (uniforms: [steps, rollouts], a row for each decode step in [0, 1)) are served by ops.sample in the step-wise
+        # loop, with its exact filters: equal logits stay or go together
+        if not 0.0 <= min_p <= 1.0:
+            raise ValueError(f"min_p in 0 .. 1, got {min_p}")
+        if (min_p > 0.0 or uniforms is not None) and (self.mode != "sampling" or store_all_logp):
+            raise ValueError("min_p and uniforms are for sampling without store_all_logp")
+        if uniforms is not None and (uniforms.dim() != 2 or uniforms.dtype != torch.float32):
+            raise ValueError("uniforms: a float32 tensor [steps, rollouts]")
+        self.min_p, self.uniforms, self._draws, self._numbers = float(min_p), uniforms, 0, None
         self.actions, self.logprobs = [], []
+
+    @property
+    def draws_given(self):
+        """The choice is made by ops.sample: never inside the fused rollout."""
+        return self.min_p > 0.0 or self.uniforms is not None
+
+    def _draw(self, logits, mask):
+        """One sampling step by ops.sample: tanh clipping as in process_logits (decoding.py:311-341), then temperature, top-k, top-p, min-p."""
+        R = logits.shape[0]
+        if self.uniforms is not None:
+            if self._draws >= self.uniforms.shape[0] or self.uniforms.shape[1] != R:
+                raise ValueError(f"uniforms {tuple(self.uniforms.shape)}: step {self._draws} of {R} rollouts needs a row of its own")
+            u = self.uniforms[self._draws].to(logits.device)
+        else:
+            if self._numbers is None:
+                self._numbers = torch.Generator(device=logits.device).manual_seed(self.seed % (2 ** 63))
+            u = torch.rand(R, device=logits.device, generator=self._numbers)
+        self._draws += 1
+        if self.tanh_clipping > 0:
+            logits = torch.tanh(logits) * self.tanh_clipping
+        return sample(logits, u, temperature=float(self.temperature), top_k=self.top_k, top_p=self.top_p, min_p=self.min_p, mask=mask)
 
     def pre_decoder_hook(self, td, env, action=None):
         """decoding.py:157-205."""
@@ -91,6 +122,14 @@ class DecodingStrategy:
         logits = logits.contiguous()
         R, N = logits.shape
         m = mask.contiguous() if (self.mask_logits and mask is not None) else None
+        if self.draws_given:
+            if getattr(self, "matnet_clamp", False):
+                raise NotImplementedError("min_p and uniforms with the MatNet baseline's own process_logits")
+            sel, lp = self._draw(logits, m)
+            td.set("action", sel)
+            self.actions.append(sel)
+            self.logprobs.append(lp)
+            return td
         sel = torch.empty(R, dtype=torch.int64, device=logits.device)
         lp = torch.empty(R, dtype=torch.float32, device=logits.device)
         lp_all = torch.empty(R, N, dtype=torch.float32, device=logits.device) if self.store_all_logp else None

@@ -364,6 +364,8 @@ class RRNetPolicy(nn.Module):
             mask_logits=decoding_kwargs.pop("mask_logits", self.mask_logits),
             store_all_logp=decoding_kwargs.pop("store_all_logp", return_entropy), **decoding_kwargs)
 
+        if capture is not None and strategy.min_p > 0.0:
+            raise NotImplementedError("min_p in a training step: the replayed log-likelihood has no filters")
         td, env, num_starts = strategy.pre_decoder_hook(td, env)
         td, env, cache = self.decoder.pre_decoder_hook(td, env, (row_emb, col_emb), num_starts, packed=packed,
                                                        status=getattr(self, "_range_status", None))
@@ -377,7 +379,7 @@ class RRNetPolicy(nn.Module):
         filters_fused = (not filters) or (fused_filters_ok(getattr(self, "precision", "32"), capture is not None)
                                           and strategy.mode in ("greedy", "sampling"))
         if (fused and not strategy.store_all_logp and self.env_name in PROB_ID and strategy.mask_logits and filters_fused
-                and not getattr(strategy, "is_beam_search", False)):
+                and not getattr(strategy, "is_beam_search", False) and not strategy.draws_given):
             dump = None
             if capture is not None:      # training: keep what the hand-written backward needs (models/dec_backward.py)
                 dump = capture.setdefault("dump", {})

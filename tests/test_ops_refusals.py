@@ -1,0 +1,143 @@
+"""What the decoder operators refuse, on the CPU: the Python side by shape, type and value, the C entry points by their own checks (they return before any launch)."""
+import ctypes as C
+
+import pytest
+import torch
+
+from rrnco_amd import _lib as L
+from rrnco_amd import ops
+from rrnco_amd.models import CrossAttention
+from rrnco_amd.models.decoding import get_decoding_strategy
+
+Q, K = torch.zeros(2, 3, 4, 16), torch.zeros(2, 5, 2, 16)
+
+
+def test_no_cpu_fallback():
+    for f in (lambda: ops.cross_attention(Q, K, K), lambda: ops.add_rms_norm(torch.zeros(2, 8)), lambda: ops.add_rms_norm_fp8(torch.zeros(2, 8)),
+              lambda: ops.sample(torch.zeros(2, 8), torch.zeros(2))):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            f()
+
+
+@pytest.mark.parametrize("q,k,v,kw,err", [
+    (Q.double(), K.double(), K.double(), {}, TypeError), (Q, K.half(), K.half(), {}, TypeError), (Q, K, K.bfloat16(), {}, TypeError),
+    (Q[0], K, K, {}, ValueError), (Q, K, K[:, :4], {}, ValueError), (Q, K[:1], K[:1], {}, ValueError), (Q, torch.zeros(2, 5, 2, 24), torch.zeros(2, 5, 2, 24), {}, ValueError),
+    (torch.zeros(2, 3, 4, 12), torch.zeros(2, 5, 2, 12), torch.zeros(2, 5, 2, 12), {}, ValueError),
+    (torch.zeros(2, 3, 4, 136), torch.zeros(2, 5, 2, 136), torch.zeros(2, 5, 2, 136), {}, ValueError),
+    (torch.zeros(2, 3, 3, 16), K, K, {}, ValueError), (Q, torch.zeros(2, 5, 0, 16), torch.zeros(2, 5, 0, 16), {}, ValueError),
+    (Q, K, K, dict(mask=torch.ones(2, 4, 3, 5)), ValueError), (Q, K, K, dict(mask=torch.ones(2, 3, 5, dtype=torch.bool)), ValueError),
+    (Q, K, K, dict(mask=torch.ones(2, 2, 3, 5, dtype=torch.bool)), ValueError), (Q, K, K, dict(kv_lens=torch.ones(3, dtype=torch.int32)), ValueError),
+    (Q, K, K, dict(kv_lens=torch.ones(2)), ValueError), (Q, K, K, dict(scale=0.0), ValueError), (Q, K, K, dict(scale=-1.0), ValueError),
+    (Q, K, K, dict(scale=float("nan")), ValueError), (Q, K, K, dict(scale=float("inf")), ValueError),
+])
+def test_cross_attention_refuses(q, k, v, kw, err):
+    with pytest.raises(err):
+        ops.cross_attention(q, k, v, **kw)
+
+
+@pytest.mark.parametrize("x,r,w,kw,err", [
+    (torch.zeros(2, 8).double(), None, None, {}, TypeError), (torch.zeros(2, 8, dtype=torch.int32), None, None, {}, TypeError), (torch.zeros(()), None, None, {}, ValueError),
+    (torch.zeros(2, 0), None, None, {}, ValueError), (torch.zeros(1, 16385), None, None, {}, ValueError), (torch.zeros(2, 8), torch.zeros(1, 8), None, {}, ValueError),
+    (torch.zeros(2, 8), torch.zeros(2, 8).half(), None, {}, ValueError), (torch.zeros(2, 8), None, torch.zeros(9), {}, ValueError),
+    (torch.zeros(2, 8), None, torch.zeros(8).half(), {}, ValueError), (torch.zeros(2, 8), None, None, dict(eps=-1.0), ValueError), (torch.zeros(2, 8), None, None, dict(eps=float("nan")), ValueError),
+])
+def test_norms_refuse(x, r, w, kw, err):
+    for f in (ops.add_rms_norm, ops.add_rms_norm_fp8):
+        with pytest.raises(err):
+            f(x, r, w, **kw)
+
+
+L8, U2 = torch.zeros(2, 8), torch.zeros(2)
+
+
+@pytest.mark.parametrize("x,u,kw,err", [
+    (L8.double(), U2, {}, TypeError), (torch.zeros(()), torch.zeros(()), {}, ValueError), (torch.zeros(2, 0), U2, {}, ValueError), (L8, torch.zeros(3), {}, ValueError),
+    (L8, U2.double(), {}, ValueError), (L8, torch.zeros(2, 1), {}, ValueError), (L8, U2, dict(mask=torch.ones(2, 8)), ValueError),
+    (L8, U2, dict(mask=torch.ones(3, 8, dtype=torch.bool)), ValueError), (L8, U2, dict(mask=torch.ones(1, 2, 8, dtype=torch.bool)), ValueError),
+    (L8, U2, dict(temperature=-0.5), ValueError), (L8, U2, dict(temperature=float("nan")), ValueError), (L8, U2, dict(temperature=float("inf")), ValueError),
+    (L8, U2, dict(top_k=-1), ValueError), (L8, U2, dict(top_k=2.5), ValueError), (L8, U2, dict(top_p=1.5), ValueError), (L8, U2, dict(top_p=-0.1), ValueError),
+    (L8, U2, dict(min_p=2.0), ValueError), (L8, U2, dict(temperature=torch.ones(3)), ValueError), (L8, U2, dict(top_k="5"), TypeError), (L8, U2, dict(top_p=None), TypeError),
+    (L8, U2, dict(top_k=torch.ones(2, dtype=torch.bool)), ValueError),
+])
+def test_sample_refuses(x, u, kw, err):
+    with pytest.raises(err):
+        ops.sample(x, u, **kw)
+
+
+def test_strategies_and_modules_refuse():
+    with pytest.raises(ValueError):
+        get_decoding_strategy("sampling", min_p=1.5)
+    for kw in (dict(min_p=0.1), dict(uniforms=torch.zeros(3, 4))):
+        for kind in ("greedy", "evaluate", "beam_search"):
+            with pytest.raises(ValueError):
+                get_decoding_strategy(kind, **kw)
+        with pytest.raises(ValueError):
+            get_decoding_strategy("sampling", store_all_logp=True, **kw)
+        assert get_decoding_strategy("multistart_sampling", num_starts=4, **kw).draws_given
+    with pytest.raises(ValueError):
+        get_decoding_strategy("sampling", uniforms=torch.zeros(4))
+    assert not get_decoding_strategy("sampling").draws_given
+    for bad in ((100, 8), (128, 3), (128, 8, 3), (1024, 4)):
+        with pytest.raises(ValueError):
+            CrossAttention(*bad)
+    m = CrossAttention(128, 8)
+    with pytest.raises(ValueError):
+        m(torch.zeros(1, 2, 128))
+
+
+class IO(C.Structure):                                       # include/rrnco_hip.h: XAttnIO
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "out", "lse", "mask", "kv_lens", "dout", "delta", "dq", "dk", "dv", "workspace")] + \
+        [(n, C.c_longlong * 3) for n in ("q_stride", "k_stride", "v_stride", "mask_stride", "dout_stride")] + [("workspace_bytes", C.c_longlong)] + \
+        [(n, C.c_int) for n in ("lens_int64", "dtype", "B", "Lq", "Lk", "Hk", "G", "D")] + [("scale", C.c_float)]
+
+
+def _io(**kw):
+    p = 4096                                                  # never followed: every call below is refused first
+    io = IO(q=p, k=p, v=p, out=p, lse=p, dout=p, delta=p, dq=p, dk=p, dv=p, B=2, Lq=3, Lk=5, Hk=2, G=2, D=16, scale=0.25)
+    io.q_stride, io.k_stride, io.v_stride, io.dout_stride = (192, 64, 16), (160, 32, 16), (160, 32, 16), (192, 64, 16)
+    for n, v in kw.items():
+        setattr(io, n, tuple(v) if isinstance(v, tuple) else v)
+    return io
+
+
+@pytest.mark.parametrize("kw", [dict(D=12), dict(D=0), dict(D=136), dict(B=0), dict(Lq=0), dict(Hk=0), dict(G=0), dict(dtype=3), dict(dtype=-1), dict(scale=0.0), dict(scale=float("nan")),
+                                dict(q=None), dict(k=None), dict(v=4100), dict(out=None), dict(q_stride=(192, 65, 16)), dict(k_stride=(160, 32, 2)), dict(Lk=-1),
+                                dict(Lk=100000, workspace=None), dict(B=2 ** 30, Hk=2 ** 30)], ids=str)
+def test_cross_attention_entry_refuses(kw):
+    lib = L.lib()
+    for fn in (lib.rr_cross_attn, lib.rr_cross_attn_bwd):
+        assert fn(C.addressof(_io(**kw)), None) == -1
+    assert lib.rr_cross_attn(None, None) == -1 and lib.rr_cross_attn_bwd(None, None) == -1
+
+
+@pytest.mark.parametrize("kw", [dict(lse=None), dict(delta=None), dict(dout=None), dict(dq=None), dict(dk=None), dict(dv=4104), dict(dout_stride=(192, 64, 3)), dict(Lk=0)], ids=str)
+def test_cross_attention_backward_entry_refuses(kw):
+    assert L.lib().rr_cross_attn_bwd(C.addressof(_io(**kw)), None) == -1
+
+
+def test_workspace_sizes():
+    lib = L.lib()
+    assert lib.rr_cross_attn_workspace(0, 2, 3, 5, 2, 2, 12, 0) == -1
+    assert lib.rr_cross_attn_workspace(2, 64, 1000, 100, 8, 1, 64, 0) == 0                          # enough workgroups: no splits
+    n = lib.rr_cross_attn_workspace(2, 1, 1, 100000, 1, 4, 128, 0)                                  # one token on long states: split
+    assert n > 0 and n % (4 * 4 * 132) == 0
+    assert lib.rr_draw_workspace(100, 1000) == 0 and lib.rr_draw_workspace(4, 100000) > 0 and lib.rr_draw_workspace(5000, 100000) == 0
+
+
+def test_norm_and_draw_entries_refuse():
+    lib, p = L.lib(), 4096
+    ok = [0, p, 8, p, 8, p, 0, p, p, None, None, None, 2, 8, 1e-5, None]
+    for i, v in ((0, 3), (1, None), (13, 0), (13, 16385), (12, -1), (7, None), (9 + 1, p), (2, -1)):
+        bad = list(ok)
+        bad[i] = v
+        assert lib.rr_add_rms_norm(*bad) == -1, (i, v)
+    ok = [0, p, 8, p, 8, p, 0, p, 8, p, 8, p, p, p, p, 4, 2, 8, None]
+    for i, v in ((0, 7), (1, None), (7, None), (11, None), (12, None), (14, None), (15, 0), (16, 0), (17, 0)):
+        bad = list(ok)
+        bad[i] = v
+        assert lib.rr_add_rms_norm_bwd(*bad) == -1, (i, v)
+    ok = [0, p, 8, None, 0, p, p, p, 2, 8, 1.0, 0, 0.0, 0.0, None, None, None, None, None, 0, None]
+    for i, v in ((0, 5), (1, None), (5, None), (6, None), (7, None), (8, -1), (9, 0), (9, (1 << 24) + 1), (10, -1.0), (10, float("nan")), (11, -1), (12, 1.5), (13, -0.5), (2, -8), (9, 100000)):
+        bad = list(ok)
+        bad[i] = v
+        assert lib.rr_draw(*bad) == -1, (i, v)
