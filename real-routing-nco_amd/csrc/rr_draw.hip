@@ -444,9 +444,9 @@ __device__ __forceinline__ unsigned long long steps_of(double w) {       // w <=
 }
 
 // E keys a thread of NT * E consecutive ones from `base` on: piece-major, then thread, VEC keys each (index order within each level)
-template <typename T, int NT, int E, bool VECTOR>
+template <typename T, int NT, int E>
 struct Keys {
-  static constexpr int VEC = VECTOR ? rr_vec_of<T>::N : 1, P = E / VEC, N = NT * E;
+  static constexpr int VEC = rr_vec_of<T>::N, P = E / VEC, N = NT * E;
   uint32_t key[E];
   int base;
   __device__ __forceinline__ int index(int e) const { return base + (e / VEC * NT + (int)threadIdx.x) * VEC + e % VEC; }
@@ -554,9 +554,9 @@ struct Kept {
 
 // the choice among the keys of one stretch: `base` is the mass before it, `total` the row's (below 0: this stretch is the row).  Each wave's mass of each
 // piece goes to LDS, every wave finds the (piece, wave) that the target falls in, that wave scans its lanes, the lane walks its VEC keys
-template <typename T, int NT, int E, bool VECTOR, typename S>
-__device__ __forceinline__ void locate(const Draw& a, const Par& q, int r, const Keys<T, NT, E, VECTOR>& ks, const Kept& kept, double base, double total, S& sh) {
-  using K = Keys<T, NT, E, VECTOR>;
+template <typename T, int NT, int E, typename S>
+__device__ __forceinline__ void locate(const Draw& a, const Par& q, int r, const Keys<T, NT, E>& ks, const Kept& kept, double base, double total, S& sh) {
+  using K = Keys<T, NT, E>;
   constexpr int NW = NT / 64, N = K::P * NW, PER = (N + 63) / 64;
   static_assert(N <= 512, "the table of parts");
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -735,9 +735,9 @@ __device__ __forceinline__ uint32_t thresholds(const Draw& a, const Par& q, uint
 }
 
 // A row of any length by one workgroup.  ONE: the row's keys fit its registers; else stretch after stretch is loaded again for every walk
-template <typename T, int NT, int E, bool VECTOR, bool ONE, typename S>
+template <typename T, int NT, int E, bool ONE, typename S>
 __device__ __forceinline__ void draw_row(const Draw& a, int r, S& sh) {
-  using K = Keys<T, NT, E, VECTOR>;
+  using K = Keys<T, NT, E>;
   const T* row = (const T*)a.logits + (long long)r * a.ld;
   const uint8_t* mask = a.mask ? a.mask + (long long)r * a.ldm : nullptr;
   const Par q = par_of(a, r);
@@ -789,10 +789,10 @@ __device__ __forceinline__ void draw_row(const Draw& a, int r, S& sh) {
     locate(a, q, r, ks, kept, before, total, sh);
   }
 }
-template <typename T, int NT, int E, bool VECTOR, bool ONE>
+template <typename T, int NT, int E, bool ONE>
 __global__ __launch_bounds__(NT) void k_draw_row(Draw a) {
   __shared__ Scratch<NT, 1024> sh;
-  draw_row<T, NT, E, VECTOR, ONE>(a, blockIdx.x, sh);
+  draw_row<T, NT, E, ONE>(a, blockIdx.x, sh);
 }
 
 // ---- few long rows: every stretch of a row has its own workgroup, five launches
@@ -823,18 +823,18 @@ struct LongScratch : Scratch<RR_DRAW_NT, RR_DRAW_LIST> {
 __device__ __forceinline__ bool by_count(const Par& q, uint32_t n) { return q.k > 0 && n > (uint32_t)q.k; }
 __device__ __forceinline__ bool by_mass(const Par& q) { return q.p > 0.0 && q.p < 1.0; }
 
-template <typename T, bool VECTOR>
-using LongKeys = Keys<T, RR_DRAW_NT, RR_DRAW_STRETCH / RR_DRAW_NT, VECTOR>;
-template <typename T, bool VECTOR>
-__device__ __forceinline__ void load_stretch(LongKeys<T, VECTOR>& ks, const Draw& a, int r, int c) {
+template <typename T>
+using LongKeys = Keys<T, RR_DRAW_NT, RR_DRAW_STRETCH / RR_DRAW_NT>;
+template <typename T>
+__device__ __forceinline__ void load_stretch(LongKeys<T>& ks, const Draw& a, int r, int c) {
   ks.load((const T*)a.logits + (long long)r * a.ld, a.mask ? a.mask + (long long)r * a.ldm : nullptr, c * RR_DRAW_STRETCH, a.V);
 }
-template <typename T, bool VECTOR>
+template <typename T>
 __global__ __launch_bounds__(RR_DRAW_NT) void k_draw_top(Draw a, Long l) {
   __shared__ uint32_t red[RR_DRAW_NT / 64];
   const int r = blockIdx.x / l.C, c = blockIdx.x % l.C;
-  LongKeys<T, VECTOR> ks;
-  load_stretch<T, VECTOR>(ks, a, r, c);
+  LongKeys<T> ks;
+  load_stretch<T>(ks, a, r, c);
   uint32_t top = 0u, n = 0u;
   ks.each([&](uint32_t k, int) { top = k > top ? k : top; n += k != 0u; });
   top = block_max<RR_DRAW_NT>(top, red);
@@ -847,13 +847,13 @@ __global__ __launch_bounds__(RR_DRAW_NT) void k_draw_top(Draw a, Long l) {
   }
 }
 
-template <typename T, bool VECTOR>
+template <typename T>
 __global__ __launch_bounds__(RR_DRAW_NT) void k_draw_measure(Draw a, Long l) {
   __shared__ LongScratch sh;
   constexpr int NT = RR_DRAW_NT;
   const int r = blockIdx.x / l.C, c = blockIdx.x % l.C, lane = threadIdx.x & 63;
-  LongKeys<T, VECTOR> ks;
-  load_stretch<T, VECTOR>(ks, a, r, c);
+  LongKeys<T> ks;
+  load_stretch<T>(ks, a, r, c);
   const Par q = par_of(a, r);
   uint32_t top = 0u, n = 0u;                                             // the row's maximum and its number of keys, by each wave itself
   for (int i = lane; i < l.C; i += 64) {
@@ -967,7 +967,7 @@ __device__ __forceinline__ void sort_list(LongScratch& sh, int size) {
 }
 
 // a workgroup a row: the thresholds among the list, the choice
-template <typename T, bool VECTOR>
+template <typename T>
 __global__ __launch_bounds__(RR_DRAW_NT) void k_draw_pick(Draw a, Long l) {
   __shared__ LongScratch sh;
   constexpr int NT = RR_DRAW_NT;
@@ -979,7 +979,7 @@ __global__ __launch_bounds__(RR_DRAW_NT) void k_draw_pick(Draw a, Long l) {
     return;
   }
   if (mode == RR_ALONE) {
-    draw_row<T, NT, RR_DRAW_STRETCH / NT, VECTOR, false>(a, r, sh);
+    draw_row<T, NT, RR_DRAW_STRETCH / NT, false>(a, r, sh);
     return;
   }
   const double topd = (double)value_of(top);
@@ -990,8 +990,8 @@ __global__ __launch_bounds__(RR_DRAW_NT) void k_draw_pick(Draw a, Long l) {
     int at;
     double before, total;
     pick_stretch(l.C, q.u, [&](int i) { return l.masses[(long long)r * l.C + i]; }, at, before, total);
-    LongKeys<T, VECTOR> ks;
-    load_stretch<T, VECTOR>(ks, a, r, at);
+    LongKeys<T> ks;
+    load_stretch<T>(ks, a, r, at);
     locate(a, q, r, ks, kept, before, total, sh);
     return;
   }
@@ -1089,8 +1089,8 @@ __global__ __launch_bounds__(RR_DRAW_NT) void k_draw_pick(Draw a, Long l) {
       if (key[e] >= cut && kept(key[e]) > 0.0) atomicAdd(&sh.mass[pos[e] / RR_DRAW_STRETCH], w[e]);
     __syncthreads();
     pick_stretch(C, q.u, [&](int c) { return l.masses[(long long)r * C + c] + (double)sh.mass[c] / RR_DRAW_STEP; }, at, before, total);
-    LongKeys<T, VECTOR> ks;
-    load_stretch<T, VECTOR>(ks, a, r, at);
+    LongKeys<T> ks;
+    load_stretch<T>(ks, a, r, at);
     locate(a, q, r, ks, kept, before, total, sh);
     return;
   }
@@ -1126,7 +1126,7 @@ __global__ __launch_bounds__(RR_DRAW_NT) void k_draw_pick(Draw a, Long l) {
   }
 }
 
-template <typename T, bool VECTOR>
+template <typename T>
 __global__ __launch_bounds__(RR_DRAW_NT) void k_draw_gather(Draw a, Long l) {
   __shared__ uint32_t list[RR_DRAW_LIST], where[RR_DRAW_LIST];
   __shared__ double red[RR_DRAW_NT / 64];
@@ -1134,8 +1134,8 @@ __global__ __launch_bounds__(RR_DRAW_NT) void k_draw_gather(Draw a, Long l) {
   constexpr int NT = RR_DRAW_NT;
   const int r = blockIdx.x / l.C, c = blockIdx.x % l.C, mode = l.mode[r];
   if (mode != RR_LIST_ALL && mode != RR_LIST_BORDER) return;
-  LongKeys<T, VECTOR> ks;
-  load_stretch<T, VECTOR>(ks, a, r, c);
+  LongKeys<T> ks;
+  load_stretch<T>(ks, a, r, c);
   const uint32_t top = l.top[r];
   const int bin = l.bin[r];
   const Par q = par_of(a, r);
@@ -1177,7 +1177,7 @@ size_t long_bytes(long long R, int V) {
   return (size_t)R * (C * 8 + RR_DRAW_BINS * 8 + 16 + C * 8 + RR_DRAW_BINS * 4 + RR_DRAW_LIST * 8 + 24);
 }
 
-template <typename T, bool VECTOR>
+template <typename T>
 int draw_long(const Draw& a, void* ws, hipStream_t st) {
   Long l;
   const size_t R = (size_t)a.R, C = (size_t)stretches(a.V);
@@ -1200,23 +1200,23 @@ int draw_long(const Draw& a, void* ws, hipStream_t st) {
   l.n = (uint32_t*)take(R * 4);
   l.C = (int)C;
   const dim3 grid((unsigned)(R * C)), one((unsigned)R), nt(RR_DRAW_NT);
-  hipLaunchKernelGGL((k_draw_top<T, VECTOR>), grid, nt, 0, st, a, l);
-  hipLaunchKernelGGL((k_draw_measure<T, VECTOR>), grid, nt, 0, st, a, l);
+  hipLaunchKernelGGL((k_draw_top<T>), grid, nt, 0, st, a, l);
+  hipLaunchKernelGGL((k_draw_measure<T>), grid, nt, 0, st, a, l);
   hipLaunchKernelGGL(k_draw_border, one, nt, 0, st, a, l);
-  hipLaunchKernelGGL((k_draw_gather<T, VECTOR>), grid, nt, 0, st, a, l);
-  hipLaunchKernelGGL((k_draw_pick<T, VECTOR>), one, nt, 0, st, a, l);
+  hipLaunchKernelGGL((k_draw_gather<T>), grid, nt, 0, st, a, l);
+  hipLaunchKernelGGL((k_draw_pick<T>), one, nt, 0, st, a, l);
   return rr_check(hipGetLastError());
 }
 
-template <typename T, bool VECTOR>
+template <typename T>
 int draw_rows(const Draw& a, hipStream_t st) {
   const dim3 grid((unsigned)a.R);
   // the fewest threads whose registers hold the row (8 .. 32 keys each; 1 024 threads of 32 spill); what fits none is walked in stretches
-  if (a.V <= 2048) hipLaunchKernelGGL((k_draw_row<T, 256, 8, VECTOR, true>), grid, dim3(256), 0, st, a);
-  else if (a.V <= 4096) hipLaunchKernelGGL((k_draw_row<T, 256, 16, VECTOR, true>), grid, dim3(256), 0, st, a);
-  else if (a.V <= 8192) hipLaunchKernelGGL((k_draw_row<T, 256, 32, VECTOR, true>), grid, dim3(256), 0, st, a);
-  else if (a.V <= 16384) hipLaunchKernelGGL((k_draw_row<T, 512, 32, VECTOR, true>), grid, dim3(512), 0, st, a);
-  else hipLaunchKernelGGL((k_draw_row<T, 1024, 16, VECTOR, false>), grid, dim3(1024), 0, st, a);
+  if (a.V <= 2048) hipLaunchKernelGGL((k_draw_row<T, 256, 8, true>), grid, dim3(256), 0, st, a);
+  else if (a.V <= 4096) hipLaunchKernelGGL((k_draw_row<T, 256, 16, true>), grid, dim3(256), 0, st, a);
+  else if (a.V <= 8192) hipLaunchKernelGGL((k_draw_row<T, 256, 32, true>), grid, dim3(256), 0, st, a);
+  else if (a.V <= 16384) hipLaunchKernelGGL((k_draw_row<T, 512, 32, true>), grid, dim3(512), 0, st, a);
+  else hipLaunchKernelGGL((k_draw_row<T, 1024, 16, false>), grid, dim3(1024), 0, st, a);
   return rr_check(hipGetLastError());
 }
 
@@ -1227,7 +1227,7 @@ int draw_go(const Draw& a, void* ws, hipStream_t st) {
   // (51 200 x 100 float32: 27 us with a wave a row)
   if (a.V <= 128 && a.pk == nullptr && a.pp == nullptr && (a.k <= 0 || a.k >= a.V) && !(a.p > 0.0 && a.p < 1.0)) {
     constexpr int N = rr_vec_of<T>::N;
-    const bool vec = a.V % N == 0 && a.ld % N == 0 && rr_aligned16(a.logits);
+    const bool vec = a.V % N == 0;
     if (vec && a.V <= 16 * N) hipLaunchKernelGGL((k_draw_group<T, N, true>), wg16, dim3(256), 0, st, a);
     else if (vec) hipLaunchKernelGGL((k_draw_group<T, 8, true>), wg16, dim3(256), 0, st, a);
     else if (a.V <= 32) hipLaunchKernelGGL((k_draw_group<T, 2, false>), wg16, dim3(256), 0, st, a);
@@ -1242,10 +1242,7 @@ int draw_go(const Draw& a, void* ws, hipStream_t st) {
   else if (a.V <= 512) hipLaunchKernelGGL((k_draw_wave<T, 8>), wg, dim3(256), 0, st, a);
   else if (a.V <= 1024) hipLaunchKernelGGL((k_draw_wave<T, 16>), wg, dim3(256), 0, st, a);
   else {
-    const int e = 16 / (int)sizeof(T);
-    const bool vec = a.ld % e == 0 && rr_aligned16(a.logits);
-    if (by_stretches(a.R, a.V)) return vec ? draw_long<T, true>(a, ws, st) : draw_long<T, false>(a, ws, st);
-    return vec ? draw_rows<T, true>(a, st) : draw_rows<T, false>(a, st);
+    return by_stretches(a.R, a.V) ? draw_long<T>(a, ws, st) : draw_rows<T>(a, st);
   }
   return rr_check(hipGetLastError());
 }

@@ -37,35 +37,33 @@ template <> struct code<float> { static constexpr int v = RR_F32; };
 template <> struct code<rr_f16> { static constexpr int v = RR_F16; };
 template <> struct code<rr_bf16> { static constexpr int v = RR_BF16; };
 
-// N weights from column c on, of the inputs' type or float32 (aligned like the rows where N > 1), ones without a weight
+// N weights from column c on, n of them in the row, of the inputs' type or float32; ones without a weight
 template <typename T, int N>
-__device__ __forceinline__ void load_w(const void* w, int w32, int c, float (&x)[N]) {
+__device__ __forceinline__ void load_w(const void* w, int w32, int c, int n, float (&x)[N]) {
   if (w == nullptr) {
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = 1.f;
   } else if (w32 || code<T>::v == RR_F32) {
-    if constexpr (N == 1) x[0] = ((const float*)w)[c];
-    else {
 #pragma unroll
-      for (int i = 0; i < N; i += 4) {
-        const float4 v = *reinterpret_cast<const float4*>((const float*)w + c + i);
-        x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
-      }
+    for (int i = 0; i < N; i += 4) {
+      float v[4];
+      rr_load_first<float, 4>((const float*)w + c + i, n - i, v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[i + e] = v[e];
     }
   } else {
-    rr_load_n<T, N>((const T*)w + c, x);
+    rr_load_first<T, N>((const T*)w + c, n, x);
   }
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-template <typename T, int VEC, int TPR, int NC, bool FP8>
+template <typename T, int TPR, int NC, bool FP8>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_fwd(const T* __restrict__ x, long ldx, const T* __restrict__ res, long ldr,
                                                                   const void* __restrict__ w, int w32, T* __restrict__ y, T* __restrict__ h,
                                                                   float* __restrict__ rstd, uint8_t* __restrict__ q, float* __restrict__ qs,
                                                                   long rows, int E, float eps) {
-  constexpr int BLK = TPR > 256 ? TPR : 256, TEAMS = BLK / TPR;
+  constexpr int VEC = rr_vec_of<T>::N, BLK = TPR > 256 ? TPR : 256, TEAMS = BLK / TPR;
   __shared__ float red[BLK / 64];
-  __shared__ uint32_t gmax[FP8 && VEC == 1 ? TEAMS * 128 : 1];
   const int team = threadIdx.x / TPR, lane = threadIdx.x % TPR;
   const long row = (long)blockIdx.x * TEAMS + team;
   const bool live = row < rows;                                            // (a dead team still takes part in the barriers)
@@ -77,14 +75,14 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_fwd(const T* __re
 #pragma unroll
     for (int i = 0; i < VEC; ++i) v[c][i] = 0.f;
     if (live && col < E) {
-      rr_load_n<T, VEC>(x + row * ldx + col, v[c]);
+      rr_load_first<T, VEC>(x + row * ldx + col, E - col, v[c]);
       if (res != nullptr) {
         float r[VEC];
-        rr_load_n<T, VEC>(res + row * ldr + col, r);
+        rr_load_first<T, VEC>(res + row * ldr + col, E - col, r);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) v[c][i] += r[i];
       }
-      if (h != nullptr) rr_store_n<T, VEC>(h + row * (long)E + col, v[c]);
+      if (h != nullptr) rr_store_first<T, VEC>(h + row * (long)E + col, E - col, v[c]);
     }
 #pragma unroll
     for (int i = 0; i < VEC; ++i) ss = fmaf(v[c][i], v[c][i], ss);
@@ -98,18 +96,14 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_fwd(const T* __re
       const int col = (c * TPR + lane) * VEC;
       if (live && col < E) {
         float g[VEC];
-        load_w<T, VEC>(w, w32, col, g);
+        load_w<T, VEC>(w, w32, col, E - col, g);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) g[i] = v[c][i] * s * g[i];
-        rr_store_n<T, VEC>(y + row * (long)E + col, g);
+        rr_store_first<T, VEC>(y + row * (long)E + col, E - col, g);
       }
     }
   } else {
     const int G = (E + 127) / 128;
-    if constexpr (VEC == 1) {                     // 128 columns are two waves: a group's maximum over LDS (a maximum has no order)
-      for (int i = threadIdx.x; i < TEAMS * 128; i += BLK) gmax[i] = 0u;
-      __syncthreads();
-    }
     float a[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -117,41 +111,39 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_fwd(const T* __re
       a[c] = 0.f;
       if (live && col < E) {
         float g[VEC];
-        load_w<T, VEC>(w, w32, col, g);
+        load_w<T, VEC>(w, w32, col, E - col, g);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) { v[c][i] = v[c][i] * s * g[i]; a[c] = fmaxf(a[c], fabsf(v[c][i])); }
-        if constexpr (VEC == 1) atomicMax(&gmax[team * 128 + col / 128], __float_as_uint(a[c]));
+        for (int i = 0; i < VEC; ++i) { v[c][i] = v[c][i] * s * g[i]; a[c] = fmaxf(a[c], fabsf(v[c][i])); }      // (zeros behind the row's end)
       }
-      if constexpr (VEC > 1) {
-        constexpr int GL = 128 / VEC;             // lanes of a group
+      constexpr int GL = 128 / VEC;               // lanes of a group
 #pragma unroll
-        for (int o = 1; o < (TPR < GL ? TPR : GL); o <<= 1) a[c] = fmaxf(a[c], __shfl_xor(a[c], o));
-      }
+      for (int o = 1; o < (TPR < GL ? TPR : GL); o <<= 1) a[c] = fmaxf(a[c], __shfl_xor(a[c], o));
     }
-    if constexpr (VEC == 1) __syncthreads();
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int col = (c * TPR + lane) * VEC;
       if (live && col < E) {
-        const float am = VEC == 1 ? __uint_as_float(gmax[team * 128 + col / 128]) : a[c];
-        const float sc = am == 0.f ? 1.f : am / 448.0f;
+        const float sc = a[c] == 0.f ? 1.f : a[c] / 448.0f;
         if (col % 128 == 0) qs[row * G + col / 128] = sc;
         const float inv = 1.0f / sc;                                       // one quotient a group; y * inv is off by a step of float32 at the most
-        float z[VEC < 4 ? 4 : VEC];
+        uint32_t p[VEC / 4];
 #pragma unroll
-        for (int i = 0; i < (VEC < 4 ? 4 : VEC); ++i) {
-          const float e = i < VEC ? v[c][i < VEC ? i : 0] * inv : 0.f;
-          z[i] = e != e ? e : fminf(fmaxf(e, -448.f), 448.f);             // the quotient may pass 448 by a rounding
+        for (int i = 0; i < VEC; i += 4) {
+          float z[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            z[e] = v[c][i + e] * inv;
+            z[e] = z[e] != z[e] ? z[e] : fminf(fmaxf(z[e], -448.f), 448.f);      // the product may pass 448 by a rounding
+          }
+          int b = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
+          p[i / 4] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], b, true);
         }
-        int p0 = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
-        p0 = __builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], p0, true);
         uint8_t* dst = q + row * (long)E + col;
-        if constexpr (VEC == 1) dst[0] = (uint8_t)(p0 & 0xff);
-        if constexpr (VEC == 4) *reinterpret_cast<int*>(dst) = p0;
-        if constexpr (VEC == 8) {
-          int p1 = __builtin_amdgcn_cvt_pk_fp8_f32(z[4], z[5], 0, false);
-          p1 = __builtin_amdgcn_cvt_pk_fp8_f32(z[6], z[7], p1, true);
-          *reinterpret_cast<int2*>(dst) = make_int2(p0, p1);
+        if (col + VEC <= E) __builtin_memcpy(dst, p, VEC);
+        else {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i)
+            if (col + i < E) dst[i] = (uint8_t)(p[i / 4] >> (8 * (i % 4)));
         }
       }
     }
@@ -159,12 +151,12 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_fwd(const T* __re
 }
 
 // ------------------------------------------------------------------------------------------------ backward
-template <typename T, int VEC, int TPR, int NC>
+template <typename T, int TPR, int NC>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_bwd(const T* __restrict__ x, long ldx, const T* __restrict__ res, long ldr,
                                                                   const void* __restrict__ w, int w32, const T* __restrict__ dy, long lddy,
                                                                   const T* __restrict__ dh, long lddh, const float* __restrict__ rstd,
                                                                   T* __restrict__ dx, float* __restrict__ dwp, long rows, int E) {
-  constexpr int BLK = TPR > 256 ? TPR : 256, TEAMS = BLK / TPR;
+  constexpr int VEC = rr_vec_of<T>::N, BLK = TPR > 256 ? TPR : 256, TEAMS = BLK / TPR;
   __shared__ float red[BLK / 64];
   __shared__ float join[TEAMS > 1 ? TEAMS * TPR * VEC : 1];
   const int team = threadIdx.x / TPR, lane = threadIdx.x % TPR;
@@ -174,7 +166,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_bwd(const T* __re
     const int col = (c * TPR + lane) * VEC;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) { gw[c][i] = 0.f; acc[c][i] = 0.f; }
-    if (col < E) load_w<T, VEC>(w, w32, col, gw[c]);
+    if (col < E) load_w<T, VEC>(w, w32, col, E - col, gw[c]);
   }
   for (long r0 = (long)blockIdx.x * TEAMS; r0 < rows; r0 += (long)gridDim.x * TEAMS) {     // (uniform in the workgroup: the barriers inside are met)
     const long row = r0 + team;
@@ -188,14 +180,14 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_bwd(const T* __re
 #pragma unroll
       for (int i = 0; i < VEC; ++i) { n[c][i] = 0.f; g[c][i] = 0.f; }
       if (live && col < E) {
-        rr_load_n<T, VEC>(x + row * ldx + col, n[c]);
+        rr_load_first<T, VEC>(x + row * ldx + col, E - col, n[c]);
         if (res != nullptr) {
           float r[VEC];
-          rr_load_n<T, VEC>(res + row * ldr + col, r);
+          rr_load_first<T, VEC>(res + row * ldr + col, E - col, r);
 #pragma unroll
           for (int i = 0; i < VEC; ++i) n[c][i] += r[i];
         }
-        rr_load_n<T, VEC>(dy + row * lddy + col, g[c]);
+        rr_load_first<T, VEC>(dy + row * lddy + col, E - col, g[c]);
       }
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
@@ -213,10 +205,10 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_bwd(const T* __re
         float o[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) o[i] = 0.f;
-        if (dh != nullptr) rr_load_n<T, VEC>(dh + row * lddh + col, o);
+        if (dh != nullptr) rr_load_first<T, VEC>(dh + row * lddh + col, E - col, o);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) o[i] = fmaf(s, g[c][i] - n[c][i] * dot, o[i]);
-        rr_store_n<T, VEC>(dx + row * (long)E + col, o);
+        rr_store_first<T, VEC>(dx + row * (long)E + col, E - col, o);
       }
     }
   }
@@ -240,7 +232,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_bwd(const T* __re
     }
     if (team == 0 && col < E) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) dwp[(long)blockIdx.x * E + col + i] = acc[c][i];
+      for (int i = 0; i < VEC; ++i)
+        if (col + i < E) dwp[(long)blockIdx.x * E + col + i] = acc[c][i];
     }
   }
 }
@@ -268,49 +261,37 @@ __global__ __launch_bounds__(1024) void k_rms_dw(const float* __restrict__ dwp, 
   }
 }
 
-int rms_launched(hipError_t e) { return e == hipSuccess ? RR_OK : RR_ELAUNCH; }
-
-// team size and pieces a lane by the number of pieces (VEC elements each) of a row
-#define RR_NORM_DISPATCH(T, V, RUN)                                                                                                       \
+// team size and pieces a lane by the number of 16-byte pieces of a row
+#define RR_NORM_DISPATCH(RUN)                                                                                                              \
   do {                                                                                                                                    \
-    const int pieces = (E + V - 1) / V;                                                                                                   \
-    if (pieces <= 16) { RUN(T, V, 16, 1); } else if (pieces <= 32) { RUN(T, V, 32, 1); } else if (pieces <= 64) { RUN(T, V, 64, 1); }      \
-    else if (pieces <= 128) { RUN(T, V, 64, 2); } else if (pieces <= 256) { RUN(T, V, 64, 4); } else if (pieces <= 512) { RUN(T, V, 256, 2); } \
-    else if (pieces <= 1024) { RUN(T, V, 256, 4); } else if (pieces <= 4096) { RUN(T, V, 1024, 4); }                                      \
-    else { if constexpr (V == 1) { RUN(T, V, 1024, 16); } else return RR_EINVAL; }                                                        \
+    const int pieces = (E + rr_vec_of<T>::N - 1) / rr_vec_of<T>::N;                                                                       \
+    if (pieces <= 16) { RUN(16, 1); } else if (pieces <= 32) { RUN(32, 1); } else if (pieces <= 64) { RUN(64, 1); }                        \
+    else if (pieces <= 128) { RUN(64, 2); } else if (pieces <= 256) { RUN(64, 4); } else if (pieces <= 512) { RUN(256, 2); }               \
+    else if (pieces <= 1024) { RUN(256, 4); } else { RUN(1024, 4); }      /* up to 16 384 float32 */                                       \
   } while (0)
 
 template <typename T>
 int norm_fwd(const void* x, long ldx, const void* res, long ldr, const void* w, int w32, void* y, void* h, float* rstd, uint8_t* q, float* qs, long rows, int E,
              float eps, hipStream_t st) {
-  constexpr int N = rr_vec_of<T>::N;
-  const bool vec = E % N == 0 && ldx % N == 0 && ldr % N == 0 && rr_aligned16(x) && rr_aligned16(res) && rr_aligned16(y) && rr_aligned16(h) && rr_aligned16(q) && rr_aligned16(w);
-#define RR_GO8(T_, V, TPR, NC) \
-  hipLaunchKernelGGL((k_rms_fwd<T_, V, TPR, NC, true>), dim3((unsigned)((rows + (TPR > 256 ? 1 : 256 / TPR) - 1) / (TPR > 256 ? 1 : 256 / TPR))), \
-                     dim3(TPR > 256 ? TPR : 256), 0, st, (const T*)x, ldx, (const T*)res, ldr, w, w32, (T*)y, (T*)h, rstd, q, qs, rows, E, eps)
-#define RR_GOT(T_, V, TPR, NC) \
-  hipLaunchKernelGGL((k_rms_fwd<T_, V, TPR, NC, false>), dim3((unsigned)((rows + (TPR > 256 ? 1 : 256 / TPR) - 1) / (TPR > 256 ? 1 : 256 / TPR))), \
-                     dim3(TPR > 256 ? TPR : 256), 0, st, (const T*)x, ldx, (const T*)res, ldr, w, w32, (T*)y, (T*)h, rstd, q, qs, rows, E, eps)
-  if (q != nullptr) {
-    if (vec) RR_NORM_DISPATCH(T, N, RR_GO8); else RR_NORM_DISPATCH(T, 1, RR_GO8);
-  } else {
-    if (vec) RR_NORM_DISPATCH(T, N, RR_GOT); else RR_NORM_DISPATCH(T, 1, RR_GOT);
-  }
-  return rms_launched(hipGetLastError());
+#define RR_GRID(TPR) dim3((unsigned)((rows + (TPR > 256 ? 1 : 256 / TPR) - 1) / (TPR > 256 ? 1 : 256 / TPR))), dim3(TPR > 256 ? TPR : 256)
+#define RR_GO8(TPR, NC) \
+  hipLaunchKernelGGL((k_rms_fwd<T, TPR, NC, true>), RR_GRID(TPR), 0, st, (const T*)x, ldx, (const T*)res, ldr, w, w32, (T*)y, (T*)h, rstd, q, qs, rows, E, eps)
+#define RR_GOT(TPR, NC) \
+  hipLaunchKernelGGL((k_rms_fwd<T, TPR, NC, false>), RR_GRID(TPR), 0, st, (const T*)x, ldx, (const T*)res, ldr, w, w32, (T*)y, (T*)h, rstd, q, qs, rows, E, eps)
+  if (q != nullptr) RR_NORM_DISPATCH(RR_GO8);
+  else RR_NORM_DISPATCH(RR_GOT);
+  return rr_check(hipGetLastError());
 }
 
 template <typename T>
 int norm_bwd(const void* x, long ldx, const void* res, long ldr, const void* w, int w32, const void* dy, long lddy, const void* dh, long lddh, const float* rstd,
              void* dx, void* dw, float* dwp, int parts, long rows, int E, hipStream_t st) {
-  constexpr int N = rr_vec_of<T>::N;
-  const bool vec = E % N == 0 && ldx % N == 0 && ldr % N == 0 && lddy % N == 0 && lddh % N == 0 && rr_aligned16(x) && rr_aligned16(res) && rr_aligned16(dy) &&
-                   rr_aligned16(dh) && rr_aligned16(dx) && rr_aligned16(w);
-#define RR_GOB(T_, V, TPR, NC) \
-  hipLaunchKernelGGL((k_rms_bwd<T_, V, TPR, NC>), dim3((unsigned)parts), dim3(TPR > 256 ? TPR : 256), 0, st, (const T*)x, ldx, (const T*)res, ldr, w, w32, \
+#define RR_GOB(TPR, NC) \
+  hipLaunchKernelGGL((k_rms_bwd<T, TPR, NC>), dim3((unsigned)parts), dim3(TPR > 256 ? TPR : 256), 0, st, (const T*)x, ldx, (const T*)res, ldr, w, w32, \
                      (const T*)dy, lddy, (const T*)dh, lddh, rstd, (T*)dx, dw != nullptr ? dwp : (float*)nullptr, rows, E)
-  if (vec) RR_NORM_DISPATCH(T, N, RR_GOB); else RR_NORM_DISPATCH(T, 1, RR_GOB);
+  RR_NORM_DISPATCH(RR_GOB);
   if (dw != nullptr) hipLaunchKernelGGL(k_rms_dw, dim3((E + 15) / 16), dim3(1024), 0, st, dwp, parts, E, dw, w32 ? RR_F32 : code<T>::v);
-  return rms_launched(hipGetLastError());
+  return rr_check(hipGetLastError());
 }
 
 }  // namespace

@@ -15,7 +15,8 @@ template <> struct rr_vec_of<float> { static constexpr int N = 4; };
 template <> struct rr_vec_of<rr_f16> { static constexpr int N = 8; };
 template <> struct rr_vec_of<rr_bf16> { static constexpr int N = 8; };
 
-// N consecutive elements as floats: one 16-byte (N elements of T are 16 bytes) or one element-wide access
+// N consecutive elements as floats by one access of N elements; the address needs the element's alignment only (global memory takes 16 bytes at any place:
+// rows of odd widths and odd strides go the same way as others)
 template <typename T, int N>
 __device__ __forceinline__ void rr_load_n(const T* __restrict__ p, float (&x)[N]) {
   if constexpr (N == 1) {
@@ -23,7 +24,8 @@ __device__ __forceinline__ void rr_load_n(const T* __restrict__ p, float (&x)[N]
   } else {
     static_assert(N * sizeof(T) == 16, "one 16-byte access");
     typedef T V __attribute__((ext_vector_type(N)));
-    const V v = *reinterpret_cast<const V*>(p);
+    typedef V U __attribute__((aligned(sizeof(T))));
+    const V v = *reinterpret_cast<const U*>(p);
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = (float)v[i];
   }
@@ -35,10 +37,29 @@ __device__ __forceinline__ void rr_store_n(T* __restrict__ p, const float (&x)[N
   } else {
     static_assert(N * sizeof(T) == 16, "one 16-byte access");
     typedef T V __attribute__((ext_vector_type(N)));
+    typedef V U __attribute__((aligned(sizeof(T))));
     V v;
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = (T)x[i];
-    *reinterpret_cast<V*>(p) = v;
+    *reinterpret_cast<U*>(p) = v;
+  }
+}
+// the first n of them (the others as zeros, unwritten)
+template <typename T, int N>
+__device__ __forceinline__ void rr_load_first(const T* __restrict__ p, int n, float (&x)[N]) {
+  if (n >= N) rr_load_n<T, N>(p, x);
+  else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = i < n ? (float)p[i] : 0.f;
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void rr_store_first(T* __restrict__ p, int n, const float (&x)[N]) {
+  if (n >= N) rr_store_n<T, N>(p, x);
+  else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < n) p[i] = (T)x[i];
   }
 }
 __host__ __forceinline__ bool rr_aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
