@@ -539,6 +539,7 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_dq(XAttn a) {
   using M = Mx<T>;
   using Dm = Dims<T, DP>;
   constexpr bool TIGHT = DP == 128 && QT == 2, SKIP = sizeof(T) == 4;
+  constexpr int STEPS = sizeof(T) == 2 && (ONE || DP == 128) ? 1 : 4;      // of a tile, unrolled (those spill if they are; the others gain 4%)
   __shared__ __attribute__((aligned(16))) T sk[2][RR_XA_KT * Dm::PX];
   __shared__ __attribute__((aligned(16))) T sv[2][RR_XA_KT * Dm::PR];
   __shared__ uint32_t flag[2][2];
@@ -605,7 +606,8 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_dq(XAttn a) {
     for (int t = 0; t < QT; ++t) dsum[t] = 0.f;
 #pragma unroll 1
     for (int phase = ONE ? 0 : 1; phase < 2; ++phase) {
-#pragma unroll
+    if (ONE) asm volatile("" ::: "memory");       // or the compiler lifts the tile's reads out of the loop over the phases, and keeps them in scratch memory
+#pragma unroll STEPS
     for (int n = 0; n < 4; n += M::PT) {
       if (SKIP && k0 + 16 * n >= seen) break;
       f32x4 s[QT][M::PT], dp[QT][M::PT];
@@ -693,7 +695,7 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_dq(XAttn a) {
     __syncthreads();
     int at = 0;
     for (int k0 = first; k0 < last; k0 += RR_XA_KT, at ^= 1) {
-      const bool more = k0 + RR_XA_KT < last;
+      const bool more = !ONE && k0 + RR_XA_KT < last;
       if (more) {
         pk.load(krow(k0 + RR_XA_KT), a.kl, seen - k0 - RR_XA_KT, a.D);
         pv.load(vrow(k0 + RR_XA_KT), a.vl, seen - k0 - RR_XA_KT, a.D);
@@ -756,6 +758,8 @@ __global__ __launch_bounds__(256, (DP == 128 && (sizeof(T) == 4 || KW == 2) ? 1 
   using M = Mx<T>;
   using Dm = Dims<T, DP>;
   constexpr bool TIGHT = DP >= 64 && KW == 2, SKIP = sizeof(T) == 4;
+  // steps of a tile, unrolled.  128 columns spill if they are: 16 query heads of 1 500, 4 of 2 048 keys took 264 us, 218 as a loop
+  constexpr int STEPS = sizeof(T) == 2 && DP >= 64 ? 1 : 4;
   constexpr int MP = RR_XA_KT + 4;           // a key's mask bytes of the tile's rows: a lane reads those of its four rows at once
   __shared__ __attribute__((aligned(16))) T sq[2][RR_XA_KT * Dm::PX];
   __shared__ __attribute__((aligned(16))) T sg[2][RR_XA_KT * Dm::PX];
@@ -831,7 +835,7 @@ __global__ __launch_bounds__(256, (DP == 128 && (sizeof(T) == 4 || KW == 2) ? 1 
     const T *tq = sq[at], *tg = sg[at];
     const uint32_t* fl = flag[at];
     const bool some = a.mask != nullptr || safe();      // (uniform)
-#pragma unroll
+#pragma unroll STEPS
     for (int n = 0; n < 4; n += M::PT) {
       if (SKIP && 16 * n >= rows) break;
       f32x4 s[KW][M::PT], dp[KW][M::PT];
