@@ -539,7 +539,7 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_dq(XAttn a) {
   using M = Mx<T>;
   using Dm = Dims<T, DP>;
   constexpr bool TIGHT = DP == 128 && QT == 2, SKIP = sizeof(T) == 4;
-  constexpr int STEPS = sizeof(T) == 2 && (ONE || DP == 128) ? 1 : 4;      // of a tile, unrolled (those spill if they are; the others gain 4%)
+  static constexpr int STEPS = sizeof(T) == 2 && (ONE || DP == 128) ? 1 : 4;      // of a tile, unrolled (those spill if they are; the others gain 4%)
   __shared__ __attribute__((aligned(16))) T sk[2][RR_XA_KT * Dm::PX];
   __shared__ __attribute__((aligned(16))) T sv[2][RR_XA_KT * Dm::PR];
   __shared__ uint32_t flag[2][2];
@@ -754,12 +754,12 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_dq(XAttn a) {
 
 // ------------------------------------------------------------------------------------------------ backward: dk, dv (walks over the rows)
 template <typename T, int DP, int KW>        // KW x 16 keys a wave
-__global__ __launch_bounds__(256, (DP == 128 && (sizeof(T) == 4 || KW == 2) ? 1 : 2)) void k_xattn_dkv(XAttn a) {
+__global__ __launch_bounds__(256, (DP == 128 ? 1 : 2)) void k_xattn_dkv(XAttn a) {
   using M = Mx<T>;
   using Dm = Dims<T, DP>;
   constexpr bool TIGHT = DP >= 64 && KW == 2, SKIP = sizeof(T) == 4;
   // steps of a tile, unrolled.  128 columns spill if they are: 16 query heads of 1 500, 4 of 2 048 keys took 264 us, 218 as a loop
-  constexpr int STEPS = sizeof(T) == 2 && DP >= 64 ? 1 : 4;
+  static constexpr int STEPS = sizeof(T) == 2 && DP >= 64 ? 1 : 4;
   constexpr int MP = RR_XA_KT + 4;           // a key's mask bytes of the tile's rows: a lane reads those of its four rows at once
   __shared__ __attribute__((aligned(16))) T sq[2][RR_XA_KT * Dm::PX];
   __shared__ __attribute__((aligned(16))) T sg[2][RR_XA_KT * Dm::PX];
@@ -978,11 +978,11 @@ int head_pad(int D) { return D <= 16 ? 16 : D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
 // rows (or keys) of a workgroup: 4 waves of 16 or 32
 struct Plan { int wide, nblk, nsplit, tiles_per_split; };
-Plan plan_for(long long kept, long long walked, long long outer, bool f32) {
+Plan plan_for(long long kept, long long walked, long long outer, bool narrow) {
   Plan p;
   // 16-bit types: with 16 rows a wave the reads of the staged tiles take LDS twice as long as the products take the matrix pipe, with 32 as long.
   // float32 products are eight times slower: 16 rows, more waves
-  p.wide = !f32 && kept > 64 ? 2 : 1;
+  p.wide = !narrow && kept > 64 ? 2 : 1;
   p.nblk = (int)((kept + 64 * p.wide - 1) / (64 * p.wide));
   const long long tiles = (walked + RR_XA_KT - 1) / RR_XA_KT;
   const long long blocks = outer * p.nblk;
@@ -1015,9 +1015,12 @@ int bwd_go(XAttn& a, const Plan& p, const Plan& pk, hipStream_t st) {
   const dim3 grid((unsigned)((long long)a.B * a.Hk * p.nsplit * p.nblk));
   a.nsplit = p.nsplit; a.tiles_per_split = p.tiles_per_split; a.nblk = p.nblk;
   if constexpr (sizeof(T) == 2) {
-    if (a.Lk <= RR_XA_KT && p.wide == 2) hipLaunchKernelGGL((k_xattn_dq<T, DP, 2, true>), grid, dim3(256), 0, st, a);
-    else if (a.Lk <= RR_XA_KT) hipLaunchKernelGGL((k_xattn_dq<T, DP, 1, true>), grid, dim3(256), 0, st, a);
-    else if (p.wide == 2) hipLaunchKernelGGL((k_xattn_dq<T, DP, 2, false>), grid, dim3(256), 0, st, a);
+    if (a.Lk <= RR_XA_KT) {
+      if constexpr (DP < 128) {
+        if (p.wide == 2) hipLaunchKernelGGL((k_xattn_dq<T, DP, 2, true>), grid, dim3(256), 0, st, a);
+      }
+      if (p.wide == 1) hipLaunchKernelGGL((k_xattn_dq<T, DP, 1, true>), grid, dim3(256), 0, st, a);
+    } else if (p.wide == 2) hipLaunchKernelGGL((k_xattn_dq<T, DP, 2, false>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((k_xattn_dq<T, DP, 1, false>), grid, dim3(256), 0, st, a);
   } else {
     hipLaunchKernelGGL((k_xattn_dq<T, DP, 1, false>), grid, dim3(256), 0, st, a);
@@ -1038,7 +1041,7 @@ int bwd_go(XAttn& a, const Plan& p, const Plan& pk, hipStream_t st) {
   return xa_launched();
 }
 
-struct Sizes { Plan q, k; size_t fwd, bwd; bool ok; };
+struct Sizes { Plan q, dq, k; size_t fwd, bwd; bool ok; };
 Sizes sizes_of(long long B, long long Lq, long long Lk, long long Hk, long long G, int D, int dtype) {
   Sizes s{};
   const long long lim = 0x7fffffffLL;
@@ -1048,10 +1051,13 @@ Sizes sizes_of(long long B, long long Lq, long long Lk, long long Hk, long long 
   if (!s.ok) return s;
   s.q = plan_for(G * Lq, Lk, B * Hk, dtype == RR_F32);
   s.k = plan_for(Lk > 0 ? Lk : 1, G * ((Lq + RR_XA_KT - 1) / RR_XA_KT) * RR_XA_KT, B * Hk, dtype == RR_F32);
-  if (B * Hk * s.q.nblk > lim / 256 || B * Hk * s.k.nblk > lim / 256 || B * Hk * G * Lq > lim) { s.ok = false; return s; }
+  // dq of 128 columns on keys of one tile holds too much for 32 rows a wave without spilling: 120 queries on 60 keys, 2 048 heads, 182 us spilling, 132 with one
+  // workgroup a CU, 97 with 16 rows a wave
+  s.dq = plan_for(G * Lq, Lk, B * Hk, dtype == RR_F32 || (D > 64 && Lk <= RR_XA_KT));
+  if (B * Hk * s.q.nblk > lim / 256 || B * Hk * s.dq.nblk > lim / 256 || B * Hk * s.k.nblk > lim / 256 || B * Hk * G * Lq > lim) { s.ok = false; return s; }
   const int DP = head_pad(D);
   s.fwd = s.q.nsplit > 1 ? (size_t)(B * Hk * G * Lq) * s.q.nsplit * (DP + 4) * 4 : 0;
-  const size_t b1 = s.q.nsplit > 1 ? (size_t)s.q.nsplit * B * Lq * Hk * G * D * 4 : 0, b2 = s.k.nsplit > 1 ? (size_t)s.k.nsplit * 2 * B * Lk * Hk * D * 4 : 0;
+  const size_t b1 = s.dq.nsplit > 1 ? (size_t)s.dq.nsplit * B * Lq * Hk * G * D * 4 : 0, b2 = s.k.nsplit > 1 ? (size_t)s.k.nsplit * 2 * B * Lk * Hk * D * 4 : 0;
   s.bwd = b1 > b2 ? b1 : b2;
   return s;
 }
@@ -1131,7 +1137,7 @@ extern "C" int rr_cross_attn_bwd(const XAttnIO* io, hipStream_t st) {
   const Sizes s = sizes_of(io->B, io->Lq, io->Lk, io->Hk, io->G, io->D, io->dtype);
   XAttn a;
   if (!s.ok || xa_fill(io, a, true) != RR_OK || (s.bwd > 0 && (io->workspace == nullptr || (size_t)io->workspace_bytes < s.bwd || !rr_aligned16(io->workspace)))) return RR_EINVAL;
-#define RR_CALL(T, DP) bwd_go<T, DP>(a, s.q, s.k, st)
+#define RR_CALL(T, DP) bwd_go<T, DP>(a, s.dq, s.k, st)
   if (io->dtype == RR_F32) { RR_XA_BY_DIM(float, RR_CALL) }
   if (io->dtype == RR_F16) { RR_XA_BY_DIM(rr_f16, RR_CALL) }
   RR_XA_BY_DIM(rr_bf16, RR_CALL)
