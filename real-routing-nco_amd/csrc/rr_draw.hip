@@ -1221,7 +1221,7 @@ int draw_rows(const Draw& a, hipStream_t st) {
 }
 
 template <typename T>
-int draw_go(const Draw& a, void* ws, hipStream_t st) {
+int draw_go(const Draw& a, bool stretches, void* ws, hipStream_t st) {
   const dim3 wg((unsigned)((a.R + 3) / 4)), wg16((unsigned)((a.R + 15) / 16));
   // without top-k and top-p rows of up to 128 keys take 16 lanes: the scans, the logarithm and the choice are paid once for four rows
   // (51 200 x 100 float32: 27 us with a wave a row)
@@ -1242,7 +1242,7 @@ int draw_go(const Draw& a, void* ws, hipStream_t st) {
   else if (a.V <= 512) hipLaunchKernelGGL((k_draw_wave<T, 8>), wg, dim3(256), 0, st, a);
   else if (a.V <= 1024) hipLaunchKernelGGL((k_draw_wave<T, 16>), wg, dim3(256), 0, st, a);
   else {
-    return by_stretches(a.R, a.V) ? draw_long<T>(a, ws, st) : draw_rows<T>(a, st);
+    return stretches ? draw_long<T>(a, ws, st) : draw_rows<T>(a, st);
   }
   return rr_check(hipGetLastError());
 }
@@ -1254,7 +1254,7 @@ extern "C" long long rr_draw_workspace(int R, int V) { return R > 0 && V > 0 && 
 extern "C" int rr_draw(int dtype, const void* logits, long long ld, const uint8_t* mask, long long ldm, const float* uniforms, int64_t* index, float* logp, int R, int V,
                        double temperature, int top_k, double top_p, double min_p, const float* row_temperature, const int* row_top_k, const float* row_top_p,
                        const float* row_min_p, void* workspace, long long workspace_bytes, hipStream_t st) {
-  if (R < 0 || V < 1 || V > (1 << 24) || logits == nullptr || uniforms == nullptr || index == nullptr || logp == nullptr || ld < 0 || ldm < 0) return RR_EINVAL;
+  if (dtype < RR_F32 || dtype > RR_BF16 || R < 0 || V < 1 || V > (1 << 24) || logits == nullptr || uniforms == nullptr || index == nullptr || logp == nullptr || ld < 0 || ldm < 0) return RR_EINVAL;
   if ((row_temperature == nullptr && !(temperature >= 0.0 && temperature < 1e30)) || (row_top_p == nullptr && !(top_p >= 0.0 && top_p <= 1.0)) ||
       (row_min_p == nullptr && !(min_p >= 0.0 && min_p <= 1.0)) || (row_top_k == nullptr && top_k < 0))
     return RR_EINVAL;
@@ -1262,10 +1262,24 @@ extern "C" int rr_draw(int dtype, const void* logits, long long ld, const uint8_
   if (by_stretches(R, V) && (workspace == nullptr || (size_t)workspace_bytes < long_bytes(R, V) || !rr_aligned16(workspace))) return RR_EINVAL;
   const Draw a = {logits, mask, uniforms, index, logp, row_temperature, row_top_p, row_min_p, row_top_k, temperature, 1.44269504088896340736 / temperature, top_p, min_p, ld, ldm,
                   top_k, R, V};
-  switch (dtype) {
-    case RR_F32: return draw_go<float>(a, workspace, st);
-    case RR_F16: return draw_go<rr_f16>(a, workspace, st);
-    case RR_BF16: return draw_go<rr_bf16>(a, workspace, st);
+  // a launch holds fewer than 2^32 threads: at most 64 a row up to 1 024 keys, at most 1 024 beyond
+  const int most = V <= 1024 ? 1 << 25 : 1 << 21, size = dtype == RR_F32 ? 4 : 2;
+  for (long long r = 0; r < R; r += most) {
+    Draw b = a;
+    b.R = (int)(R - r < most ? R - r : most);
+    b.logits = (const char*)logits + r * ld * size;
+    if (mask != nullptr) b.mask += r * ldm;
+    b.u += r;
+    b.index += r;
+    b.logp += r;
+    if (b.pt != nullptr) b.pt += r;
+    if (b.pk != nullptr) b.pk += r;
+    if (b.pp != nullptr) b.pp += r;
+    if (b.pm != nullptr) b.pm += r;
+    const int rc = dtype == RR_F32 ? draw_go<float>(b, by_stretches(R, V), workspace, st)
+                   : dtype == RR_F16 ? draw_go<rr_f16>(b, by_stretches(R, V), workspace, st)
+                                     : draw_go<rr_bf16>(b, by_stretches(R, V), workspace, st);
+    if (rc != RR_OK) return rc;
   }
-  return RR_EINVAL;
+  return RR_OK;
 }

@@ -4,7 +4,7 @@
 //
 //   forward    s = rsqrt(mean h^2 + eps); the norm is taken of the 32-bit sum, h and y are rounded once each when stored
 //   backward   g = dy w, n = h s:   dx = dr = dh + s (g - n mean(g n)),   dw = sum over the rows of dy n
-//   8 bits     a = max |y| over a group of 128 columns, scale = a / 448 (1 for a group of zeros), q = e4m3(y / scale)
+//   8 bits     a = max |y| over a group of 128 columns, scale = max(a / 448, 2^-126) (1 for a group of zeros), q = e4m3(y / scale)
 //
 // Bound by memory: each tensor is read and written once, a row's elements stay in registers between the two uses.
 // A team of TPR lanes owns a row (TPR 16 .. 1024, chosen so that a lane holds 16 bytes up to a width of 64 such pieces and at
@@ -30,6 +30,21 @@ __device__ __forceinline__ float team_sum(float v, float* red) {          // red
     for (int i = 0; i < NW; ++i) v += red[i];                              // TPR > 64: the workgroup is one team
   }
   return v;
+}
+
+// 1 / sqrt(mean h^2 + eps) from the sum of squares.  Where that left the range of 32 bits (elements beyond 1e18, or under 1e-15 with hardly an eps) it is taken
+// again of the elements times a power of two
+template <int TPR, int NC, int VEC>
+__device__ __forceinline__ float rstd_of(float ss, const float (&v)[NC][VEC], int E, float eps, float* red) {
+  const float m = ss / (float)E + eps;
+  if (m >= 0x1p-100f && m < INFINITY) return 1.0f / sqrtf(m);            // (one value in all lanes of the team)
+  const float f = m < 1.f ? 0x1p75f : 0x1p-75f;
+  ss = 0.f;
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) ss = fmaf(v[c][i] * f, v[c][i] * f, ss);
+  return f / sqrtf(team_sum<TPR>(ss, red) / (float)E + eps * f * f);
 }
 
 template <typename T> struct code;
@@ -88,7 +103,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_fwd(const T* __re
     for (int i = 0; i < VEC; ++i) ss = fmaf(v[c][i], v[c][i], ss);
   }
   ss = team_sum<TPR>(ss, red);
-  const float s = 1.0f / sqrtf(ss / (float)E + eps);
+  const float s = rstd_of<TPR>(ss, v, E, eps, red);
   if (rstd != nullptr && live && lane == 0) rstd[row] = s;
   if constexpr (!FP8) {
 #pragma unroll
@@ -123,7 +138,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_rms_fwd(const T* __re
     for (int c = 0; c < NC; ++c) {
       const int col = (c * TPR + lane) * VEC;
       if (live && col < E) {
-        const float sc = a[c] == 0.f ? 1.f : a[c] / 448.0f;
+        const float sc = a[c] == 0.f ? 1.f : fmaxf(a[c] / 448.0f, 0x1p-126f);      // (a smaller one has no finite reciprocal)
         if (col % 128 == 0) qs[row * G + col / 128] = sc;
         const float inv = 1.0f / sc;                                       // one quotient a group; y * inv is off by a step of float32 at the most
         uint32_t p[VEC / 4];
@@ -300,8 +315,20 @@ extern "C" int rr_add_rms_norm(int dtype, const void* x, long long ldx, const vo
                                uint8_t* q, float* qscale, long long rows, int E, float eps, hipStream_t st) {
   if (rows < 0 || E < 1 || E > 16384 || x == nullptr || rows > 0x7fffffffLL || (y == nullptr) == (q == nullptr) || (q == nullptr) != (qscale == nullptr) || ldx < 0 || ldr < 0)
     return RR_EINVAL;
-  if (rows == 0) return RR_OK;
   if (res == nullptr) ldr = 0;
+  // a launch holds fewer than 2^32 threads: 16 .. 64 a row up to 128 columns, at most 1 024 beyond
+  const long long most = E <= 128 ? 1 << 25 : 1 << 21, size = dtype == RR_F32 ? 4 : 2, G = (E + 127) / 128;
+  for (; rows > most; rows -= most) {
+    const int rc = rr_add_rms_norm(dtype, x, ldx, res, ldr, w, w_is_f32, y, h, rstd, q, qscale, most, E, eps, st);
+    if (rc != RR_OK) return rc;
+    x = (const char*)x + most * ldx * size;
+    if (res != nullptr) res = (const char*)res + most * ldr * size;
+    if (y != nullptr) y = (char*)y + most * E * size;
+    if (h != nullptr) h = (char*)h + most * E * size;
+    if (rstd != nullptr) rstd += most;
+    if (q != nullptr) { q += most * E; qscale += most * G; }
+  }
+  if (rows == 0) return RR_OK;
   switch (dtype) {
     case RR_F32: return norm_fwd<float>(x, ldx, res, ldr, w, w_is_f32, y, h, rstd, q, qscale, rows, E, eps, st);
     case RR_F16: return norm_fwd<rr_f16>(x, ldx, res, ldr, w, w_is_f32, y, h, rstd, q, qscale, rows, E, eps, st);

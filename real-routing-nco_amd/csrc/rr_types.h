@@ -1,4 +1,4 @@
-// Element types of the operators that serve float32, float16 and bfloat16 alike (rr_norm.hip, rr_xattn.hip, rr_sample.hip).
+// Element types of the operators that serve float32, float16 and bfloat16 alike (rr_norm.hip, rr_xattn.hip, rr_draw.hip).
 // Every sum, maximum and statistic is held in 32 bits or more; a value is rounded to its type once, when it is stored.
 #pragma once
 #include "rr_common.h"
@@ -32,17 +32,13 @@ __device__ __forceinline__ void rr_load_n(const T* __restrict__ p, float (&x)[N]
 }
 template <typename T, int N>
 __device__ __forceinline__ void rr_store_n(T* __restrict__ p, const float (&x)[N]) {
-  if constexpr (N == 1) {
-    p[0] = (T)x[0];
-  } else {
-    static_assert(N * sizeof(T) == 16, "one 16-byte access");
-    typedef T V __attribute__((ext_vector_type(N)));
-    typedef V U __attribute__((aligned(sizeof(T))));
-    V v;
+  static_assert(N * sizeof(T) == 16, "one 16-byte access");
+  typedef T V __attribute__((ext_vector_type(N)));
+  typedef V U __attribute__((aligned(sizeof(T))));
+  V v;
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = (T)x[i];
-    *reinterpret_cast<U*>(p) = v;
-  }
+  for (int i = 0; i < N; ++i) v[i] = (T)x[i];
+  *reinterpret_cast<U*>(p) = v;
 }
 // the first n of them (the others as zeros, unwritten)
 template <typename T, int N>

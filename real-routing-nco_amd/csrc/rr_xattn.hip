@@ -972,8 +972,6 @@ __global__ __launch_bounds__(256) void k_xattn_add(const float* __restrict__ par
 }
 
 // ------------------------------------------------------------------------------------------------ host
-int xa_launched() { return hipGetLastError() == hipSuccess ? RR_OK : RR_ELAUNCH; }
-
 int head_pad(int D) { return D <= 16 ? 16 : D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 
 // rows (or keys) of a workgroup: 4 waves of 16 or 32
@@ -1008,7 +1006,7 @@ int fwd_go(XAttn& a, const Plan& p, hipStream_t st) {
   }
   if (p.wide == 1) hipLaunchKernelGGL((k_xattn_fwd<T, DP, 1>), grid, dim3(256), 0, st, a);
   if (p.nsplit > 1) hipLaunchKernelGGL((k_xattn_join<T, DP>), dim3((unsigned)(((long long)a.B * a.Hk * a.G * a.Lq + 1024 / DP - 1) / (1024 / DP))), dim3(256), 0, st, a);
-  return xa_launched();
+  return rr_check(hipGetLastError());
 }
 template <typename T, int DP>
 int bwd_go(XAttn& a, const Plan& p, const Plan& pk, hipStream_t st) {
@@ -1038,15 +1036,15 @@ int bwd_go(XAttn& a, const Plan& p, const Plan& pk, hipStream_t st) {
     hipLaunchKernelGGL((k_xattn_add<T>), blocks(nk4), dim3(256), 0, st, a.part, 8 * nk4, pk.nsplit, (T*)a.dk, nk4);
     hipLaunchKernelGGL((k_xattn_add<T>), blocks(nk4), dim3(256), 0, st, a.part + 4 * nk4, 8 * nk4, pk.nsplit, (T*)a.dv, nk4);
   }
-  return xa_launched();
+  return rr_check(hipGetLastError());
 }
 
 struct Sizes { Plan q, dq, k; size_t fwd, bwd; bool ok; };
 Sizes sizes_of(long long B, long long Lq, long long Lk, long long Hk, long long G, int D, int dtype) {
   Sizes s{};
   const long long lim = 0x7fffffffLL;
-  // counts that index rows, keys and workgroups are 32-bit; offsets into the tensors are 64-bit
-  s.ok = B >= 1 && Lq >= 1 && Lk >= 0 && Hk >= 1 && G >= 1 && D >= 8 && D <= 128 && D % 8 == 0 && Lq <= lim && Lk <= lim - 256 && G * (Lq + 64) <= lim - 256 && B <= lim && Hk <= lim &&
+  // counts that index rows, keys and workgroups are 32-bit (the last split's end may pass Lk by a tile a split); offsets into the tensors are 64-bit
+  s.ok = B >= 1 && Lq >= 1 && Lk >= 0 && Hk >= 1 && G >= 1 && D >= 8 && D <= 128 && D % 8 == 0 && Lq <= lim && Lk <= lim - 65536 && G * (Lq + 64) <= lim - 256 && B <= lim && Hk <= lim &&
          B * Hk <= lim && G * Hk <= lim;
   if (!s.ok) return s;
   s.q = plan_for(G * Lq, Lk, B * Hk, dtype == RR_F32);

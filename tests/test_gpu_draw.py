@@ -208,3 +208,22 @@ def test_same_choices_on_another_stream_and_in_a_graph():
         eager = draw(nx, nu, nm, nl, nul)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, eager)), i
+
+
+@pytest.mark.parametrize("R,V,s", [((1 << 25) + 5, 2, dict()), ((1 << 25) + 5, 2, dict(k=1)), ((1 << 21) + 5, 1040, dict(k=40, p=0.9))], ids=["narrow", "filtered", "wide"])
+def test_more_rows_than_a_launch_holds(R, V, s):
+    """Rows in front of, around and behind the border between two launches are the same as on their own, settings of each row among them."""
+    g = torch.Generator("cuda").manual_seed(V)
+    x = torch.randn(R, V, device="cuda", generator=g, dtype=torch.bfloat16)
+    u = torch.rand(R, device="cuda", generator=g)
+    t = 0.5 + torch.rand(R, device="cuda", generator=g)
+    mask = torch.rand(1, V, device="cuda", generator=g) < 0.9
+    mask[0, 0] = True
+    set_ = dict(top_k=s.get("k", 0), top_p=s.get("p", 0.0))
+    idx, lp = _ops().sample(x, u, temperature=t, mask=mask, **set_)
+    border = R & ~0xff
+    for part in (slice(0, 64), slice(border - 100, R)):
+        i1, l1 = _ops().sample(x[part], u[part], temperature=t[part], mask=mask, **set_)
+        assert torch.equal(idx[part], i1) and torch.equal(lp[part], l1)
+    tail = slice(R - 20, R)
+    check(x[tail], u[tail], mask=mask, t=t[tail], **s)

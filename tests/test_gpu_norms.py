@@ -216,3 +216,58 @@ def test_eight_bit_form(dt, shape):
         assert not q.double()[..., :128].any() and bool((scale[..., 0] == 1).all())
     same_h = _ops().add_rms_norm(x, r, w)[1]
     assert torch.equal(h, same_h)
+
+
+@pytest.mark.parametrize("E", [24, 128, 300, 5000])
+@pytest.mark.parametrize("dt,big,eps", [(torch.float32, 1e25, 1e-5), (torch.bfloat16, 1e25, 1e-5), (torch.float32, 1e-25, 0.0), (torch.bfloat16, 1e-25, 0.0), (torch.float16, 6e4, 1e-5)])
+def test_rows_whose_squares_leave_32_bits(dt, big, eps, E):
+    """The elements' squares overflow, or vanish, in 32 bits; the norm does not.  Tolerances as above: the power of two that the sum is taken with is exact."""
+    g = torch.Generator("cuda").manual_seed(E)
+    x = (big * (0.5 + 0.5 * torch.rand(5, E, device="cuda", generator=g))).to(dt).requires_grad_()
+    w = torch.randn(E, device="cuda", generator=g).to(dt).requires_grad_()
+    dy = torch.randn(5, E, device="cuda", generator=g).to(dt)
+    ref = reference(x, None, w, eps, dy)
+    y, _ = _ops().add_rms_norm(x, None, w, eps)
+    close("y", y.detach(), tuple(t.detach() for t in ref["y"]))
+    dw, = torch.autograd.grad(y, (w,), dy)
+    close("dw", dw, tuple(t.detach() for t in ref["dw"]))
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_eight_bit_groups_of_tiny_values(dt):
+    """y of 2^-131 .. 0 in a group: its 448th part has no finite reciprocal, the scale is 2^-126 and nothing becomes NaN.
+    y / scale is sqrt(2) 2^-5 here: with three bits behind the leading one its step is 2^-8, half of it 2^-9 (the first bound written here took e4m3's smallest
+    step, 2^-9, which holds below 2^-5 only); 2^-22 more for y's own error, a step of the subnormal numbers, 2^-149, over 2^-126."""
+    x = torch.ones(3, 256, device="cuda", dtype=dt)
+    x[:, ::2] = 0.0
+    w = torch.full((256,), 2.0 ** -131, device="cuda", dtype=torch.float32)
+    w[128:] = 1.0
+    q, scale, _ = _ops().add_rms_norm_fp8(x, None, w)
+    y = reference(x, None, w, 1e-5)["y"][0]
+    assert bool((scale[:, 0] == 2.0 ** -126).all())
+    z = y[:, :128] / 2.0 ** -126
+    assert bool(((q.double()[:, :128] - z).abs() <= 2.0 ** -9 + 2.0 ** -22).all())
+    assert not q.double()[:, ::2].any()
+
+
+@pytest.mark.parametrize("rows,E", [((1 << 25) + 3, 2), ((1 << 21) + 5, 136)], ids=["narrow", "wide"])
+def test_more_rows_than_a_launch_holds(rows, E):
+    """Rows in front of, around and behind the border between two launches are the same as on their own."""
+    g = torch.Generator("cuda").manual_seed(E)
+    x = torch.randn(rows, E, device="cuda", generator=g, dtype=torch.bfloat16)
+    w = torch.randn(E, device="cuda", generator=g)
+    one = x[7:8].expand(rows, E)                                                  # (a residual of stride 0)
+    y, h = _ops().add_rms_norm(x, one, w)
+    q, scale, h8 = _ops().add_rms_norm_fp8(x, one, w)
+    border = rows & ~0xff
+    for part in (slice(0, 64), slice(border - 100, rows)):
+        y1, h1 = _ops().add_rms_norm(x[part], one[part], w)
+        q1, s1, _ = _ops().add_rms_norm_fp8(x[part], one[part], w)
+        assert torch.equal(y[part], y1) and torch.equal(h[part], h1) and torch.equal(h8[part], h1)
+        assert torch.equal(q[part].view(torch.uint8), q1.view(torch.uint8)) and torch.equal(scale[part], s1)
+    ref = reference(x[-50:], one[-50:], w, 1e-5)
+    close("y", y[-50:], ref["y"])
+    xg, wg = x[:rows].requires_grad_(), w.clone().requires_grad_()
+    dx, = torch.autograd.grad(_ops().add_rms_norm(xg, one, wg)[0], (xg,), h)
+    ref = reference(x[-50:], one[-50:], w, 1e-5, h[-50:])
+    close("dx", dx[-50:], tuple(t.detach() for t in ref["dx"]))
