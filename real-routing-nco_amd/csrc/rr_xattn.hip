@@ -216,13 +216,26 @@ __device__ __forceinline__ uint32_t mask4(const uint8_t* row, int key, int Lk) {
   for (int i = 0; i < Lk; ++i) m |= (uint32_t)row[i] << (8 * i);
   return key < 4 ? m >> (8 * key) : 0u;
 }
+// the same at key k0 + i of a tile; whole tiles need none of the conditions (WHOLE: where there are registers for both)
+template <bool WHOLE>
+__device__ __forceinline__ uint32_t mask_at(const uint8_t* row, int k0, int i, int Lk) {
+  uint32_t m;
+  if (WHOLE && k0 + RR_XA_KT <= Lk) __builtin_memcpy(&m, row + k0 + i, 4);          // (uniform)
+  else m = mask4(row, k0 + i, Lk);
+  return m;
+}
 __device__ __forceinline__ uint32_t first_bytes(uint32_t b, int n) {     // the first n of four bytes
   return n >= 4 ? b : n <= 0 ? 0u : b & ((1u << (8 * n)) - 1u);
 }
-// x where the byte of its place is set, y elsewhere (selects without branches: the four values stay in their registers)
+// x where the byte of its place is 1, y where it is 0.  By bit fields (two instructions a value, three with comparisons) and without branches: the four values stay
+// in their registers
 __device__ __forceinline__ void keep4(f32x4& x, uint32_t bytes, float y) {
-  const float a = x[0], b = x[1], c = x[2], d = x[3];
-  const f32x4 r = {bytes & 0xffu ? a : y, bytes & 0xff00u ? b : y, bytes & 0xff0000u ? c : y, bytes & 0xff000000u ? d : y};
+  f32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t k = (uint32_t)__builtin_amdgcn_sbfe((int)bytes, 8 * i, 1);
+    r[i] = __uint_as_float((__float_as_uint(x[i]) & k) | (__float_as_uint(y) & ~k));
+  }
   x = r;
 }
 // the flags of four consecutive rows of a tile as bytes
@@ -256,12 +269,12 @@ __device__ __forceinline__ Blk block_of(const XAttn& a) {
   // workgroups go to the eight XCDs in turn: each gets one stretch of the work, so that the heads of an instance, which share its cache lines and
   // its mask, meet in one L2
   const unsigned n = gridDim.x, x = blockIdx.x & 7u, q = n >> 3, r = n & 7u;
-  long long i = x * q + (x < r ? x : r) + (blockIdx.x >> 3);
+  unsigned i = x * q + (x < r ? x : r) + (blockIdx.x >> 3);
   Blk w;
-  w.blk = (int)(i % a.nblk); i /= a.nblk;
-  w.split = (int)(i % a.nsplit); i /= a.nsplit;
-  w.hk = (int)(i % a.Hk);
-  w.b = (int)(i / a.Hk);
+  w.blk = (int)(i % (unsigned)a.nblk); i /= (unsigned)a.nblk;
+  w.split = (int)(i % (unsigned)a.nsplit); i /= (unsigned)a.nsplit;
+  w.hk = (int)(i % (unsigned)a.Hk);
+  w.b = (int)(i / (unsigned)a.Hk);
   return w;
 }
 
@@ -320,7 +333,7 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_fwd(XAttn a) {
 #pragma unroll
       for (int t = 0; t < QT; ++t)
 #pragma unroll
-        for (int n = 0; n < 4; ++n) mb[t][n] = mask4(mrow[t], k0 + 16 * n + 4 * g, a.Lk);
+        for (int n = 0; n < 4; ++n) mb[t][n] = mask_at<!TIGHT>(mrow[t], k0, 16 * n + 4 * g, a.Lk);
     }
     const int parts = SKIP ? (seen - k0 + 15) >> 4 : 4;
     f32x4 s[QT][4];
@@ -343,7 +356,10 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_fwd(XAttn a) {
       for (int t = 0; t < QT; ++t)
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-          keep4(s[t][n], first_bytes(a.mask != nullptr ? mb[t][n] : 0x01010101u, seen - (k0 + 16 * n + 4 * g)), -INFINITY);
+          if (SKIP && n >= parts) continue;
+          uint32_t b = a.mask != nullptr ? mb[t][n] : 0x01010101u;
+          if (k0 + RR_XA_KT > seen) b = first_bytes(b, seen - (k0 + 16 * n + 4 * g));
+          keep4(s[t][n], b, -INFINITY);
         }
     }
     // the running maximum moves only when a score passes it by 2^8: weights up to that are as exact as those up to one, and a tile
@@ -354,9 +370,11 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_fwd(XAttn a) {
     for (int t = 0; t < QT; ++t) {
       mx[t] = s[t][0][0];
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
+      for (int n = 0; n < 4; ++n) {
+        if (SKIP && n >= parts) break;
 #pragma unroll
         for (int i = 0; i < 4; ++i) mx[t] = fmaxf(mx[t], s[t][n][i]);
+      }
       move |= mx[t] * c2 > m[t] + 8.0f;
     }
     if (__any(move)) {
@@ -375,12 +393,14 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_fwd(XAttn a) {
       const float mu = finite_or_zero(m[t]);
       float sum = 0.f;
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
+      for (int n = 0; n < 4; ++n) {
+        if (SKIP && n >= parts) break;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           s[t][n][i] = __builtin_amdgcn_exp2f(fmaf(s[t][n][i], c2, -mu));
           sum += s[t][n][i];
         }
+      }
       l[t] += sum;
     }
 #pragma unroll
@@ -599,7 +619,7 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_dq(XAttn a) {
 #pragma unroll
       for (int t = 0; t < QT; ++t)
 #pragma unroll
-        for (int n = 0; n < 4; ++n) mb[t][n] = mask4(mrow[t], k0 + 16 * n + 4 * g, a.Lk);
+        for (int n = 0; n < 4; ++n) mb[t][n] = mask_at<!TIGHT>(mrow[t], k0, 16 * n + 4 * g, a.Lk);
     }
     float dsum[QT];
 #pragma unroll
