@@ -460,7 +460,7 @@ int rr_select_matnet(const float* logits, const uint8_t* mask, const int64_t* ac
  * Cross attention: G * Hk query heads on Hk key heads, out = softmax(scale q k^T over the keys that may be seen) v, lse = log sum exp
  * (a query that sees nothing: zeros, -inf).  q [B][Lq][G*Hk][D], k, v [B][Lk][Hk][D] by element strides (batch, position, head), the
  * last axis contiguous, bases and strides on 16 bytes; D a multiple of 8 up to 128.  mask: bytes [B][G*Hk][Lq][Lk] by strides (batch, head,
- * query), 1 = may be seen, or NULL; kv_lens [B] int32 / int64 or NULL.  out, dq [B][Lq][G*Hk][D], dk, dv [B][Lk][Hk][D], lse and delta
+ * query), 1 = may be seen, 0 = not, or NULL; kv_lens [B] int32 / int64 or NULL.  out, dq [B][Lq][G*Hk][D], dk, dv [B][Lk][Hk][D], lse and delta
  * [B][G*Hk][Lq] (delta: scratch of the backward) are contiguous.  workspace: rr_cross_attn_workspace bytes (-1: sizes refused). */
 typedef struct {
   const void *q, *k, *v;
