@@ -13,6 +13,11 @@
 // the inputs' type for the second product (half a step of a weight <= 1, under the rounding of the output).
 // float32 runs on v_mfma_f32_16x16x4 (exact products), 16-bit types on v_mfma_f32_16x16x32.
 // The backward recomputes P from lse; dq walks over keys, (dk, dv) over rows: no atomics, the same result every time.
+// Products run at a raised wave priority in the forward and dq: with two waves a SIMD one computes weights while the other holds the matrix pipe
+// (forward 2 000 x 4 099, 64 heads of 128: 372 -> 360 us, dq of 1 500 x 2 049, 32 heads of 64: 69.4 -> 68.2; dk, dv: nothing).
+// Bounds and figures (float16 / bfloat16 unless said): forward of 2 000 x 4 099, 64 heads of 128, 740 TFLOP/s, matrix pipe 29% and vector pipe 34% busy, the rest
+// waits that two waves a SIMD (253 registers) do not hide.  One token on 48 x 8 192 states, 4 key heads of 128: 132 us, 4.6 TB/s, the copy's rate.  float32 with heads
+// of 16 (512 x 100 on 100): 66 us, bound by issue (products 32%, vector instructions 48%).  Backward of 2 x 1 500 on 2 049, 16 / 4 heads of 64: dq 68 us, (dk, dv) 79 us.
 // Few rows: the key axis is split over workgroups and joined by a second launch.
 // Non-finite values where nothing may look (a masked key whose value is NaN): 0 * NaN would spoil the products, so a workgroup
 // whose accumulators end non-finite walks its tiles once more with the non-finite 16-byte pieces replaced by zeros and their
@@ -335,6 +340,7 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_fwd(XAttn a) {
 #pragma unroll
         for (int n = 0; n < 4; ++n) mb[t][n] = mask_at<!TIGHT>(mrow[t], k0, 16 * n + 4 * g, a.Lk);
     }
+    __builtin_amdgcn_s_setprio(1);
     const int parts = SKIP ? (seen - k0 + 15) >> 4 : 4;
     f32x4 s[QT][4];
 #pragma unroll
@@ -351,6 +357,7 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_fwd(XAttn a) {
       }
       in_order<TIGHT>();
     }
+    __builtin_amdgcn_s_setprio(0);
     if (a.mask != nullptr || k0 + RR_XA_KT > seen) {
 #pragma unroll
       for (int t = 0; t < QT; ++t)
@@ -403,6 +410,7 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_fwd(XAttn a) {
       }
       l[t] += sum;
     }
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int n = 0; n < 4; n += M::PT) {
       if (SKIP && n >= parts) break;
@@ -417,6 +425,7 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_fwd(XAttn a) {
         if ((d & 3) == 3) in_order<TIGHT>();
       }
     }
+    __builtin_amdgcn_s_setprio(0);
     const uint32_t* fl = flag[at];
     if constexpr (safe()) if (fl[0] | fl[1]) {               // rare: what visible keys hold in the pieces that were zeroed
 #pragma unroll
@@ -631,6 +640,7 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_dq(XAttn a) {
     for (int n = 0; n < 4; n += M::PT) {
       if (SKIP && k0 + 16 * n >= seen) break;
       f32x4 s[QT][M::PT], dp[QT][M::PT];
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int u = 0; u < M::PT; ++u) {
 #pragma unroll
@@ -644,6 +654,7 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_dq(XAttn a) {
         }
         in_order<TIGHT>();
       }
+      __builtin_amdgcn_s_setprio(0);
       if (ONE && phase == 0) {
 #pragma unroll
         for (int t = 0; t < QT; ++t)
@@ -677,6 +688,7 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_dq(XAttn a) {
         }
         pf[t] = M::pack(s[t]);
       }
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int d = 0; d < Dm::DT; ++d) {
         const typename M::Frag f = M::tr(tk, Dm::PX, 16 * n, 16 * d, lane);
@@ -684,6 +696,7 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_dq(XAttn a) {
         for (int t = 0; t < QT; ++t) o[t][d] = M::mma(f, pf[t], o[t][d]);
         if ((d & 3) == 3) in_order<TIGHT>();
       }
+      __builtin_amdgcn_s_setprio(0);
     }
     if (ONE && phase == 0) {
 #pragma unroll
