@@ -815,7 +815,8 @@ __global__ __launch_bounds__(256, (DP == 128 ? 1 : 2)) void k_xattn_dkv(XAttn a)
   last = block0 < seen ? (last < a.G * per_head ? last : a.G * per_head) : first;      // (a workgroup behind the last key only writes zeros)
   Piece<T, DP> pq, pg;
   float nl = 0.f, nd = 0.f;                                              // the tile's lse (in powers of two) and delta, a row a thread
-  uint32_t nm[4 * KW];                                                   // its mask: four keys' bytes of a row, 4 KW times a thread
+  uint32_t nm[4 * KW];                                                   // its mask: KW times four keys' bytes of four rows a thread
+  const int mrow = threadIdx.x / (16 * KW) * 4;                          // the first of them
   auto load_tile = [&](int tile) {
     const int h = tile / per_head, s0 = (tile - h * per_head) * RR_XA_KT, rows = a.Lq - s0, head = w.hk * a.G + h;
     pq.load(qp + h * a.qh + s0 * a.ql, a.ql, rows, a.D);
@@ -830,7 +831,7 @@ __global__ __launch_bounds__(256, (DP == 128 ? 1 : 2)) void k_xattn_dkv(XAttn a)
       const int key = block0 + threadIdx.x % (16 * KW) * 4;
 #pragma unroll
       for (int c = 0; c < 4 * KW; ++c) {
-        const int r = threadIdx.x / (16 * KW) + c * (256 / (16 * KW));
+        const int r = mrow + c / 4 * (256 / (4 * KW)) + c % 4;
         nm[c] = mask4(mp + (r < rows ? r : rows - 1) * a.ml, key, a.Lk);
       }
     }
@@ -841,10 +842,14 @@ __global__ __launch_bounds__(256, (DP == 128 ? 1 : 2)) void k_xattn_dkv(XAttn a)
     if (threadIdx.x < RR_XA_KT) { sl[at][threadIdx.x] = nl; sd[at][threadIdx.x] = nd; }
     if (a.mask != nullptr) {
 #pragma unroll
-      for (int c = 0; c < 4 * KW; ++c) {
-        const int r = threadIdx.x / (16 * KW) + c * (256 / (16 * KW)), key = threadIdx.x % (16 * KW) * 4;
+      for (int c = 0; c < 4 * KW; c += 4) {                              // four rows by four keys, turned over
+        const uint32_t lo0 = __builtin_amdgcn_perm(nm[c + 1], nm[c], 0x05010400), hi0 = __builtin_amdgcn_perm(nm[c + 1], nm[c], 0x07030602);
+        const uint32_t lo1 = __builtin_amdgcn_perm(nm[c + 3], nm[c + 2], 0x05010400), hi1 = __builtin_amdgcn_perm(nm[c + 3], nm[c + 2], 0x07030602);
+        const uint32_t k4[4] = {__builtin_amdgcn_perm(lo1, lo0, 0x05040100), __builtin_amdgcn_perm(lo1, lo0, 0x07060302), __builtin_amdgcn_perm(hi1, hi0, 0x05040100),
+                                __builtin_amdgcn_perm(hi1, hi0, 0x07060302)};
+        const int r = mrow + c / 4 * (256 / (4 * KW)), key = threadIdx.x % (16 * KW) * 4;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sm[at][(key + e) * MP + r] = (uint8_t)(nm[c] >> (8 * e));
+        for (int e = 0; e < 4; ++e) *reinterpret_cast<uint32_t*>(&sm[at][(key + e) * MP + r]) = k4[e];
       }
     }
   };
