@@ -227,3 +227,23 @@ def test_more_rows_than_a_launch_holds(R, V, s):
         assert torch.equal(idx[part], i1) and torch.equal(lp[part], l1)
     tail = slice(R - 20, R)
     check(x[tail], u[tail], mask=mask, t=t[tail], **s)
+
+
+def test_calls_on_two_streams_at_once():
+    """Long rows (a workspace each) and short ones run against each other on two streams."""
+    x, u, _ = make(torch.bfloat16, 9, 60000, seed=5)
+    y, w, _ = make(torch.float32, 9, 40000, seed=6)
+    ops = _ops()
+    calls = [lambda: ops.sample(x, u, top_p=0.9, top_k=700), lambda: ops.sample(y, w, temperature=0.5, min_p=0.01)]
+    alone = [c() for c in calls]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(calls[i]())
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for r in got[i] for a, b in zip(alone[i], r))

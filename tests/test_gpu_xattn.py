@@ -313,3 +313,43 @@ def test_offsets_beyond_32_bits():
     assert k.stride(0) > 2 ** 31 - 1
     got = _ops().cross_attention(q, k, k)
     close("out", got, reference(q, k, k)["out"])
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("c", [(2, 5, 1, 2, 2, 16, "rows"), (2, 70, 2, 4, 2, 32, "rows"), (3, 9, 3, 2, 1, 64, "heads"), (2, 40, 5, 2, 2, 128, "both"),
+                               (2, 100, 64, 4, 4, 16, "both"), (3, 90, 128, 4, 2, 32, "both"), (2, 129, 192, 2, 2, 128, "both"),
+                               (1, 1, 4096, 4, 2, 64, "both"), (2, 120, 60, 4, 2, 128, "rows")], ids=lambda c: "-".join(map(str, c)))
+def test_masks_of_a_few_keys_and_of_whole_tiles(dt, c):
+    q, k, v, m, lens, do = make(dt, *c, seed=11)
+    got, ref = run(q, k, v, m, lens, do), reference(q, k, v, m, lens, do=do)
+    for n in ("out", "lse", "dq", "dk", "dv"):
+        close(n, got[n], ref[n])
+
+
+def test_calls_on_two_streams_at_once():
+    """Split forward and backward calls (workspaces of their own) run against each other, none waits for the other."""
+    cases = [make(torch.bfloat16, 1, n, 6000, 4, 2, 64, "keys", seed=n) for n in (3, 70)]
+    alone = [run(*c) for c in cases]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(run(*cases[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            assert all(torch.equal(alone[i][n], r[n]) for n in r)
+
+
+def test_one_tensor_in_every_place():
+    """The same leaf as query, key and value: its gradient is the sum of the three."""
+    x = torch.randn(2, 30, 4, 32, device="cuda", generator=torch.Generator("cuda").manual_seed(4))
+    do = torch.randn_like(x)
+    parts = run(x, x, x, None, None, do)
+    one = x.clone().requires_grad_()
+    got, = torch.autograd.grad(_ops().cross_attention(one, one, one), (one,), do)
+    want = parts["dq"].double() + parts["dk"].double() + parts["dv"].double()
+    assert bool(((got.double() - want).abs() <= 2 * E24 * (parts["dq"].abs() + parts["dk"].abs() + parts["dv"].abs()).double()).all())      # two additions, each rounded once
