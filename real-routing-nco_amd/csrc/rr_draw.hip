@@ -15,8 +15,9 @@
 // leave open (one ballot a register and step); what it keeps, where it fits one register a lane, moves together, in index order, so that
 // only kept keys pay for their 64-bit weight.  Longer rows: a workgroup a row, its keys in registers up to 16 384: a histogram over the
 // distance from the maximum, then only the keys of the bin that holds the border are looked at.  Masses there are 64-bit whole numbers of steps
-// of 2^-45, so that atomics may add them in any order.  Few rows beyond that: a workgroup for every 16 384 keys, five launches (below).
-// Bound by the 64-bit arithmetic (some 20 instructions a weight), not by the one read of the logits.
+// of 2^-45, so that atomics may add them in any order.  Longer rows: a workgroup for every 16 384 keys, five launches (below).
+// Bound by the 64-bit arithmetic (some 20 instructions a weight), not by the one read of the logits: 51 200 x 100 float32 with a mask 17 us (1.5 TB/s), 4 096 x 1 001 with all
+// filters 22 us, 64 x 131 072 bf16 with settings of each row 69 us in five launches (6 + 16 + 5 + 13 + 28).
 #include "rr_types.h"
 
 namespace {
@@ -1169,11 +1170,18 @@ __global__ __launch_bounds__(RR_DRAW_NT) void k_draw_gather(Draw a, Long l) {
 }
 
 // ------------------------------------------------------------------------------------------------ host
-// long rows that are too few to give each CU one go by stretches, where the row does not fit one workgroup's registers
-bool by_stretches(long long R, int V) { return V > 16384 && R <= 1024; }
+// rows that do not fit one workgroup's registers go by stretches, a workgroup each (4 096 x 131 072 float32, top-k and top-p: 1 580 us, 2 710 with a workgroup a row; 64 x 131 072:
+// 45 and 133); a workgroup a row is quicker only where the rows just fill the chip and are hardly longer (256 x 20 000: 46 us against 55)
+bool by_stretches(long long R, int V) { return V > 16384 && !(R >= 128 && R <= 512 && V <= 32768); }
 int stretches(int V) { return (V + RR_DRAW_STRETCH - 1) / RR_DRAW_STRETCH; }
+// rows of one pass over the five launches: what the workspace holds (some 65 KB a row), and fewer than 2^32 threads
+int rows_at_once(int V) {
+  const int most = (1 << 21) / stretches(V);
+  return most < 4096 ? most : 4096;
+}
 size_t long_bytes(long long R, int V) {
   const size_t C = (size_t)stretches(V);
+  R = R < rows_at_once(V) ? R : rows_at_once(V);
   return (size_t)R * (C * 8 + RR_DRAW_BINS * 8 + 16 + C * 8 + RR_DRAW_BINS * 4 + RR_DRAW_LIST * 8 + 24);
 }
 
@@ -1235,7 +1243,7 @@ int draw_go(const Draw& a, bool stretches, void* ws, hipStream_t st) {
     else hipLaunchKernelGGL((k_draw_group<T, 8, false>), wg16, dim3(256), 0, st, a);
     return rr_check(hipGetLastError());
   }
-  // up to 1 024 keys a wave a row (16 registers of keys a lane)
+  // up to 1 024 keys a wave a row (16 registers of keys a lane; 4 096 x 1 024 float32: 14 us, 20 with top-k and top-p; a workgroup a row: 19 and 49)
   if (a.V <= 64) hipLaunchKernelGGL((k_draw_wave<T, 1>), wg, dim3(256), 0, st, a);
   else if (a.V <= 128) hipLaunchKernelGGL((k_draw_wave<T, 2>), wg, dim3(256), 0, st, a);
   else if (a.V <= 256) hipLaunchKernelGGL((k_draw_wave<T, 4>), wg, dim3(256), 0, st, a);
@@ -1263,7 +1271,7 @@ extern "C" int rr_draw(int dtype, const void* logits, long long ld, const uint8_
   const Draw a = {logits, mask, uniforms, index, logp, row_temperature, row_top_p, row_min_p, row_top_k, temperature, 1.44269504088896340736 / temperature, top_p, min_p, ld, ldm,
                   top_k, R, V};
   // a launch holds fewer than 2^32 threads: at most 64 a row up to 1 024 keys, at most 1 024 beyond
-  const int most = V <= 1024 ? 1 << 25 : 1 << 21, size = dtype == RR_F32 ? 4 : 2;
+  const int most = by_stretches(R, V) ? rows_at_once(V) : V <= 1024 ? 1 << 25 : 1 << 21, size = dtype == RR_F32 ? 4 : 2;
   for (long long r = 0; r < R; r += most) {
     Draw b = a;
     b.R = (int)(R - r < most ? R - r : most);

@@ -247,3 +247,12 @@ def test_calls_on_two_streams_at_once():
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(a, b) for r in got[i] for a, b in zip(alone[i], r))
+
+
+@pytest.mark.parametrize("R,V", [(300, 16400), (300, 32768), (513, 20001), (4100, 16500)])
+def test_long_rows_in_every_number(R, V):
+    """A workgroup a row and stretches of a row, and more rows than one pass over the stretches takes."""
+    x, u, mask = make(torch.bfloat16, R, V, seed=V, masked=0.1)
+    rows = [0, 1, 2, R // 2, R - 5, R - 4, R - 3, R - 1]
+    for s in (dict(), dict(k=40, p=0.9, mp=0.01), dict(p=0.95, t=1.4)):
+        check(x, u, mask=mask, rows=rows, **s)

@@ -121,7 +121,8 @@ def test_workspace_sizes():
     assert lib.rr_cross_attn_workspace(2, 64, 1000, 100, 8, 1, 64, 0) == 0                          # enough workgroups: no splits
     n = lib.rr_cross_attn_workspace(2, 1, 1, 100000, 1, 4, 128, 0)                                  # one token on long states: split
     assert n > 0 and n % (4 * 4 * 132) == 0
-    assert lib.rr_draw_workspace(100, 1000) == 0 and lib.rr_draw_workspace(4, 100000) > 0 and lib.rr_draw_workspace(5000, 100000) == 0
+    assert lib.rr_draw_workspace(100, 1000) == 0 and lib.rr_draw_workspace(4, 100000) > 0 and lib.rr_draw_workspace(256, 20000) == 0
+    assert lib.rr_draw_workspace(5000, 100000) == lib.rr_draw_workspace(4096, 100000) > lib.rr_draw_workspace(4095, 100000)      # passes of 4 096 rows
 
 
 def test_norm_and_draw_entries_refuse():
