@@ -18,5 +18,5 @@ def add_rms_norm_fp8(x, residual=None, weight=None, eps: float = 1e-5):
     """add_rms_norm with y handed on in 8 bits: -> (q, scale, h), y ~ q * scale of its group.
 
     q [..., E] float8_e4m3fn; scale [..., ceil(E / 128)] float32, one for every 128 columns (the last group may be shorter): the group's
-    largest |y| / 448, or 1 where the group is all zeros.  Inference only: refused where a gradient would be asked for."""
+    largest |y| / 448 (2^-126 at the least), or 1 where the group is all zeros.  Inference only: refused where a gradient would be asked for."""
     return (L._native or L.native()).add_rms_norm_fp8(x, residual, weight, eps)
