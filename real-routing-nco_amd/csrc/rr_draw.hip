@@ -14,10 +14,13 @@
 // Up to 1 024 keys: a wave a row, its keys in registers.  The k-th largest by bisection over the bit patterns that the row's extremes
 // leave open (one ballot a register and step); what it keeps, where it fits one register a lane, moves together, in index order, so that
 // only kept keys pay for their 64-bit weight.  Longer rows: a workgroup a row, its keys in registers up to 16 384: a histogram over the
-// distance from the maximum, then only the keys of the bin that holds the border are looked at.  Masses there are 64-bit whole numbers of steps
-// of 2^-45, so that atomics may add them in any order.  Longer rows: a workgroup for every 16 384 keys, five launches (below).
+// distance from the maximum, then only the keys of the bin that holds the border are looked at.  Masses there are whole numbers of steps
+// of 2^-45, so that atomics may add them in any order; sums over more than 2^18 keys may pass 64 bits and are kept in 128.  Longer rows: a workgroup for every 16 384 keys, five
+// launches (below).
 // Bound by the 64-bit arithmetic (some 20 instructions a weight), not by the one read of the logits: 51 200 x 100 float32 with a mask 17 us (1.5 TB/s), 4 096 x 1 001 with all
 // filters 22 us, 64 x 131 072 bf16 with settings of each row 69 us in five launches (6 + 16 + 5 + 13 + 28).
+#include <type_traits>
+
 #include "rr_types.h"
 
 namespace {
@@ -139,6 +142,28 @@ __device__ __forceinline__ unsigned long long wave_total(unsigned long long v) {
 #undef RR_ADD
   return (unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
+typedef unsigned __int128 rr_u128;
+__device__ __forceinline__ unsigned long long hi_of(rr_u128 v) { return (unsigned long long)(v >> 64); }
+__device__ __forceinline__ rr_u128 wave_total(rr_u128 v) {
+#define RR_WORD(W, CTRL, ROWS) (rr_u128)(uint32_t)RR_DPP((uint32_t)(v >> (32 * W)), 0, CTRL, ROWS) << (32 * W)
+#define RR_ADD(CTRL, ROWS) v += RR_WORD(3, CTRL, ROWS) | RR_WORD(2, CTRL, ROWS) | RR_WORD(1, CTRL, ROWS) | RR_WORD(0, CTRL, ROWS)
+  RR_ADD(0x111, 0xf); RR_ADD(0x112, 0xf); RR_ADD(0x114, 0xf); RR_ADD(0x118, 0xf); RR_ADD(0x142, 0xa); RR_ADD(0x143, 0xc);
+#undef RR_ADD
+#undef RR_WORD
+  rr_u128 t = 0;
+#pragma unroll
+  for (int w = 3; w >= 0; --w) t = t << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> (32 * w)), 63);
+  return t;
+}
+// sums as 64-bit floats: never falling in the sum, which is all that the comparisons with a limit need
+__device__ __forceinline__ double float_of(uint32_t v) { return (double)v; }
+__device__ __forceinline__ double float_of(unsigned long long v) { return (double)v; }
+__device__ __forceinline__ double float_of(rr_u128 v) { return (double)hi_of(v) * 18446744073709551616.0 + (double)(unsigned long long)v; }
+template <typename V>
+__device__ __forceinline__ V lanes_up(V v, int o) {
+  if constexpr (sizeof(V) == 16) return (rr_u128)__shfl_up(hi_of(v), o) << 64 | __shfl_up((unsigned long long)v, o);
+  else return __shfl_up(v, o);
+}
 __device__ __forceinline__ void wave_lds() {                             // LDS written by a lane of this wave may be read by another from here on
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
@@ -184,7 +209,7 @@ __device__ __forceinline__ uint32_t kth_largest(const uint32_t (&key)[E], int k,
 // The threshold of top-p among a wave's keys and weights: the smallest value with less than `lim` of mass strictly above it, `above` of which is
 // outside these keys (all larger).  Weights of 64-bit floats or of whole steps.
 template <int E, typename W>
-__device__ __forceinline__ uint32_t mass_threshold(const uint32_t (&key)[E], const W (&w)[E], uint32_t top, W above, double lim, uint32_t* skey, W* sw, int lane) {
+__device__ __forceinline__ uint32_t mass_threshold(const uint32_t (&key)[E], const W (&w)[E], uint32_t top, double above, double lim, uint32_t* skey, W* sw, int lane) {
   uint32_t low = top;
 #pragma unroll
   for (int e = 0; e < E; ++e) low = key[e] && key[e] < low ? key[e] : low;
@@ -195,8 +220,7 @@ __device__ __forceinline__ uint32_t mass_threshold(const uint32_t (&key)[E], con
     int n = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) m += key[e] > mid ? w[e] : W(0);
-    m = above + wave_total(m);
-    if ((double)m < lim) hi = mid; else lo = mid + 1u;
+    if (above + (double)wave_total(m) < lim) hi = mid; else lo = mid + 1u;
     // one value between the ends: the next key from lo on is the threshold
 #pragma unroll
     for (int e = 0; e < E; ++e) n += __popcll(__ballot(key[e] >= lo && key[e] <= hi));
@@ -218,7 +242,7 @@ __device__ __forceinline__ uint32_t mass_threshold(const uint32_t (&key)[E], con
         const uint32_t k1[1] = {lane < n ? skey[lane] : 0u};
         const W w1[1] = {lane < n ? sw[lane] : W(0)};
         wave_lds();
-        return mass_threshold<1, W>(k1, w1, wave_max_u(k1[0]), above + wave_total(over), lim, skey, sw, lane);
+        return mass_threshold<1, W>(k1, w1, wave_max_u(k1[0]), above + (double)wave_total(over), lim, skey, sw, lane);
       }
     }
   }
@@ -501,30 +525,30 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {
   return t;
 }
 
-// the first bin, from the top, at which the running sum of h reaches `need` (> 0): its number and the sum before it (RR_DRAW_BINS where it is never reached)
-template <int NT, typename V>
-__device__ __forceinline__ void find_bin(const V* h, double need, V* red, int* found, V* above) {
+// the first bin, from the top, at which the running sum of the bins' h reaches `need` (> 0), the last one if none before it does: its number and the sum before it
+template <int NT, typename V, typename H>
+__device__ __forceinline__ void find_bin(H h, double need, V* red, int* found, V* above) {
   constexpr int PER = RR_DRAW_BINS / NT;
   static_assert(PER >= 1, "a bin for each thread");
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b0 = threadIdx.x * PER;
   V mine = 0;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) mine += h[b0 + i];
+  for (int i = 0; i < PER; ++i) mine += h(b0 + i);
   V run = mine;                                                          // inclusive over the wave
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const V x = __shfl_up(run, o);
+    const V x = lanes_up(run, o);
     if (lane >= o) run += x;
   }
   __syncthreads();
   if (lane == 63) red[wave] = run;
-  if (threadIdx.x == 0) *found = RR_DRAW_BINS;
+  if (threadIdx.x == 0) *found = RR_DRAW_BINS - 1;
   __syncthreads();
   V base = run - mine;
   for (int i = 0; i < wave; ++i) base += red[i];
   for (int i = 0; i < PER; ++i) {
-    const V next = base + h[b0 + i];
-    if ((double)base < need && (double)next >= need) { *found = b0 + i; *above = base; }      // one thread at the most: sums do not fall
+    const V next = base + h(b0 + i);
+    if (float_of(base) < need && (float_of(next) >= need || b0 + i == RR_DRAW_BINS - 1)) { *found = b0 + i; *above = base; }      // one thread at the most: sums do not fall
     base = next;
   }
   __syncthreads();
@@ -621,10 +645,15 @@ __device__ __forceinline__ void locate(const Draw& a, const Par& q, int r, const
   a.logp[r] = (float)(z_of(kk, kept.top, q.c2) - log_of(total));
 }
 
-// The thresholds of a row.  WALK(f) calls f(key) for all keys of the row, each by one thread of the workgroup.
-template <int NT, typename WALK, typename S>
+// The thresholds of a row.  WALK(f) calls f(key) for all keys of the row, each by one thread of the workgroup.  WIDE: sums of masses over the row may pass
+// 64 bits; a bin of the histogram is then two words, of the lower 39 bits (2^24 keys: 63 bits) and of the upper 6 of each weight
+template <int NT, bool WIDE, typename WALK, typename S>
 __device__ __forceinline__ uint32_t thresholds(const Draw& a, const Par& q, uint32_t top, uint32_t all, WALK walk, S& sh) {
+  typedef std::conditional_t<WIDE, rr_u128, unsigned long long> M;
   constexpr int LIST = S::LISTED;
+  M *red, *above_m;
+  if constexpr (WIDE) { red = sh.redw; above_m = &sh.above_w; }
+  else { red = sh.redm; above_m = &sh.above_m; }
   const int lane = threadIdx.x & 63;
   const double topd = (double)value_of(top);
   const float topv = value_of(top), per = (float)(22.180709777918249 * q.c2);      // 32 / T
@@ -660,7 +689,7 @@ __device__ __forceinline__ uint32_t thresholds(const Draw& a, const Par& q, uint
     __syncthreads();
     walk([&](uint32_t k) { if (k) atomicAdd(&sh.cnt[bin_of(k, topv, per)], 1u); });
     __syncthreads();
-    find_bin<NT>(sh.cnt, (double)q.k, sh.redu, &sh.found, &sh.above_c);
+    find_bin<NT>([&](int b) { return sh.cnt[b]; }, (double)q.k, sh.redu, &sh.found, &sh.above_c);
     const int bin = sh.found;
     const uint32_t need = (uint32_t)q.k - sh.above_c;                    // the need-th largest of the bin
     const int n = gather(bin, 1u);
@@ -688,21 +717,32 @@ __device__ __forceinline__ uint32_t thresholds(const Draw& a, const Par& q, uint
     }
   }
   if (q.p > 0.0 && q.p < 1.0) {
-    for (int i = threadIdx.x; i < RR_DRAW_BINS; i += NT) sh.mass[i] = 0ull;
+    for (int i = threadIdx.x; i < RR_DRAW_BINS; i += NT) {
+      sh.mass[i] = 0ull;
+      if constexpr (WIDE) sh.cnt[i] = 0u;
+    }
     __syncthreads();
-    unsigned long long m = 0ull;
+    unsigned long long m = 0ull;                                         // (a thread's part of 2^24 keys: under 2^60)
     walk([&](uint32_t k) {
       if (k >= cut) {
         const unsigned long long w = steps_of(weight_of(k, top, topd, q.c2));
         m += w;
-        if (w) atomicAdd(&sh.mass[bin_of(k, topv, per)], w);
+        if constexpr (WIDE) {
+          const int b = bin_of(k, topv, per);
+          if (w & 0x7fffffffffull) atomicAdd(&sh.mass[b], w & 0x7fffffffffull);
+          if (w >> 39) atomicAdd(&sh.cnt[b], (uint32_t)(w >> 39));
+        } else if (w) {
+          atomicAdd(&sh.mass[bin_of(k, topv, per)], w);
+        }
       }
     });
-    m = block_sum<NT>(m, sh.redm);                                       // (its barriers stand between the histogram's writes and reads)
-    const double lim = q.p * (double)m;
-    find_bin<NT>(sh.mass, lim, sh.redm, &sh.found, &sh.above_m);
+    const double lim = q.p * float_of(block_sum<NT>((M)m, red));         // (its barriers stand between the histogram's writes and reads)
+    find_bin<NT>([&](int b) {
+      if constexpr (WIDE) return ((rr_u128)sh.cnt[b] << 39) + sh.mass[b];
+      else return sh.mass[b];
+    }, lim, red, &sh.found, above_m);
     const int bin = sh.found;
-    const unsigned long long before = sh.above_m;
+    const double before = float_of(*above_m);
     const int n = gather(bin, cut);
     if (n <= 256) {
       if (threadIdx.x < 64) {
@@ -726,8 +766,7 @@ __device__ __forceinline__ uint32_t thresholds(const Draw& a, const Par& q, uint
         const uint32_t mid = lo + ((hi - lo) >> 1);
         unsigned long long s = 0ull;
         each(n, bin, cut, [&](uint32_t k) { if (k > mid) s += steps_of(weight_of(k, top, topd, q.c2)); });
-        s = before + block_sum<NT>(s, sh.redm);
-        if ((double)s < lim) hi = mid; else lo = mid + 1u;
+        if (before + float_of(block_sum<NT>((M)s, red)) < lim) hi = mid; else lo = mid + 1u;
       }
       cut = lo;
     }
@@ -735,8 +774,8 @@ __device__ __forceinline__ uint32_t thresholds(const Draw& a, const Par& q, uint
   return cut;
 }
 
-// A row of any length by one workgroup.  ONE: the row's keys fit its registers; else stretch after stretch is loaded again for every walk
-template <typename T, int NT, int E, bool ONE, typename S>
+// A row of any length by one workgroup.  ONE: the row's keys fit its registers; else stretch after stretch is loaded again for every walk.  WIDE: it may hold more than 2^18 keys
+template <typename T, int NT, int E, bool ONE, bool WIDE, typename S>
 __device__ __forceinline__ void draw_row(const Draw& a, int r, S& sh) {
   using K = Keys<T, NT, E>;
   const T* row = (const T*)a.logits + (long long)r * a.ld;
@@ -764,7 +803,7 @@ __device__ __forceinline__ void draw_row(const Draw& a, int r, S& sh) {
     return;
   }
   if (q.k > 0 && q.k < a.V) n = block_sum<NT>(n, sh.redu);
-  const uint32_t cut = thresholds<NT>(a, q, top, n, [&](auto f) { walk_at([&](uint32_t k, int) { f(k); }); }, sh);
+  const uint32_t cut = thresholds<NT, WIDE>(a, q, top, n, [&](auto f) { walk_at([&](uint32_t k, int) { f(k); }); }, sh);
   const Kept kept = {top, cut, (double)value_of(top), q.c2, q.mp};
   if constexpr (ONE) {
     locate(a, q, r, ks, kept, 0.0, -1.0, sh);
@@ -793,7 +832,7 @@ __device__ __forceinline__ void draw_row(const Draw& a, int r, S& sh) {
 template <typename T, int NT, int E, bool ONE>
 __global__ __launch_bounds__(NT) void k_draw_row(Draw a) {
   __shared__ Scratch<NT, 1024> sh;
-  draw_row<T, NT, E, ONE>(a, blockIdx.x, sh);
+  draw_row<T, NT, E, ONE, false>(a, blockIdx.x, sh);
 }
 
 // ---- few long rows: every stretch of a row has its own workgroup, five launches
@@ -808,10 +847,11 @@ __global__ __launch_bounds__(NT) void k_draw_row(Draw a) {
 struct Long {
   uint32_t *tops, *counts;             // [R][C]
   double* masses;                      // [R][C]
-  unsigned long long* mass;            // [R][bins]
+  unsigned long long* mass;            // [R][bins] the lower 52 bits of the stretches' masses (at most 2^59 each, 1 024 of them) ...
+  uint32_t* high;                      // [R][bins] ... and what is above
   uint32_t* cnt;                       // [R][bins]
   uint32_t *list, *where;              // [R][RR_DRAW_LIST]
-  unsigned long long *whole, *above;   // [R] the row's mass, that above the border's bin
+  double *whole, *above;               // [R] the row's mass in steps, that above the border's bin
   uint32_t *top, *n;                   // [R]
   int *nlist, *mode, *bin, *greedy;      // [R]
   int C;
@@ -819,6 +859,7 @@ struct Long {
 enum { RR_NOTHING = 0, RR_LIST_ALL = 1, RR_LIST_BORDER = 2, RR_ALONE = 3, RR_UNFILTERED = 4, RR_GREEDY = 5 };
 struct LongScratch : Scratch<RR_DRAW_NT, RR_DRAW_LIST> {
   uint32_t where[RR_DRAW_LIST];
+  rr_u128 redw[RR_DRAW_NT / 64], above_w;
 };
 
 __device__ __forceinline__ bool by_count(const Par& q, uint32_t n) { return q.k > 0 && n > (uint32_t)q.k; }
@@ -844,6 +885,7 @@ __global__ __launch_bounds__(RR_DRAW_NT) void k_draw_top(Draw a, Long l) {
   if (c == 0) {
     l.cnt[(long long)r * RR_DRAW_BINS + threadIdx.x] = 0u;
     l.mass[(long long)r * RR_DRAW_BINS + threadIdx.x] = 0ull;
+    l.high[(long long)r * RR_DRAW_BINS + threadIdx.x] = 0u;
     if (threadIdx.x == 0) { l.nlist[r] = 0; l.greedy[r] = 0x7fffffff; }
   }
 }
@@ -901,12 +943,16 @@ __global__ __launch_bounds__(RR_DRAW_NT) void k_draw_measure(Draw a, Long l) {
   __syncthreads();
   const long long at = (long long)r * RR_DRAW_BINS + threadIdx.x;
   if (sh.cnt[threadIdx.x]) atomicAdd(&l.cnt[at], sh.cnt[threadIdx.x]);
-  if (sh.mass[threadIdx.x]) atomicAdd(&l.mass[at], sh.mass[threadIdx.x]);
+  const unsigned long long m = sh.mass[threadIdx.x];
+  if (m) atomicAdd(&l.mass[at], m & 0xfffffffffffffull);
+  if (m >> 52) atomicAdd(&l.high[at], (uint32_t)(m >> 52));
 }
 
 // a workgroup a row: the bin of the border, and how the row goes on
 __global__ __launch_bounds__(RR_DRAW_NT) void k_draw_border(Draw a, Long l) {
-  __shared__ Scratch<RR_DRAW_NT, 64> sh;
+  __shared__ uint32_t cnt[RR_DRAW_BINS], redu[RR_DRAW_NT / 64], above_c;
+  __shared__ rr_u128 redw[RR_DRAW_NT / 64], above_w;
+  __shared__ int found;
   constexpr int NT = RR_DRAW_NT;
   const int r = blockIdx.x;
   const uint32_t n = l.n[r];
@@ -915,20 +961,19 @@ __global__ __launch_bounds__(RR_DRAW_NT) void k_draw_border(Draw a, Long l) {
   const bool counts = by_count(q, n), masses = !counts;
   const long long at = (long long)r * RR_DRAW_BINS + threadIdx.x;
   const uint32_t mine = l.cnt[at];
-  const unsigned long long mym = l.mass[at];
-  sh.cnt[threadIdx.x] = mine;
-  sh.mass[threadIdx.x] = mym;
-  const unsigned long long whole = block_sum<NT>(mym, sh.redm);
-  sh.above_m = 0ull;
-  if (counts) find_bin<NT>(sh.cnt, (double)q.k, sh.redu, &sh.found, &sh.above_c);
-  else find_bin<NT>(sh.mass, q.p * (double)whole, sh.redm, &sh.found, &sh.above_m);
-  const int bin = sh.found;
-  const uint32_t upto = block_sum<NT>((int)threadIdx.x <= bin ? mine : 0u, sh.redu), within = sh.cnt[bin];
+  const rr_u128 mym = ((rr_u128)l.high[at] << 52) + l.mass[at];
+  cnt[threadIdx.x] = mine;
+  if (threadIdx.x == 0) above_w = 0;
+  const double whole = float_of(block_sum<NT>(mym, redw));
+  if (counts) find_bin<NT>([&](int) { return mine; }, (double)q.k, redu, &found, &above_c);      // (a thread's own bin)
+  else find_bin<NT>([&](int) { return mym; }, q.p * whole, redw, &found, &above_w);
+  const int bin = found;
+  const uint32_t upto = block_sum<NT>((int)threadIdx.x <= bin ? mine : 0u, redu), within = cnt[bin];
   if (threadIdx.x == 0) {
     l.mode[r] = upto <= RR_DRAW_LIST ? RR_LIST_ALL : masses && within <= RR_DRAW_LIST ? RR_LIST_BORDER : RR_ALONE;
     l.bin[r] = bin;
     l.whole[r] = whole;
-    l.above[r] = sh.above_m;
+    l.above[r] = float_of(above_w);
   }
 }
 
@@ -980,7 +1025,7 @@ __global__ __launch_bounds__(RR_DRAW_NT) void k_draw_pick(Draw a, Long l) {
     return;
   }
   if (mode == RR_ALONE) {
-    draw_row<T, NT, RR_DRAW_STRETCH / NT, false>(a, r, sh);
+    draw_row<T, NT, RR_DRAW_STRETCH / NT, false, true>(a, r, sh);
     return;
   }
   const double topd = (double)value_of(top);
@@ -1006,7 +1051,7 @@ __global__ __launch_bounds__(RR_DRAW_NT) void k_draw_pick(Draw a, Long l) {
     key[e] = i < cnt ? list[i] : 0u;
     pos[e] = i < cnt ? where[i] : 0xffffffffu;
   }
-  const double whole = counted ? -1.0 : (double)l.whole[r];              // what top-p refers to, in steps
+  const double whole = counted ? -1.0 : l.whole[r];              // what top-p refers to, in steps
   int size = 64;
   while (size < cnt) size <<= 1;                                         // <= RR_DRAW_LIST
   if (mode == RR_LIST_ALL && cnt <= 256) {                               // the first wave, as a short row
@@ -1067,13 +1112,13 @@ __global__ __launch_bounds__(RR_DRAW_NT) void k_draw_pick(Draw a, Long l) {
   uint32_t cut = 1u;
   if (by_mass(q)) {
     const double m = counted ? (double)block_sum<NT>(w[0] + w[1], sh.redm) : whole;
-    const unsigned long long before = mode == RR_LIST_BORDER ? l.above[r] : 0ull;
+    const double before = mode == RR_LIST_BORDER ? l.above[r] : 0.0;
     const double lim = q.p * m;
     extremes(lo, hi);
     for (int step = 0; lo < hi; ++step) {
       const uint32_t mid = between(lo, hi, step);
-      const unsigned long long s = before + block_sum<NT>((key[0] > mid ? w[0] : 0ull) + (key[1] > mid ? w[1] : 0ull), sh.redm);
-      if ((double)s < lim) hi = mid; else lo = mid + 1u;
+      const double s = before + (double)block_sum<NT>((key[0] > mid ? w[0] : 0ull) + (key[1] > mid ? w[1] : 0ull), sh.redm);
+      if (s < lim) hi = mid; else lo = mid + 1u;
     }
     cut = lo;
   }
@@ -1174,7 +1219,7 @@ __global__ __launch_bounds__(RR_DRAW_NT) void k_draw_gather(Draw a, Long l) {
 // 45 and 133); a workgroup a row is quicker only where the rows just fill the chip and are hardly longer (256 x 20 000: 46 us against 55)
 bool by_stretches(long long R, int V) { return V > 16384 && !(R >= 128 && R <= 512 && V <= 32768); }
 int stretches(int V) { return (V + RR_DRAW_STRETCH - 1) / RR_DRAW_STRETCH; }
-// rows of one pass over the five launches: what the workspace holds (some 65 KB a row), and fewer than 2^32 threads
+// rows of one pass over the five launches: what the workspace holds (33 KB a row up to 131 072 keys), and fewer than 2^32 threads
 int rows_at_once(int V) {
   const int most = (1 << 21) / stretches(V);
   return most < 4096 ? most : 4096;
@@ -1182,7 +1227,7 @@ int rows_at_once(int V) {
 size_t long_bytes(long long R, int V) {
   const size_t C = (size_t)stretches(V);
   R = R < rows_at_once(V) ? R : rows_at_once(V);
-  return (size_t)R * (C * 8 + RR_DRAW_BINS * 8 + 16 + C * 8 + RR_DRAW_BINS * 4 + RR_DRAW_LIST * 8 + 24);
+  return (size_t)R * (C * 8 + RR_DRAW_BINS * 8 + 16 + C * 8 + RR_DRAW_BINS * 8 + RR_DRAW_LIST * 8 + 24);
 }
 
 template <typename T>
@@ -1193,10 +1238,11 @@ int draw_long(const Draw& a, void* ws, hipStream_t st) {
   auto take = [&](size_t bytes) { void* at = p; p += bytes; return at; };
   l.masses = (double*)take(R * C * 8);
   l.mass = (unsigned long long*)take(R * RR_DRAW_BINS * 8);
-  l.whole = (unsigned long long*)take(R * 8);
-  l.above = (unsigned long long*)take(R * 8);
+  l.whole = (double*)take(R * 8);
+  l.above = (double*)take(R * 8);
   l.tops = (uint32_t*)take(R * C * 4);
   l.counts = (uint32_t*)take(R * C * 4);
+  l.high = (uint32_t*)take(R * RR_DRAW_BINS * 4);
   l.cnt = (uint32_t*)take(R * RR_DRAW_BINS * 4);
   l.list = (uint32_t*)take(R * RR_DRAW_LIST * 4);
   l.where = (uint32_t*)take(R * RR_DRAW_LIST * 4);

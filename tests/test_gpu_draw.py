@@ -256,3 +256,29 @@ def test_long_rows_in_every_number(R, V):
     rows = [0, 1, 2, R // 2, R - 5, R - 4, R - 3, R - 1]
     for s in (dict(), dict(k=40, p=0.9, mp=0.01), dict(p=0.95, t=1.4)):
         check(x, u, mask=mask, rows=rows, **s)
+
+
+def _wide_row(kind, V, dt, g):
+    if kind == "equal":
+        return torch.zeros(1, V, device="cuda", dtype=dt)
+    if kind == "nearly flat":
+        return (0.01 * torch.randn(1, V, device="cuda", generator=g)).to(dt)
+    x = -1.0 - 19.0 * torch.rand(1, V, device="cuda", generator=g)                 # "two levels": most keys at 0, the others spread below, few to each bin
+    return torch.where(torch.rand(1, V, device="cuda", generator=g) < 0.7, torch.zeros_like(x), x).to(dt)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("V", [1 << 19, (1 << 20) + 3, 1 << 24])
+@pytest.mark.parametrize("kind,p", [("equal", 0.9), ("nearly flat", 0.9), ("two levels", 0.995)])
+def test_weights_that_sum_past_half_a_million(kind, p, V, dt):
+    """Flat rows so wide that their masses pass 64 bits in steps of 2^-45: top-p keeps what the definition keeps, alone and with top-k and min-p.
+    A kept set that is off by n keys moves the log-probability by n / V, and the choice with it; the sums of both sides are exact to 2^-29."""
+    g = torch.Generator("cuda").manual_seed(V)
+    x = _wide_row(kind, V, dt, g)
+    u = torch.rand(1, device="cuda", generator=g)
+    check(x, u, p=p)
+    if V <= 1 << 21:
+        check(x, u, p=p, k=V // 2)
+        check(x, 1 - u, p=p, mp=0.3, t=0.9)
+        mask = torch.rand(1, V, device="cuda", generator=g) < 0.97
+        check(torch.cat([x, -x]), torch.cat([u, 1 - u]), mask=mask, p=p, k=2500)
