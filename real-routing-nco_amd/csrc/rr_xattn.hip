@@ -10,7 +10,7 @@
 // keys: the softmax's rescaling is one factor a lane, and P^T is in the registers exactly as the second product
 // O^T = V^T P^T takes it (the sum over the keys runs in the order that the registers hold, V^T is read with the same order:
 // ds_read_b64_tr_b16 for 16-bit types, four plain reads for float32).  The running maximum and sum are in 32 bits; P is rounded to
-// the inputs' type for the second product (half a step of a weight <= 1, under the rounding of the output).
+// the inputs' type for the second product, half a step of each weight; in float16 a weight keeps that down to 2^-25 of the row's largest (Range below).
 // float32 runs on v_mfma_f32_16x16x4 (exact products), 16-bit types on v_mfma_f32_16x16x32.
 // The backward recomputes P from lse; dq walks over keys, (dk, dv) over rows: no atomics, the same result every time.
 // Products run at a raised wave priority in the forward and dq: with two waves a SIMD one computes weights while the other holds the matrix pipe
@@ -290,6 +290,11 @@ template <bool TIGHT>
 __device__ __forceinline__ void in_order() {
   if constexpr (TIGHT) __builtin_amdgcn_sched_barrier(0);
 }
+// A row's weights are taken relative to 2^(its running maximum - UP), and the running maximum moves only when a score passes it by 2^SLACK: weights up to that are as exact as those up
+// to one, and a tile that does not move it needs no exchange between the lanes of a row and no rescaling.  float16 has 2^15 above one and 2^-14 below: with UP
+// the largest weight stands between 2^11 and 2^15 instead of 1 and 2^8, so that small ones keep their bits (20 000 keys of 1.47 2^-24 beside one of 1 lost a third of their sum)
+template <typename T> struct Range { static constexpr float UP = 0.f, SLACK = 8.f; };
+template <> struct Range<rr_f16> { static constexpr float UP = 11.f, SLACK = 4.f; };
 template <typename T, int DP> struct Waves { static constexpr int N = sizeof(T) == 4 && DP == 128 ? 1 : 2; };
 
 template <typename T, int DP, int QT>
@@ -369,8 +374,6 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_fwd(XAttn a) {
           keep4(s[t][n], b, -INFINITY);
         }
     }
-    // the running maximum moves only when a score passes it by 2^8: weights up to that are as exact as those up to one, and a tile
-    // that does not move it needs no exchange between the lanes of a row and no rescaling
     float mx[QT];
     bool move = false;
 #pragma unroll
@@ -382,12 +385,12 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_fwd(XAttn a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) mx[t] = fmaxf(mx[t], s[t][n][i]);
       }
-      move |= mx[t] * c2 > m[t] + 8.0f;
+      move |= mx[t] * c2 > m[t] + (Range<T>::UP + Range<T>::SLACK);
     }
     if (__any(move)) {
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
-        const float mn = fmaxf(m[t], group_max(mx[t]) * c2);
+        const float mn = fmaxf(m[t], group_max(mx[t]) * c2 - Range<T>::UP);
         const float al = __builtin_amdgcn_exp2f(m[t] - finite_or_zero(mn));
         l[t] *= al;
         m[t] = mn;

@@ -353,3 +353,21 @@ def test_one_tensor_in_every_place():
     got, = torch.autograd.grad(_ops().cross_attention(one, one, one), (one,), do)
     want = parts["dq"].double() + parts["dk"].double() + parts["dv"].double()
     assert bool(((got.double() - want).abs() <= 2 * E24 * (parts["dq"].abs() + parts["dk"].abs() + parts["dv"].abs()).double()).all())      # two additions, each rounded once
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("B", [1, 600])
+@pytest.mark.parametrize("first", [True, False])
+def test_many_small_weights_beside_a_large_one(dt, B, first):
+    """20 000 keys of a weight of 1.47 2^-24 each beside one of weight 1 whose value is zero: the result is the small ones' sum, 1.75e-3.  One sequence: the keys are split over workgroups, 600: they are not.
+    The scores are exact in the type; a weight is rounded by half a step, u, its exponent is off by 2^-24 (16 + 8 + 4) 16.25 < 3e-5, twice that in the weight, and the sums of
+    20 000 equal terms in 32 bits by 2^-24 each, 1.2e-3 at the worst where all go one way, in numerator and quotient; the result is rounded by u again."""
+    n = 20001
+    q = torch.full((B, 1, 1, 16), 0.25, device="cuda", dtype=dt)
+    k = torch.full((1, n, 1, 16), -4.0625, device="cuda", dtype=dt)              # scale 1: scores of -16.25
+    v = torch.ones(1, n, 1, 16, device="cuda", dtype=dt)
+    at = 0 if first else n - 1
+    k[:, at], v[:, at] = 0, 0
+    got = _ops().cross_attention(q, k.expand(B, -1, -1, -1), v.expand(B, -1, -1, -1), scale=1.0).double()
+    w = 20000 * math.exp(-16.25)
+    assert float((got / (w / (1 + w)) - 1).abs().max()) <= 2 * U[dt] + 6e-5 + 2.4e-3
