@@ -12,7 +12,8 @@
 // ds_read_b64_tr_b16 for 16-bit types, four plain reads for float32).  The running maximum and sum are in 32 bits; P is rounded to
 // the inputs' type for the second product, half a step of each weight; in float16 a weight keeps that down to 2^-25 of the row's largest (Range below).
 // float32 runs on v_mfma_f32_16x16x4 (exact products), 16-bit types on v_mfma_f32_16x16x32.
-// The backward recomputes P from lse; dq walks over keys, (dk, dv) over rows: no atomics, the same result every time.
+// The backward recomputes P from lse; dq walks over keys, (dk, dv) over rows: no atomics, the same result every time.  P and ds are rounded to the inputs' type for its second
+// products too; in float16 ds is taken times a power of two, of a row's own in dq and of a key's own in dk, and P times 2^14 in dv (Scaled below).
 // Products run at a raised wave priority in the forward and dq: with two waves a SIMD one computes weights while the other holds the matrix pipe
 // (forward 2 000 x 4 099, 64 heads of 128: 372 -> 360 us, dq of 1 500 x 2 049, 32 heads of 64: 69.4 -> 68.2; dk, dv: nothing).
 // Bounds and figures (float16 / bfloat16 unless said): forward of 2 000 x 4 099, 64 heads of 128, 740 TFLOP/s, matrix pipe 29% and vector pipe 34% busy, the rest
@@ -295,6 +296,18 @@ __device__ __forceinline__ void in_order() {
 // the largest weight stands between 2^11 and 2^15 instead of 1 and 2^8, so that small ones keep their bits (20 000 keys of 1.47 2^-24 beside one of 1 lost a third of their sum)
 template <typename T> struct Range { static constexpr float UP = 0.f, SLACK = 8.f; };
 template <> struct Range<rr_f16> { static constexpr float UP = 11.f, SLACK = 4.f; };
+// float16 in the backward.  ds = p (do.v - delta) may be of any size: a mean loss over long states leaves 1e-7 and less, large gradients on few keys pass 65 504 though dq and dk fit.  The
+// second products take ds 2^n, n of a row's (a key's) own, undone in 32 bits at the end.  n begins at 60 and falls, the sums with it, whenever a value would pass 2^15: to where the largest
+// of the step stands at 2^9 .. 2^10, so that it rarely falls again.  Then the rounding of a small ds is off by 2^-34 of the row's (key's) largest at the most.  P <= 1 is taken times
+// 2^14: off by 2^-39 at the most.  It costs a comparison and a branch for
+// every 32 keys (rows) of a row (key) and dk a product for each weight: 2 x 1 500 on 2 049, 16 / 4 heads of 64, every key seen, dq 69 -> 77 us, (dk, dv) 122 -> 142, 120 on 60, 2 048 heads of 64:
+// 52 -> 57 and 35 -> 38; bfloat16, which has float32's exponents, does without
+#define RR_XA_UP 0x1p60f
+#define RR_XA_P_BITS 14
+template <typename T> struct Scaled { static constexpr bool v = std::is_same_v<T, rr_f16>; };
+__device__ __forceinline__ float abs4(float mx, const f32x4& x) { return fmaxf(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))), mx); }
+// the power of two that a largest value of `mx` asks for, 1 where it needs none (or is not finite: the sums are then, too)
+__device__ __forceinline__ float fall_by(float mx) { return mx > 32768.f && mx < INFINITY ? ldexpf(1.f, 10 - __builtin_amdgcn_frexp_expf(mx)) : 1.f; }
 template <typename T, int DP> struct Waves { static constexpr int N = sizeof(T) == 4 && DP == 128 ? 1 : 2; };
 
 template <typename T, int DP, int QT>
@@ -621,11 +634,12 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_dq(XAttn a) {
   }
   const float c2 = a.scale * RR_LOG2E;
   f32x4 o[QT][Dm::DT];
+  float up[QT];
   // keys behind the last one are staged as zeros: whatever their weight, they add nothing (unless it overflows, which the second walk sorts out)
   auto tile = [&](auto safe, int k0, int at) {
     const T *tk = sk[at], *tv = sv[at];
     const uint32_t* fl = flag[at];
-    const bool some = a.mask != nullptr || safe();      // (uniform) not every pair of the tile may be seen
+    const bool some = a.mask != nullptr || safe() || (Scaled<T>::v && k0 + RR_XA_KT > seen);      // (uniform) not every pair of the tile may be seen
     uint32_t mb[QT][4];
     if (a.mask != nullptr) {
 #pragma unroll
@@ -674,12 +688,13 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_dq(XAttn a) {
       typename M::Frag pf[QT];
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
+        const float ud = Scaled<T>::v ? delta[t] * up[t] : delta[t];
 #pragma unroll
         for (int u = 0; u < M::PT; ++u)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float p = __builtin_amdgcn_exp2f(fmaf(s[t][u][i], c2, -lse2[t]));
-            s[t][u][i] = p * (dp[t][u][i] - delta[t]);
+            s[t][u][i] = p * (Scaled<T>::v ? fmaf(dp[t][u][i], up[t], -ud) : dp[t][u][i] - ud);
           }
         if (some) {
 #pragma unroll
@@ -687,6 +702,17 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_dq(XAttn a) {
             const int key = 16 * (n + u) + 4 * g;
             if constexpr (safe()) keep4(s[t][u], ~(flag4(fl, key) * 0xffu), __builtin_nanf(""));      // a visible key that holds a non-finite value
             keep4(s[t][u], first_bytes(a.mask != nullptr ? mb[t][n + u] : 0x01010101u, seen - (k0 + key)), 0.f);
+          }
+        }
+        if constexpr (Scaled<T>::v) {
+          const float mx = abs4(abs4(0.f, s[t][0]), s[t][M::PT - 1]);
+          if (__any(mx > 32768.f)) {
+            const float r = fall_by(group_max(mx));
+            up[t] *= r;
+#pragma unroll
+            for (int u = 0; u < M::PT; ++u) s[t][u] *= r;
+#pragma unroll
+            for (int d = 0; d < Dm::DT; ++d) o[t][d] *= r;
           }
         }
         pf[t] = M::pack(s[t]);
@@ -716,9 +742,11 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_dq(XAttn a) {
   };
   auto walk = [&](auto safe) {
 #pragma unroll
-    for (int t = 0; t < QT; ++t)
+    for (int t = 0; t < QT; ++t) {
+      up[t] = RR_XA_UP;
 #pragma unroll
       for (int d = 0; d < Dm::DT; ++d) o[t][d] = rr_zero4();
+    }
     if constexpr (safe()) {
       clear_flag(flag[0]);
       pk.load(krow(first), a.kl, seen - first, a.D);
@@ -774,7 +802,7 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_dq(XAttn a) {
     for (int d = 0; d < Dm::DT; ++d) {
       const int c = 16 * d + 4 * g;
       if (c >= a.D) continue;
-      const f32x4 x = o[t][d] * a.scale;
+      const f32x4 x = (Scaled<T>::v ? o[t][d] * (1.f / up[t]) : o[t][d]) * a.scale;
       if (a.nsplit > 1) {
         *reinterpret_cast<f32x4*>(p + c) = x;
       } else {
@@ -826,7 +854,7 @@ __global__ __launch_bounds__(256, (DP == 128 ? 1 : 2)) void k_xattn_dkv(XAttn a)
     pg.load(gp + h * a.gh + s0 * a.gl, a.gl, rows, a.D);
     if (threadIdx.x < RR_XA_KT) {
       const long long li = ((long long)w.b * H + head) * a.Lq + s0 + ((int)threadIdx.x < rows ? (int)threadIdx.x : rows - 1);
-      nl = (int)threadIdx.x < rows ? a.lse[li] * RR_LOG2E : INFINITY;
+      nl = (int)threadIdx.x < rows ? a.lse[li] * RR_LOG2E - (Scaled<T>::v ? RR_XA_P_BITS : 0) : INFINITY;
       nd = (int)threadIdx.x < rows ? a.delta[li] : 0.f;
     }
     if (a.mask != nullptr) {
@@ -870,6 +898,7 @@ __global__ __launch_bounds__(256, (DP == 128 ? 1 : 2)) void k_xattn_dkv(XAttn a)
     }
   }
   f32x4 ok[KW][Dm::DT], ov[KW][Dm::DT];
+  float up[KW];                                                          // ds is collected times up 2^14
   // one staged tile of rows.  Rows behind the last one are zeros with an lse of infinity: their weights are zero.  Keys behind the last one hold zeros; what
   // they collect is not written
   auto tile = [&](auto safe, int rows, int at) {
@@ -907,7 +936,7 @@ __global__ __launch_bounds__(256, (DP == 128 ? 1 : 2)) void k_xattn_dkv(XAttn a)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float p = __builtin_amdgcn_exp2f(fmaf(s[t][u][i], c2, -ls[u][i]));
-            dp[t][u][i] = p * (dp[t][u][i] - de[u][i]);
+            dp[t][u][i] = p * (Scaled<T>::v ? (dp[t][u][i] - de[u][i]) * up[t] : dp[t][u][i] - de[u][i]);
             s[t][u][i] = p;
           }
         if (some) {
@@ -927,6 +956,17 @@ __global__ __launch_bounds__(256, (DP == 128 ? 1 : 2)) void k_xattn_dkv(XAttn a)
           }
         }
         pf[t] = M::pack(s[t]);
+        if constexpr (Scaled<T>::v) {
+          const float mx = abs4(abs4(0.f, dp[t][0]), dp[t][M::PT - 1]);
+          if (__any(mx > 32768.f && key0 + 16 * t + j < seen)) {
+            const float r = fall_by(group_max(mx));
+            up[t] *= r;
+#pragma unroll
+            for (int u = 0; u < M::PT; ++u) dp[t][u] *= r;
+#pragma unroll
+            for (int d = 0; d < Dm::DT; ++d) ok[t][d] *= r;
+          }
+        }
         df[t] = M::pack(dp[t]);
       }
 #pragma unroll
@@ -941,9 +981,11 @@ __global__ __launch_bounds__(256, (DP == 128 ? 1 : 2)) void k_xattn_dkv(XAttn a)
   };
   auto walk = [&](auto safe) {
 #pragma unroll
-    for (int t = 0; t < KW; ++t)
+    for (int t = 0; t < KW; ++t) {
+      up[t] = RR_XA_UP / (1 << RR_XA_P_BITS);
 #pragma unroll
       for (int d = 0; d < Dm::DT; ++d) { ok[t][d] = rr_zero4(); ov[t][d] = rr_zero4(); }
+    }
     if constexpr (safe()) {
       clear_flag(flag[0]);
       load_tile(first);
@@ -982,7 +1024,8 @@ __global__ __launch_bounds__(256, (DP == 128 ? 1 : 2)) void k_xattn_dkv(XAttn a)
     for (int d = 0; d < Dm::DT; ++d) {
       const int c = 16 * d + 4 * g;
       if (c >= a.D) continue;
-      const f32x4 zero = rr_zero4(), xk = key < seen ? ok[t][d] * a.scale : zero, xv = key < seen ? ov[t][d] : zero;
+      const float down = Scaled<T>::v ? 1.f / (1 << RR_XA_P_BITS) : 1.f;
+      const f32x4 zero = rr_zero4(), xk = key < seen ? (Scaled<T>::v ? ok[t][d] * (down / up[t]) : ok[t][d]) * a.scale : zero, xv = key < seen ? ov[t][d] * down : zero;
       if (a.nsplit > 1) {
         *reinterpret_cast<f32x4*>(p + c) = xk;
         *reinterpret_cast<f32x4*>(p + half + c) = xv;

@@ -371,3 +371,36 @@ def test_many_small_weights_beside_a_large_one(dt, B, first):
     got = _ops().cross_attention(q, k.expand(B, -1, -1, -1), v.expand(B, -1, -1, -1), scale=1.0).double()
     w = 20000 * math.exp(-16.25)
     assert float((got / (w / (1 + w)) - 1).abs().max()) <= 2 * U[dt] + 6e-5 + 2.4e-3
+
+
+def _by_norm(name, got, want, u):
+    """|got - want| in the norm: the second operand's rounding and the result's, half a step u of each at the most and with no common sign, and half of the smallest step where the result lies
+    below the type's normal numbers.  Everything else (sums in 32 bits, exponents) is under a hundredth of u."""
+    floor = 2.0 ** -25 if u == 2.0 ** -11 else 0.0
+    g = got.double()
+    assert bool(torch.isfinite(g).all()), name
+    err, lim = float((g - want).norm()), 2 * u * float(want.norm()) + floor * want.numel() ** 0.5
+    assert err <= lim, f"{name}: {err / float(want.norm()):.3g} of its norm, {err / lim:.3g} x the tolerance"
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("lq,lk,d,fq,fk,fv,fd", [
+    (64, 4099, 128, 2.0 ** -6, 16.0, 1.0, 1e-3), (300, 4099, 64, 16.0, 2.0 ** -6, 1.0, 1e-3), (40, 32768, 64, 2.0 ** -6, 16.0, 1.0, 1e-2), (64, 131072, 64, 1.0, 2.0 ** -6, 1.0, 8.0),
+    (70, 300, 32, 1.0, 1.0, 1.0, 1e-4), (1, 5000, 64, 2.0 ** -6, 16.0, 1.0, 1e-3),
+    (3, 2, 128, 0.25, 1.0, 8.0, 2000.0), (40, 60, 128, 0.25, 2.0, 8.0, 2000.0), (100, 500, 64, 0.25, 8.0, 8.0, 2000.0), (300, 1500, 128, 0.25, 8.0, 8.0, 2000.0), (90, 200, 16, 0.5, 2.0, 30.0, 3000.0),
+])
+def test_gradients_of_every_size(dt, lq, lk, d, fq, fk, fv, fd):
+    """Small gradients on long states (weights and weight gradients among float16's subnormal numbers) and large ones on few (weight gradients beyond its largest, 65 504, though dq and dk fit)."""
+    g = torch.Generator("cuda").manual_seed(lk)
+    rn = lambda n, h, f: (f * torch.randn(1, n, h, d, device="cuda", generator=g)).to(dt)        # noqa: E731
+    q, k, v, do = rn(lq, 2, fq), rn(lk, 1, fk), rn(lk, 1, fv), rn(lq, 2, fd)
+    got = run(q, k, v, None, None, do)
+    qd, kd, vd, dd = (t.double().transpose(1, 2) for t in (q, k, v, do))
+    s = qd @ kd.transpose(2, 3).contiguous() / math.sqrt(d)
+    p = torch.softmax(s, -1)
+    dp = dd @ vd.transpose(2, 3).contiguous()
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True)) / math.sqrt(d)
+    want = {"dq": (ds @ kd).transpose(1, 2), "dk": (ds.transpose(2, 3).contiguous() @ qd).sum(1, keepdim=True).transpose(1, 2), "dv": (p.transpose(2, 3).contiguous() @ dd).sum(1, keepdim=True).transpose(1, 2)}
+    for n in ("dq", "dk", "dv"):
+        if float(want[n].abs().max()) < 6e4 or dt != torch.float16:
+            _by_norm(n, got[n], want[n], U[dt])
