@@ -578,7 +578,8 @@ __global__ __launch_bounds__(256) void k_xattn_join(XAttn a) {
 
 // ------------------------------------------------------------------------------------------------ backward: dq (walks over the keys)
 // ONE: all keys lie in one tile.  delta is then sum p (do.v) over it instead of do.out, whose stored out is rounded to 16 bits: with few keys that rounding is as
-// large as the differences do.v - delta (2 keys: dq and dk off by 2.2 times what their own rounding costs, 1.4 with the sum over the tile)
+// large as the differences do.v - delta (2 keys: dq and dk off by 2.2 times what their own rounding costs, 1.4 with the sum over the tile).  The first walk takes it and the second keeps
+// it: there the pieces of a visible key that hold a non-finite value are zeros, and the key's score would be another
 template <typename T, int DP, int QT, bool ONE>
 __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_dq(XAttn a) {
   using M = Mx<T>;
@@ -651,8 +652,8 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_dq(XAttn a) {
 #pragma unroll
     for (int t = 0; t < QT; ++t) dsum[t] = 0.f;
 #pragma unroll 1
-    for (int phase = ONE ? 0 : 1; phase < 2; ++phase) {
-    if (ONE) asm volatile("" ::: "memory");       // or the compiler lifts the tile's reads out of the loop over the phases, and keeps them in scratch memory
+    for (int phase = ONE && !safe() ? 0 : 1; phase < 2; ++phase) {
+    if (ONE && !safe()) asm volatile("" ::: "memory");       // or the compiler lifts the tile's reads out of the loop over the phases, and keeps them in scratch memory
 #pragma unroll STEPS
     for (int n = 0; n < 4; n += M::PT) {
       if (SKIP && k0 + 16 * n >= seen) break;
@@ -672,7 +673,7 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_dq(XAttn a) {
         in_order<TIGHT>();
       }
       __builtin_amdgcn_s_setprio(0);
-      if (ONE && phase == 0) {
+      if (ONE && !safe() && phase == 0) {
 #pragma unroll
         for (int t = 0; t < QT; ++t)
 #pragma unroll
@@ -727,7 +728,7 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_dq(XAttn a) {
       }
       __builtin_amdgcn_s_setprio(0);
     }
-    if (ONE && phase == 0) {
+    if (ONE && !safe() && phase == 0) {
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
         delta[t] = group_sum(dsum[t]);

@@ -404,3 +404,18 @@ def test_gradients_of_every_size(dt, lq, lk, d, fq, fk, fv, fd):
     for n in ("dq", "dk", "dv"):
         if float(want[n].abs().max()) < 6e4 or dt != torch.float16:
             _by_norm(n, got[n], want[n], U[dt])
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("lk", [5, 64, 100])
+def test_a_visible_key_of_weight_zero_with_an_infinite_entry(dt, lk):
+    """Every query sees a key whose score is -inf (its first entry is infinite): its weight is zero, and out, lse and the other keys' dk and dv are those without the key."""
+    q, k, v, _, _, do = make(dt, 1, 40, lk, 2, 1, 32, seed=lk)
+    q[..., 0] = q[..., 0].abs() + 0.1
+    m = torch.ones(1, 1, 40, lk, dtype=torch.bool, device="cuda")
+    m[..., 3] = False
+    ref = reference(q, k, v, m, do=do)
+    k[0, 3, 0, 0] = -float("inf")
+    got = run(q, k, v, None, None, do)
+    for n in ("out", "lse", "dk", "dv"):
+        close(n, got[n], ref[n])
