@@ -57,6 +57,13 @@ void* ptr(const Tensor& t) { return t.data_ptr(); }
 void* ptr(const MaybeTensor& t) { return t.has_value() ? t->data_ptr() : nullptr; }
 bool tracked(const Tensor& t) { return t.requires_grad(); }
 bool tracked(const MaybeTensor& t) { return t.has_value() && t->requires_grad(); }
+// a forward-mode tangent (a dual tensor may have one without requires_grad) would be dropped without a word
+bool dual(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+bool dual(const MaybeTensor& t) { return t.has_value() && dual(*t); }
+template <typename... Ts>
+void no_tangents(const char* what, const Ts&... ts) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(dual(ts) || ...), what, ": no forward-mode derivatives");
+}
 Tensor some(const MaybeTensor& t) { return t.has_value() ? *t : Tensor(); }
 MaybeTensor maybe(const Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); }
 
@@ -194,6 +201,7 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
     const auto s = ctx->get_saved_variables();
     variable_list out(6);
     if (!g[0].defined()) return out;
+    no_tangents("cross_attention", g[0]);
     const Tensor &q = s[0], &k = s[1], &v = s[2];
     const bool create = at::GradMode::is_enabled();
     {
@@ -214,6 +222,7 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
 
 std::tuple<Tensor, MaybeTensor> cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeTensor& mask, const MaybeTensor& lens, std::optional<double> scale,
                                                 bool want_lse) {
+  no_tangents("cross_attention", q, k, v);
   const double s = attention_checked(q, k, v, mask, lens, scale);
   if (at::GradMode::is_enabled() && (tracked(q) || tracked(k) || tracked(v))) {
     auto out = CrossAttention::apply(q, k, v, mask, lens, s);
@@ -290,6 +299,7 @@ struct AddRMSNorm : torch::autograd::Function<AddRMSNorm> {
       if (dh.defined() && nr) out[1] = dh;
       return out;
     }
+    no_tangents("add_rms_norm", dy, dh);
     {
       at::NoGradGuard guard;
       const int64_t E = x.size(-1), rows = rstd.size(0);
@@ -316,6 +326,7 @@ struct AddRMSNorm : torch::autograd::Function<AddRMSNorm> {
 };
 
 std::tuple<Tensor, Tensor> add_rms_norm(const Tensor& x, const MaybeTensor& r, const MaybeTensor& w, double eps) {
+  no_tangents("add_rms_norm", x, r, w);
   norm_checked(x, r, w, eps);
   if (at::GradMode::is_enabled() && (tracked(x) || tracked(r) || tracked(w))) {
     auto o = AddRMSNorm::apply(x, r, w, eps);
@@ -326,6 +337,7 @@ std::tuple<Tensor, Tensor> add_rms_norm(const Tensor& x, const MaybeTensor& r, c
 }
 
 std::tuple<Tensor, Tensor, Tensor> add_rms_norm_fp8(const Tensor& x, const MaybeTensor& r, const MaybeTensor& w, double eps) {
+  no_tangents("add_rms_norm_fp8", x, r, w);
   norm_checked(x, r, w, eps);
   TORCH_CHECK(!(at::GradMode::is_enabled() && (tracked(x) || tracked(r) || tracked(w))), "add_rms_norm_fp8 has no gradient: call it under torch.no_grad()");
   NormOut o = norm_forward(x, r, w, eps, false, true);
@@ -343,6 +355,7 @@ Setting setting(const char* name, const py::object& v, int64_t R, const at::Devi
   Setting s;
   if (THPVariable_Check(v.ptr())) {
     const Tensor& t = THPVariable_Unpack(v.ptr());
+    no_tangents("sample", t);
     TORCH_CHECK_VALUE(t.numel() == R && t.device() == dev && !t.is_complex() && t.scalar_type() != at::kBool, "sample: ", name,
                       " is a number or a tensor of one number for each of the ", R, " rows on the logits' device");
     s.row = t.detach().reshape({R});
@@ -359,6 +372,7 @@ Setting setting(const char* name, const py::object& v, int64_t R, const at::Devi
 
 std::tuple<Tensor, Tensor> sample(const Tensor& logits, const Tensor& uniforms, const py::object& temperature, const py::object& top_k, const py::object& top_p, const py::object& min_p,
                                   const MaybeTensor& mask_) {
+  no_tangents("sample", logits);
   TORCH_CHECK_TYPE(type_code(logits) >= 0, "sample: logits float32, float16 or bfloat16, got ", logits.scalar_type());
   TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) >= 1 && logits.size(-1) <= (1 << 24), "sample: logits [..., V] with V in 1 .. ", 1 << 24, ", got shape ", shape_of(logits));
   const int64_t V = logits.size(-1), R = logits.numel() / V;

@@ -19,6 +19,6 @@ def cross_attention(query, key, value, mask=None, kv_lens=None, scale=None, retu
   In the backward the weights and the scores' gradients are rounded to it before their products too (in float16 times powers of two, so that small ones on long states keep their bits
   and large ones stay finite), and the sum of out * its gradient is taken of the stored out, except in 16 bits on at most 64 keys.
     return_lse: also the logarithm of the sum of exponentials [B, H, Lq] float32 (-inf where nothing is seen; no gradient through it).
-    Differentiable once in query, key and value; no atomics, the same inputs give the same bits."""
+    Differentiable once in query, key and value (backward; forward-mode tangents are refused); no atomics, the same inputs give the same bits."""
     out, lse = (L._native or L.native()).cross_attention(query, key, value, mask, kv_lens, scale, return_lse)
     return (out, lse) if return_lse else out

@@ -151,3 +151,14 @@ def test_policy_samples_from_given_random_numbers(fixture):
         pol(make(), env, uniforms=u[:2], **kw)
     if atsp:                                                                      # every tour is a permutation
         assert torch.equal(a["actions"].sort(1).values, torch.arange(fx["N"], device="cuda").expand(R, -1))
+
+
+def test_a_tangent_on_the_incoming_gradient_is_refused():
+    import torch.autograd.forward_ad as fwAD
+    from rrnco_amd import ops
+    q = torch.randn(1, 3, 2, 16, device="cuda", requires_grad=True)
+    x = torch.randn(3, 16, device="cuda", requires_grad=True)
+    for leaf, out in ((q, ops.cross_attention(q, q, q)), (x, ops.add_rms_norm(x)[0])):
+        with fwAD.dual_level():
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                torch.autograd.grad(out, leaf, fwAD.make_dual(torch.ones_like(out), torch.ones_like(out)))

@@ -142,3 +142,15 @@ def test_norm_and_draw_entries_refuse():
         bad = list(ok)
         bad[i] = v
         assert lib.rr_draw(*bad) == -1, (i, v)
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A tangent on any differentiable input, without requires_grad: the kernels know none, and a result without one would say that it is zero."""
+    import torch.autograd.forward_ad as fwAD
+    x, w = torch.zeros(2, 8), torch.ones(8)
+    with fwAD.dual_level():
+        d = lambda t: fwAD.make_dual(t, torch.ones_like(t))                      # noqa: E731
+        for f in (lambda: ops.cross_attention(d(Q), K, K), lambda: ops.cross_attention(Q, d(K), K), lambda: ops.cross_attention(Q, K, d(K)), lambda: ops.add_rms_norm(d(x)),
+                  lambda: ops.add_rms_norm(x, d(x)), lambda: ops.add_rms_norm(x, None, d(w)), lambda: ops.add_rms_norm_fp8(d(x)), lambda: ops.sample(d(L8), U2), lambda: ops.sample(L8, U2, temperature=d(torch.ones(2)))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                f()
