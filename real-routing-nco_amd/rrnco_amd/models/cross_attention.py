@@ -13,7 +13,8 @@ class CrossAttention(nn.Module):
     """Queries [B, Lq, embed_dim] attend to an encoder's states [B, Lk, kv_dim]: out_proj(attention(Wq x, Wkv states)).
 
     num_kv_heads < num_heads shares each key head among a group of query heads.  `precompute` gives the keys and values of the states once,
-    for the many steps of a decoder; forward takes either."""
+    for the many steps of a decoder; forward takes either.  The attention runs in the type of the keys (under torch.autocast, or with keys and values made
+    in another precision than the queries')."""
 
     def __init__(self, embed_dim: int, num_heads: int, num_kv_heads: int | None = None, kv_dim: int | None = None, bias: bool = False):
         super().__init__()
@@ -37,14 +38,14 @@ class CrossAttention(nn.Module):
         if mask is not None and mask.dim() == 3:
             mask = mask.unsqueeze(1)
         q = self.Wq(x).unflatten(-1, (self.num_heads, self.head_dim))
-        return self.out_proj(cross_attention(q, k, v, mask=mask, kv_lens=kv_lens).flatten(2))
+        return self.out_proj(cross_attention(q.to(k.dtype), k, v, mask=mask, kv_lens=kv_lens).flatten(2).to(q.dtype))
 
 
 class CrossAttentionLayer(nn.Module):
     """Norm before, residual after, the next layer's norm joined with the addition: (y, h) -> attention(y) -> h' = h + attention, y' = RMSNorm(h').
 
     forward takes the normed stream y and the residual stream h (`start` makes both from a first x) and returns the next ones, so that a stack of
-    layers reads and writes the stream once a layer."""
+    layers reads and writes the stream once a layer.  The streams keep their type, also where the attention runs in another (torch.autocast)."""
 
     def __init__(self, embed_dim: int, num_heads: int, num_kv_heads: int | None = None, kv_dim: int | None = None, bias: bool = False, eps: float = 1e-5):
         super().__init__()
@@ -58,4 +59,4 @@ class CrossAttentionLayer(nn.Module):
         return add_rms_norm(x, None, weight, eps)
 
     def forward(self, y, h, states=None, mask=None, kv_lens=None, cache=None):
-        return add_rms_norm(self.attention(y, states, mask, kv_lens, cache), h, self.norm.weight, self.eps)
+        return add_rms_norm(self.attention(y, states, mask, kv_lens, cache).to(h.dtype), h, self.norm.weight, self.eps)

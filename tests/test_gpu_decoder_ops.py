@@ -162,3 +162,43 @@ def test_a_tangent_on_the_incoming_gradient_is_refused():
         with fwAD.dual_level():
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 torch.autograd.grad(out, leaf, fwAD.make_dual(torch.ones_like(out), torch.ones_like(out)))
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+def test_layers_under_autocast(dt):
+    """The usual mixed precision: float32 parameters and residual stream, products and attention in 16 bits.  Against the definition: beside the roundings that TOL counts, each
+    of the three products rounds its two operands, ten half steps u in all, on values of size up to 4: 40 u, TOL times 4 is 64.  The parameters' gradients are
+    those of the float32 layer to within the same on their norm."""
+    x, states, mask, lens = _inputs(torch.float32)
+    layers = [_layer(torch.float32, seed=s) for s in (0, 1)]
+    gy, gh = torch.randn(3, 7, 64, device="cuda"), torch.randn(3, 7, 64, device="cuda")
+
+    def step(cache=None):
+        y, h = layers[0].start(x)
+        for i, m in enumerate(layers):
+            y, h = m(y, h, None if cache else states, mask=mask, kv_lens=lens, cache=cache[i] if cache else None)
+        return y, h, torch.autograd.grad((y, h), [p for m in layers for p in m.parameters()], (gy, gh), allow_unused=True)
+    with torch.autocast("cuda", dtype=dt):
+        y, h, grads = step()
+        with torch.no_grad():
+            early = [m.attention.precompute(states) for m in layers]
+    assert y.dtype == h.dtype == torch.float32 and all(g.dtype == torch.float32 for g in grads)
+    yd, hd = x.double() / torch.sqrt(x.double().square().mean(-1, keepdim=True) + 1e-5), x.double()
+    for m in layers:
+        yd, hd = _plain_layer(m, yd, hd, states, mask, lens)
+    assert float((y.double() - yd).abs().max()) <= TOL[dt] * 4 and float((h.double() - hd).abs().max()) <= TOL[dt] * 4
+    for g, w in zip(grads, step()[2]):
+        assert float((g - w).norm()) <= 64 * U16[dt] * float(w.norm())
+    # keys and values made in one precision, used in the other
+    with torch.no_grad():
+        late = [m.attention.precompute(states) for m in layers]
+        y1, h1 = layers[0](*layers[0].start(x), cache=early[0], mask=mask, kv_lens=lens)
+        with torch.autocast("cuda", dtype=dt):
+            y2, h2 = layers[0](*layers[0].start(x), cache=late[0], mask=mask, kv_lens=lens)
+        yd, hd = _plain_layer(layers[0], x.double() / torch.sqrt(x.double().square().mean(-1, keepdim=True) + 1e-5), x, states, mask, lens)
+    for y, h in ((y1, h1), (y2, h2)):
+        assert y.dtype == h.dtype == torch.float32
+        assert float((y.double() - yd).abs().max()) <= TOL[dt] * 4 and float((h.double() - hd).abs().max()) <= TOL[dt] * 4
+
+
+U16 = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
