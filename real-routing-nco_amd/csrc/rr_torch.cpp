@@ -164,7 +164,7 @@ void attention_call(const Tensor& q_, const Tensor& k_, const Tensor& v_, const 
     io.dv = ptr(dv);
   }
   const long long n = rr_cross_attn_workspace(io.dtype, io.B, io.Lq, io.Lk, io.Hk, io.G, io.D, back);
-  TORCH_CHECK_VALUE(n >= 0, "cross_attention: more rows, keys or heads than 32-bit counts hold");
+  TORCH_CHECK_VALUE(n >= 0, "cross_attention: more than 2^31 - 1 queries of all heads, or an instance of more than 2^29 queries or keys of its key heads");
   if (n > 0) {
     ws = at::empty({(int64_t)n}, q.options().dtype(at::kByte));
     io.workspace = ptr(ws);

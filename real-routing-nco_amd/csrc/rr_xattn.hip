@@ -43,6 +43,7 @@ struct XAttn {
   int lens64, B, Lq, Lk, Hk, G, D;
   float scale;
   int nsplit, tiles_per_split, nblk;     // splits of the walked axis, its tiles a split, workgroups along the kept axis
+  int b0;                                // the launch's first batch entry
   float* part;                           // partial results of the splits
   // backward
   const void* dout;
@@ -280,7 +281,7 @@ __device__ __forceinline__ Blk block_of(const XAttn& a) {
   w.blk = (int)(i % (unsigned)a.nblk); i /= (unsigned)a.nblk;
   w.split = (int)(i % (unsigned)a.nsplit); i /= (unsigned)a.nsplit;
   w.hk = (int)(i % (unsigned)a.Hk);
-  w.b = (int)(i / (unsigned)a.Hk);
+  w.b = a.b0 + (int)(i / (unsigned)a.Hk);
   return w;
 }
 
@@ -1084,40 +1085,52 @@ Plan plan_for(long long kept, long long walked, long long outer, bool narrow) {
   return p;
 }
 
+// a launch holds fewer than 2^32 threads: as many batch entries at a time as that allows (one at the least: sizes_of)
+#define RR_XA_GRID (0x7fffffffLL / 256)
+template <typename F>
+void by_launches(XAttn& a, const Plan& p, F launch) {
+  a.nsplit = p.nsplit; a.tiles_per_split = p.tiles_per_split; a.nblk = p.nblk;
+  const long long each = (long long)a.Hk * p.nsplit * p.nblk, most = RR_XA_GRID / each;
+  for (long long b = 0; b < a.B; b += most) {
+    a.b0 = (int)b;
+    launch(dim3((unsigned)((a.B - b < most ? a.B - b : most) * each)));
+  }
+}
 template <typename T, int DP>
 int fwd_go(XAttn& a, const Plan& p, hipStream_t st) {
-  const dim3 grid((unsigned)((long long)a.B * a.Hk * p.nsplit * p.nblk));
-  if constexpr (sizeof(T) == 2) {
-    if (p.wide == 2) hipLaunchKernelGGL((k_xattn_fwd<T, DP, 2>), grid, dim3(256), 0, st, a);
-  }
-  if (p.wide == 1) hipLaunchKernelGGL((k_xattn_fwd<T, DP, 1>), grid, dim3(256), 0, st, a);
+  by_launches(a, p, [&](dim3 grid) {
+    if constexpr (sizeof(T) == 2) {
+      if (p.wide == 2) hipLaunchKernelGGL((k_xattn_fwd<T, DP, 2>), grid, dim3(256), 0, st, a);
+    }
+    if (p.wide == 1) hipLaunchKernelGGL((k_xattn_fwd<T, DP, 1>), grid, dim3(256), 0, st, a);
+  });
   if (p.nsplit > 1) hipLaunchKernelGGL((k_xattn_join<T, DP>), dim3((unsigned)(((long long)a.B * a.Hk * a.G * a.Lq + 1024 / DP - 1) / (1024 / DP))), dim3(256), 0, st, a);
   return rr_check(hipGetLastError());
 }
 template <typename T, int DP>
 int bwd_go(XAttn& a, const Plan& p, const Plan& pk, hipStream_t st) {
-  const dim3 grid((unsigned)((long long)a.B * a.Hk * p.nsplit * p.nblk));
-  a.nsplit = p.nsplit; a.tiles_per_split = p.tiles_per_split; a.nblk = p.nblk;
-  if constexpr (sizeof(T) == 2) {
-    if (a.Lk <= RR_XA_KT) {
-      if constexpr (DP < 128) {
-        if (p.wide == 2) hipLaunchKernelGGL((k_xattn_dq<T, DP, 2, true>), grid, dim3(256), 0, st, a);
-      }
-      if (p.wide == 1) hipLaunchKernelGGL((k_xattn_dq<T, DP, 1, true>), grid, dim3(256), 0, st, a);
-    } else if (p.wide == 2) hipLaunchKernelGGL((k_xattn_dq<T, DP, 2, false>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_xattn_dq<T, DP, 1, false>), grid, dim3(256), 0, st, a);
-  } else {
-    hipLaunchKernelGGL((k_xattn_dq<T, DP, 1, false>), grid, dim3(256), 0, st, a);
-  }
+  by_launches(a, p, [&](dim3 grid) {
+    if constexpr (sizeof(T) == 2) {
+      if (a.Lk <= RR_XA_KT) {
+        if constexpr (DP < 128) {
+          if (p.wide == 2) hipLaunchKernelGGL((k_xattn_dq<T, DP, 2, true>), grid, dim3(256), 0, st, a);
+        }
+        if (p.wide == 1) hipLaunchKernelGGL((k_xattn_dq<T, DP, 1, true>), grid, dim3(256), 0, st, a);
+      } else if (p.wide == 2) hipLaunchKernelGGL((k_xattn_dq<T, DP, 2, false>), grid, dim3(256), 0, st, a);
+      else hipLaunchKernelGGL((k_xattn_dq<T, DP, 1, false>), grid, dim3(256), 0, st, a);
+    } else {
+      hipLaunchKernelGGL((k_xattn_dq<T, DP, 1, false>), grid, dim3(256), 0, st, a);
+    }
+  });
   const long long nq4 = (long long)a.B * a.Lq * a.Hk * a.G * a.D / 4, nk4 = (long long)a.B * a.Lk * a.Hk * a.D / 4;
   auto blocks = [](long long n) { return dim3((unsigned)(n / 256 + 1 < 4096 ? n / 256 + 1 : 4096)); };
   if (p.nsplit > 1) hipLaunchKernelGGL((k_xattn_add<T>), blocks(nq4), dim3(256), 0, st, a.part, 4 * nq4, p.nsplit, (T*)a.dq, nq4);
-  a.nsplit = pk.nsplit; a.tiles_per_split = pk.tiles_per_split; a.nblk = pk.nblk;
-  const dim3 gk((unsigned)((long long)a.B * a.Hk * pk.nsplit * pk.nblk));
-  if constexpr (sizeof(T) == 2) {
-    if (pk.wide == 2) hipLaunchKernelGGL((k_xattn_dkv<T, DP, 2>), gk, dim3(256), 0, st, a);
-  }
-  if (pk.wide == 1) hipLaunchKernelGGL((k_xattn_dkv<T, DP, 1>), gk, dim3(256), 0, st, a);
+  by_launches(a, pk, [&](dim3 grid) {
+    if constexpr (sizeof(T) == 2) {
+      if (pk.wide == 2) hipLaunchKernelGGL((k_xattn_dkv<T, DP, 2>), grid, dim3(256), 0, st, a);
+    }
+    if (pk.wide == 1) hipLaunchKernelGGL((k_xattn_dkv<T, DP, 1>), grid, dim3(256), 0, st, a);
+  });
   if (pk.nsplit > 1) {
     hipLaunchKernelGGL((k_xattn_add<T>), blocks(nk4), dim3(256), 0, st, a.part, 8 * nk4, pk.nsplit, (T*)a.dk, nk4);
     hipLaunchKernelGGL((k_xattn_add<T>), blocks(nk4), dim3(256), 0, st, a.part + 4 * nk4, 8 * nk4, pk.nsplit, (T*)a.dv, nk4);
@@ -1138,7 +1151,8 @@ Sizes sizes_of(long long B, long long Lq, long long Lk, long long Hk, long long 
   // dq of 128 columns on keys of one tile holds too much for 32 rows a wave without spilling: 120 queries on 60 keys, 2 048 heads, 182 us spilling, 132 with one
   // workgroup a CU, 97 with 16 rows a wave
   s.dq = plan_for(G * Lq, Lk, B * Hk, dtype == RR_F32 || (D > 64 && Lk <= RR_XA_KT));
-  if (B * Hk * s.q.nblk > lim / 256 || B * Hk * s.dq.nblk > lim / 256 || B * Hk * s.k.nblk > lim / 256 || B * Hk * G * Lq > lim) { s.ok = false; return s; }
+  auto fits = [&](const Plan& p) { return Hk * p.nsplit * p.nblk <= RR_XA_GRID; };
+  if (!fits(s.q) || !fits(s.dq) || !fits(s.k) || B * Hk * G * Lq > lim) { s.ok = false; return s; }
   const int DP = head_pad(D);
   s.fwd = s.q.nsplit > 1 ? (size_t)(B * Hk * G * Lq) * s.q.nsplit * (DP + 4) * 4 : 0;
   const size_t b1 = s.dq.nsplit > 1 ? (size_t)s.dq.nsplit * B * Lq * Hk * G * D * 4 : 0, b2 = s.k.nsplit > 1 ? (size_t)s.k.nsplit * 2 * B * Lk * Hk * D * 4 : 0;
@@ -1208,7 +1222,6 @@ extern "C" int rr_cross_attn(const XAttnIO* io, hipStream_t st) {
   const Sizes s = sizes_of(io->B, io->Lq, io->Lk, io->Hk, io->G, io->D, io->dtype);
   XAttn a;
   if (!s.ok || xa_fill(io, a, false) != RR_OK || (s.fwd > 0 && (io->workspace == nullptr || (size_t)io->workspace_bytes < s.fwd || !rr_aligned16(io->workspace)))) return RR_EINVAL;
-  a.nsplit = s.q.nsplit; a.tiles_per_split = s.q.tiles_per_split; a.nblk = s.q.nblk;
 #define RR_CALL(T, DP) fwd_go<T, DP>(a, s.q, st)
   if (io->dtype == RR_F32) { RR_XA_BY_DIM(float, RR_CALL) }
   if (io->dtype == RR_F16) { RR_XA_BY_DIM(rr_f16, RR_CALL) }

@@ -419,3 +419,21 @@ def test_a_visible_key_of_weight_zero_with_an_infinite_entry(dt, lk):
     got = run(q, k, v, None, None, do)
     for n in ("out", "lse", "dk", "dv"):
         close(n, got[n], ref[n])
+
+
+def test_more_instances_than_a_launch_holds():
+    """1 100 000 one-query instances of 8 heads (a launch holds 8 388 607 workgroups): those around the border between two launches and the last are the same as on their own."""
+    B, H, D, Lk = 1_100_000, 8, 8, 2
+    g = torch.Generator("cuda").manual_seed(7)
+    rn = lambda n, h: torch.randn(B, n, h, D, device="cuda", generator=g, dtype=torch.float16)        # noqa: E731
+    q, k, v, do = rn(1, H), rn(Lk, H), rn(Lk, H), rn(1, H)
+    lens = torch.randint(0, Lk + 1, (B,), device="cuda", generator=g, dtype=torch.int32)
+    m = torch.rand(B, H, 1, Lk, device="cuda", generator=g) < 0.8
+    got = run(q, k, v, m, lens, do)
+    border = 8388607 // H
+    for part in (slice(0, 100), slice(border - 100, border + 100), slice(B - 100, B)):
+        alone = run(q[part], k[part], v[part], m[part], lens[part], do[part])
+        assert all(torch.equal(got[n][part], alone[n]) for n in got)
+        ref = reference(q[part], k[part], v[part], m[part], lens[part], do=do[part])
+        for n in ("out", "lse", "dq", "dk", "dv"):
+            close(n, alone[n], ref[n])

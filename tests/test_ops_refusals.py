@@ -154,3 +154,10 @@ def test_forward_mode_derivatives_are_refused():
                   lambda: ops.add_rms_norm(x, d(x)), lambda: ops.add_rms_norm(x, None, d(w)), lambda: ops.add_rms_norm_fp8(d(x)), lambda: ops.sample(d(L8), U2), lambda: ops.sample(L8, U2, temperature=d(torch.ones(2)))):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 f()
+
+
+def test_cross_attention_sizes():
+    """Any number of instances up to 2^31 - 1 queries of all heads; an instance has to fit one launch."""
+    ws = L.lib().rr_cross_attn_workspace
+    assert ws(1, 1_100_000, 1, 20, 8, 1, 16, 0) == 0 == ws(1, 1_100_000, 1, 20, 8, 1, 16, 1)
+    assert ws(1, 2 ** 28, 1, 20, 8, 1, 16, 0) == -1 == ws(1, 1, 1, 2 ** 31 - 70000, 64, 1, 16, 1)
