@@ -2,6 +2,7 @@
 // Every sum, maximum and statistic is held in 32 bits or more; a value is rounded to its type once, when it is stored.
 #pragma once
 #include "rr_common.h"
+#include "../../include/rrnco_hip.h"      // the entry points and structs as callers see them
 
 #define RR_F32 0
 #define RR_F16 1

@@ -30,6 +30,7 @@
 namespace {
 
 #define RR_XA_KT 64            // keys (or rows) of a staged tile
+#define RR_XA_PART(DP) ((DP) + 4)      // floats of a row's partial result: DP sums, the maximum, the sum of weights, two unused (16-byte pieces stay aligned)
 #define RR_LOG2E 1.44269504088896340736f
 #define RR_LN2 0.69314718055994530942f
 
@@ -516,8 +517,8 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_fwd(XAttn a) {
     if (r >= R) continue;
     const RowAt at = row_at(r, a.Lq, a.G);
     const int head = w.hk * a.G + at.g;
-    if (a.nsplit > 1) {                            // partials: [B * Hk * R][nsplit][DP + 2] floats
-      float* p = a.part + (((long long)(w.b * a.Hk + w.hk) * R + r) * a.nsplit + w.split) * (DP + 4);
+    if (a.nsplit > 1) {                            // partials: [B * Hk * R][nsplit][RR_XA_PART] floats
+      float* p = a.part + (((long long)(w.b * a.Hk + w.hk) * R + r) * a.nsplit + w.split) * RR_XA_PART(DP);
 #pragma unroll
       for (int d = 0; d < Dm::DT; ++d) *reinterpret_cast<f32x4*>(p + 16 * d + 4 * g) = o[t][d];
       if (g == 0) { p[DP] = m[t]; p[DP + 1] = lt; }
@@ -549,15 +550,15 @@ __global__ __launch_bounds__(256) void k_xattn_join(XAttn a) {
   const long long row = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
   const int R = a.G * a.Lq;
   if (row >= (long long)a.B * a.Hk * R) return;
-  const float* p = a.part + row * a.nsplit * (DP + 4);
+  const float* p = a.part + row * a.nsplit * RR_XA_PART(DP);
   float m = -INFINITY;
-  for (int i = 0; i < a.nsplit; ++i) m = fmaxf(m, p[i * (DP + 4) + DP]);
+  for (int i = 0; i < a.nsplit; ++i) m = fmaxf(m, p[i * RR_XA_PART(DP) + DP]);
   const float mu = finite_or_zero(m);
   f32x4 acc = rr_zero4();
   float l = 0.f;
 #pragma unroll 4
   for (int i = 0; i < a.nsplit; ++i) {
-    const float* pi = p + i * (DP + 4);
+    const float* pi = p + i * RR_XA_PART(DP);
     const float mi = pi[DP], li = pi[DP + 1], f = __builtin_amdgcn_exp2f(mi - mu);
     const f32x4 v = *reinterpret_cast<const f32x4*>(pi + c);
     l = fmaf(li, f, l);
@@ -1154,7 +1155,7 @@ Sizes sizes_of(long long B, long long Lq, long long Lk, long long Hk, long long 
   auto fits = [&](const Plan& p) { return Hk * p.nsplit * p.nblk <= RR_XA_GRID; };
   if (!fits(s.q) || !fits(s.dq) || !fits(s.k) || B * Hk * G * Lq > lim) { s.ok = false; return s; }
   const int DP = head_pad(D);
-  s.fwd = s.q.nsplit > 1 ? (size_t)(B * Hk * G * Lq) * s.q.nsplit * (DP + 4) * 4 : 0;
+  s.fwd = s.q.nsplit > 1 ? (size_t)(B * Hk * G * Lq) * s.q.nsplit * RR_XA_PART(DP) * 4 : 0;
   const size_t b1 = s.dq.nsplit > 1 ? (size_t)s.dq.nsplit * B * Lq * Hk * G * D * 4 : 0, b2 = s.k.nsplit > 1 ? (size_t)s.k.nsplit * 2 * B * Lk * Hk * D * 4 : 0;
   s.bwd = b1 > b2 ? b1 : b2;
   return s;
@@ -1166,22 +1167,6 @@ bool well_placed(const void* p, long long sb, long long sl, long long sh, int si
 }
 
 }  // namespace
-
-typedef struct {
-  const void *q, *k, *v;
-  void* out;
-  float* lse;
-  const uint8_t* mask;
-  const void* kv_lens;
-  const void* dout;
-  float* delta;
-  void *dq, *dk, *dv;
-  void* workspace;
-  long long q_stride[3], k_stride[3], v_stride[3], mask_stride[3], dout_stride[3];
-  long long workspace_bytes;
-  int lens_int64, dtype, B, Lq, Lk, Hk, G, D;
-  float scale;
-} XAttnIO;
 
 static int xa_fill(const XAttnIO* io, XAttn& a, bool bwd) {
   const int size = io->dtype == RR_F32 ? 4 : 2;

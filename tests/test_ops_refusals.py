@@ -161,3 +161,11 @@ def test_cross_attention_sizes():
     ws = L.lib().rr_cross_attn_workspace
     assert ws(1, 1_100_000, 1, 20, 8, 1, 16, 0) == 0 == ws(1, 1_100_000, 1, 20, 8, 1, 16, 1)
     assert ws(1, 2 ** 28, 1, 20, 8, 1, 16, 0) == -1 == ws(1, 1, 1, 2 ** 31 - 70000, 64, 1, 16, 1)
+
+
+def test_the_attention_struct_has_one_definition():
+    """The kernels and the torch side read the same declaration: a second copy could differ and still link."""
+    import pathlib
+    root = pathlib.Path(L.__file__).resolve().parents[2]
+    files = [*(root / "include").glob("*.h"), *(root / "real-routing-nco_amd" / "csrc").glob("*.[hc]*")]
+    assert [f.name for f in files if "} XAttnIO;" in f.read_text()] == ["rrnco_hip.h"] and len(files) > 10
