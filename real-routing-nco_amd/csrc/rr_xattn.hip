@@ -254,6 +254,8 @@ __device__ __forceinline__ uint32_t flag4(const uint32_t* flag, int row) {
 __device__ __forceinline__ float group_max(float v) { v = fmaxf(v, __shfl_xor(v, 16)); return fmaxf(v, __shfl_xor(v, 32)); }
 __device__ __forceinline__ float group_sum(float v) { v += __shfl_xor(v, 16); return v + __shfl_xor(v, 32); }
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
+// a row's log-sum-exp in powers of two; +inf where it has no weight at all: all its weights are then exp2(score - inf) = 0
+__device__ __forceinline__ float lse2_of(float lse) { return lse == -INFINITY ? INFINITY : lse * RR_LOG2E; }
 __device__ __forceinline__ bool is_bad(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
 
 // the wave's QT x 16 rows as B operands (lane: row lane % 16, 16 bytes at piece lane / 16 of every contraction step)
@@ -620,7 +622,7 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_dq(XAttn a) {
     const int head = w.hk * a.G + at.g;
     mrow[t] = a.mask + w.b * a.mb + head * a.mh + at.s * a.ml;
     const long long li = ((long long)w.b * H + head) * a.Lq + at.s;
-    lse2[t] = busy && r < R ? a.lse[li] * RR_LOG2E : 0.f;
+    lse2[t] = busy && r < R ? lse2_of(a.lse[li]) : 0.f;
     const T* op = (const T*)a.out + (((long long)w.b * a.Lq + at.s) * H + head) * a.D;
     float d = 0.f;
 #pragma unroll
@@ -857,7 +859,7 @@ __global__ __launch_bounds__(256, (DP == 128 ? 1 : 2)) void k_xattn_dkv(XAttn a)
     pg.load(gp + h * a.gh + s0 * a.gl, a.gl, rows, a.D);
     if (threadIdx.x < RR_XA_KT) {
       const long long li = ((long long)w.b * H + head) * a.Lq + s0 + ((int)threadIdx.x < rows ? (int)threadIdx.x : rows - 1);
-      nl = (int)threadIdx.x < rows ? a.lse[li] * RR_LOG2E - (Scaled<T>::v ? RR_XA_P_BITS : 0) : INFINITY;
+      nl = (int)threadIdx.x < rows ? lse2_of(a.lse[li]) - (Scaled<T>::v ? RR_XA_P_BITS : 0) : INFINITY;
       nd = (int)threadIdx.x < rows ? a.delta[li] : 0.f;
     }
     if (a.mask != nullptr) {

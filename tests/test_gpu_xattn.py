@@ -437,3 +437,20 @@ def test_more_instances_than_a_launch_holds():
         ref = reference(q[part], k[part], v[part], m[part], lens[part], do=do[part])
         for n in ("out", "lse", "dq", "dk", "dv"):
             close(n, alone[n], ref[n])
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("lk", [5, 100])
+def test_a_query_whose_scores_are_all_minus_infinity(dt, lk):
+    """One query sees nothing but a key whose score is -inf: zeros, lse -inf and no part in any gradient, as one that sees no key."""
+    q, k, v, _, _, do = make(dt, 1, 40, lk, 2, 1, 32, seed=lk)
+    q[..., 0] = q[..., 0].abs() + 0.1
+    m = torch.ones(1, 1, 40, lk, dtype=torch.bool, device="cuda")
+    m[:, :, 7] = False
+    without = m.clone()
+    without[..., 3], m[:, :, 7, 3] = False, True
+    ref = reference(q, k, v, without, do=do)
+    k[0, 3, 0, 0] = -float("inf")
+    got = run(q, k, v, m, None, do)
+    for n in ("out", "lse", "dk", "dv"):
+        close(n, got[n], ref[n])
