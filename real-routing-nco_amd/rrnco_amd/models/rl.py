@@ -56,6 +56,8 @@ class RRNet:
         `replay_log_likelihood` (must agree with the rollout's) and `grad_norm`."""
         if self.env_name not in ("atsp", "rcvrp", "rcvrptw"):
             raise NotImplementedError(f"training_step for env '{self.env_name}'")
+        if policy_kw.get("min_p", 0.0) > 0.0:             # (with either replay and in either mode of the policy)
+            raise NotImplementedError("min_p in a training step: the replayed log-likelihood has no filters")
         from .encoder import ATSPInitEmbedding, draw_sample_indices
         td = self.env.reset(batch)
         if td.get("sample_idx", None) is None:            # the rollout and the replay must see the same neighbour sample

@@ -169,3 +169,14 @@ def test_the_attention_struct_has_one_definition():
     root = pathlib.Path(L.__file__).resolve().parents[2]
     files = [*(root / "include").glob("*.h"), *(root / "real-routing-nco_amd" / "csrc").glob("*.[hc]*")]
     assert [f.name for f in files if "} XAttnIO;" in f.read_text()] == ["rrnco_hip.h"] and len(files) > 10
+
+
+@pytest.mark.parametrize("replay", ["hip", "torch"])
+def test_min_p_in_a_training_step_is_refused(replay):
+    """Before anything runs, whichever replay computes the gradients: neither knows the filter."""
+    from rrnco_amd.models.rl import RRNet
+    m = RRNet.__new__(RRNet)
+    m.env = m.policy = None
+    m.env_name = "atsp"
+    with pytest.raises(NotImplementedError, match="min_p"):
+        m.training_step(None, replay=replay, min_p=0.05)
