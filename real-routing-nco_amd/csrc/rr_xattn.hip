@@ -12,8 +12,8 @@
 // ds_read_b64_tr_b16 for 16-bit types, four plain reads for float32).  The running maximum and sum are in 32 bits; P is rounded to
 // the inputs' type for the second product, half a step of each weight; in float16 a weight keeps that down to 2^-25 of the row's largest (Range below).
 // float32 runs on v_mfma_f32_16x16x4 (exact products), 16-bit types on v_mfma_f32_16x16x32.
-// The backward recomputes P from lse; dq walks over keys, (dk, dv) over rows: no atomics, the same result every time.  P and ds are rounded to the inputs' type for its second
-// products too; in float16 ds is taken times a power of two, of a row's own in dq and of a key's own in dk, and P times 2^14 in dv (Scaled below).
+// The backward recomputes P from lse; dq walks over keys, (dk, dv) over rows: no atomics, the same result every time.  P is rounded to the inputs' type for dv too; ds, which has both signs,
+// goes into its products in two 16-bit pieces (rest_of below).  In float16 ds is taken times a power of two, of a row's own in dq and of a key's own in dk, and P times 2^14 in dv (Scaled below).
 // Products run at a raised wave priority in the forward and dq: with two waves a SIMD one computes weights while the other holds the matrix pipe
 // (forward 2 000 x 4 099, 64 heads of 128: 372 -> 360 us, dq of 1 500 x 2 049, 32 heads of 64: 69.4 -> 68.2; dk, dv: nothing).
 // Bounds and figures (float16 / bfloat16 unless said): forward of 2 000 x 4 099, 64 heads of 128, 740 TFLOP/s, matrix pipe 29% and vector pipe 34% busy, the rest
@@ -119,6 +119,19 @@ template <> struct Mx<rr_bf16> {
 };
 
 template <typename T> using FragOf = typename Mx<T>::Frag;
+// What rounding to a 16-bit type took from two score tiles: the second piece of ds.  In one piece dq of narrow heads and of few queries was 1.5 to 1.7 times as far from 64 bits as its own
+// rounding alone, dk 1.4 to 1.6; in two 1.0 to 1.3.  P, never negative, costs dv and the output a factor of 1.4 in one piece and keeps it.  Time of a second piece, bfloat16: 2 x 1 500 on
+// 2 049, 16 / 4 heads of 64, every key seen, dq 69 -> 90 us, (dk, dv) 122 -> 139; one such of 128, 2 048 keys, 80 -> 93 and 119 -> 131; 64 x 101 on 103, 8 heads of 16, 9.1 -> 9.6 and 8.2 -> 8.8
+template <typename T>
+__device__ __forceinline__ FragOf<T> rest_of(const f32x4* x, const FragOf<T>& hi) {
+  f32x4 r[2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    r[0][i] = x[0][i] - (float)hi[i];
+    r[1][i] = x[1][i] - (float)hi[4 + i];
+  }
+  return Mx<T>::pack(r);
+}
 
 template <typename T, int DP> struct Dims {
   static constexpr int KD = DP < Mx<T>::KC ? Mx<T>::KC : DP;      // columns of a staged row (zeros behind the head dim)
@@ -690,7 +703,7 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_dq(XAttn a) {
           }
         continue;
       }
-      typename M::Frag pf[QT];
+      typename M::Frag pf[QT], pr[QT];
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
         const float ud = Scaled<T>::v ? delta[t] * up[t] : delta[t];
@@ -721,13 +734,17 @@ __global__ __launch_bounds__(256, (Waves<T, DP>::N)) void k_xattn_dq(XAttn a) {
           }
         }
         pf[t] = M::pack(s[t]);
+        if constexpr (sizeof(T) == 2) pr[t] = rest_of<T>(s[t], pf[t]);
       }
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int d = 0; d < Dm::DT; ++d) {
         const typename M::Frag f = M::tr(tk, Dm::PX, 16 * n, 16 * d, lane);
 #pragma unroll
-        for (int t = 0; t < QT; ++t) o[t][d] = M::mma(f, pf[t], o[t][d]);
+        for (int t = 0; t < QT; ++t) {
+          o[t][d] = M::mma(f, pf[t], o[t][d]);
+          if constexpr (sizeof(T) == 2) o[t][d] = M::mma(f, pr[t], o[t][d]);
+        }
         if ((d & 3) == 3) in_order<TIGHT>();
       }
       __builtin_amdgcn_s_setprio(0);
@@ -933,7 +950,7 @@ __global__ __launch_bounds__(256, (DP == 128 ? 1 : 2)) void k_xattn_dkv(XAttn a)
         ls[u] = *reinterpret_cast<const f32x4*>(&sl[at][16 * (n + u) + 4 * g]);
         de[u] = *reinterpret_cast<const f32x4*>(&sd[at][16 * (n + u) + 4 * g]);
       }
-      typename M::Frag pf[KW], df[KW];
+      typename M::Frag pf[KW], df[KW], dr[KW];
 #pragma unroll
       for (int t = 0; t < KW; ++t) {
 #pragma unroll
@@ -973,13 +990,18 @@ __global__ __launch_bounds__(256, (DP == 128 ? 1 : 2)) void k_xattn_dkv(XAttn a)
           }
         }
         df[t] = M::pack(dp[t]);
+        if constexpr (sizeof(T) == 2) dr[t] = rest_of<T>(dp[t], df[t]);
       }
 #pragma unroll
       for (int d = 0; d < Dm::DT; ++d) {
         const typename M::Frag fg = M::tr(tg, Dm::PX, 16 * n, 16 * d, lane);
         const typename M::Frag fq = M::tr(tq, Dm::PX, 16 * n, 16 * d, lane);
 #pragma unroll
-        for (int t = 0; t < KW; ++t) { ov[t][d] = M::mma(fg, pf[t], ov[t][d]); ok[t][d] = M::mma(fq, df[t], ok[t][d]); }
+        for (int t = 0; t < KW; ++t) {
+          ov[t][d] = M::mma(fg, pf[t], ov[t][d]);
+          ok[t][d] = M::mma(fq, df[t], ok[t][d]);
+          if constexpr (sizeof(T) == 2) ok[t][d] = M::mma(fq, dr[t], ok[t][d]);
+        }
         if ((d & 1) == 1) in_order<TIGHT>();
       }
     }

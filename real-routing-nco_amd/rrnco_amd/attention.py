@@ -16,8 +16,8 @@ def cross_attention(query, key, value, mask=None, kv_lens=None, scale=None, retu
     scale: > 0, D ** -0.5 if None.
     A query that sees no key gives zeros and takes part in no gradient.  A key that a query may not see never shows in its result, whatever it holds
     (non-finite values too); scores, softmax and sums are in float32, the weights are rounded to the inputs' type before the product with the values.
-  In the backward the weights and the scores' gradients are rounded to it before their products too (in float16 times powers of two, so that small ones on long states keep their bits
-  and large ones stay finite), and the sum of out * its gradient is taken of the stored out, except in 16 bits on at most 64 keys.
+  In the backward the weights are rounded to it before their product too, the scores' gradients to two values of it (in float16 all times powers of two, so that small ones on long states
+  keep their bits and large ones stay finite), and the sum of out * its gradient is taken of the stored out, except in 16 bits on at most 64 keys.
     return_lse: also the logarithm of the sum of exponentials [B, H, Lq] float32 (-inf where nothing is seen; no gradient through it).
     Differentiable once in query, key and value (backward; forward-mode tangents are refused); no atomics, the same inputs give the same bits."""
     out, lse = (L._native or L.native()).cross_attention(query, key, value, mask, kv_lens, scale, return_lse)

@@ -454,3 +454,32 @@ def test_a_query_whose_scores_are_all_minus_infinity(dt, lk):
     got = run(q, k, v, m, None, do)
     for n in ("out", "lse", "dk", "dv"):
         close(n, got[n], ref[n])
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("c", [(19, 304, 1716, 4, 4, 8, "none"), (2, 30, 213, 8, 8, 8, "none"), (12, 1, 100, 6, 2, 16, "none"), (13, 361, 348, 8, 8, 16, "rows"), (48, 3, 268, 16, 8, 40, "rows"),
+                               (24, 52, 244, 16, 2, 64, "rows"), (37, 51, 1150, 4, 4, 96, "rows"), (2, 120, 60, 8, 8, 128, "none")], ids=lambda c: "-".join(map(str, c)))
+def test_gradients_of_scores_lose_nothing_to_16_bits(dt, c):
+    """dq and dk of 16-bit inputs are as far from 64 bits as their own rounding, and what delta costs: it is taken of the stored out, off by the roundings of the weights and of out.
+    Both at the size that they have on average: a rounding is uniform in half a step, of a value anywhere in its binade, so its mean square is u^2 / 6 of the value's (the mean of 1 / m^2
+    over m in 1 .. 2 is 1/2, a third of half of u^2).  With the gradients of the scores in one 16-bit piece a third such term, as large as the result's own, came in.
+    Errors add in squares; 1.2 times the sum of the two covers sums of a few values (the mean of their mantissas)."""
+    B, Lq, Lk, H, Hk, D, mask = c
+    q, k, v, m, lens, do = make(dt, B, Lq, Lk, H, Hk, D, mask, seed=Lk)
+    got = run(q, k, v, m, lens, do)
+    G, scale = H // Hk, D ** -0.5
+    qd, kd, vd, dd = (t.double().transpose(1, 2) for t in (q, k, v, do))
+    kd, vd = kd.repeat_interleave(G, 1), vd.repeat_interleave(G, 1)
+    see = _visible(B, H, Lq, Lk, m, lens, "cuda")
+    p = torch.nan_to_num(torch.softmax((qd @ kd.transpose(2, 3).contiguous() * scale).masked_fill(~see, -math.inf), -1))
+    dp, o = dd @ vd.transpose(2, 3).contiguous(), p @ vd
+    ds = p * (dp - (dd * o).sum(-1, keepdim=True)) * scale
+    back = lambda x: x.unflatten(1, (Hk, G)).sum(2)                               # noqa: E731
+    want = {"dq": ds @ kd, "dk": back(ds.transpose(2, 3).contiguous() @ qd)}
+    var = U[dt] ** 2 / 6
+    ddelta = var * ((dd * o).square().sum(-1, keepdim=True) + (p * dp).square().sum(-1, keepdim=True))              # delta's mean square error
+    of_delta = {"dq": ddelta * (p @ kd * scale).square().sum(-1, keepdim=True), "dk": back(p.square().transpose(2, 3).contiguous() @ (ddelta * (qd * scale).square()))}
+    for n in want:
+        err = float((got[n].double().transpose(1, 2) - want[n]).norm())
+        lim = 1.2 * (var * float(want[n].square().sum()) + float(of_delta[n].sum())) ** 0.5
+        assert err <= lim, f"{n}: {err / lim:.3g} x the tolerance, {err / float(want[n].norm()) / U[dt]:.3g} u"
