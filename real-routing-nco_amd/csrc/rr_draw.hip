@@ -17,8 +17,9 @@
 // distance from the maximum, then only the keys of the bin that holds the border are looked at.  Masses there are whole numbers of steps
 // of 2^-45, so that atomics may add them in any order; sums over more than 2^18 keys may pass 64 bits and are kept in 128.  Longer rows: a workgroup for every 16 384 keys, five
 // launches (below).
-// Bound by the 64-bit arithmetic (some 20 instructions a weight), not by the one read of the logits: 51 200 x 100 float32 with a mask 17 us (1.5 TB/s), 4 096 x 1 001 with all
-// filters 22 us, 64 x 131 072 bf16 with settings of each row 69 us in five launches (6 + 16 + 5 + 13 + 28).
+// Bound by vector instructions, not by the one read of the logits: 51 200 x 100 float32 with a mask 17 us (1.5 TB/s), 762 of them a wave of four rows, 95 for each key that a lane holds, of
+// which its 64-bit weight is some 20: the rest are keys and masks, comparisons and selects in 64 bits, the scans and the logarithm.  4 096 x 1 001 with all filters 23 us, the
+// bisections' dependent steps; 64 x 131 072 bf16 with settings of each row 79 - 88 us in five launches (6 + 16 + 7 + 13 + 28).
 #include <type_traits>
 
 #include "rr_types.h"

@@ -16,9 +16,10 @@
 // goes into its products in two 16-bit pieces (rest_of below).  In float16 ds is taken times a power of two, of a row's own in dq and of a key's own in dk, and P times 2^14 in dv (Scaled below).
 // Products run at a raised wave priority in the forward and dq: with two waves a SIMD one computes weights while the other holds the matrix pipe
 // (forward 2 000 x 4 099, 64 heads of 128: 372 -> 360 us, dq of 1 500 x 2 049, 32 heads of 64: 69.4 -> 68.2; dk, dv: nothing).
-// Bounds and figures (float16 / bfloat16 unless said): forward of 2 000 x 4 099, 64 heads of 128, 740 TFLOP/s, matrix pipe 29% and vector pipe 34% busy, the rest
-// waits that two waves a SIMD (253 registers) do not hide.  One token on 48 x 8 192 states, 4 key heads of 128: 132 us, 4.6 TB/s, the copy's rate.  float32 with heads
-// of 16 (512 x 100 on 100): 66 us, bound by issue (products 32%, vector instructions 48%).  Backward of 2 x 1 500 on 2 049, 16 / 4 heads of 64: dq 68 us, (dk, dv) 79 us.
+// Bounds and figures (float16 / bfloat16 unless said): forward of 2 000 x 4 099, 64 heads of 128, 730 TFLOP/s, matrix pipe 30% and vector pipe 33% busy, the rest
+// waits that two waves a SIMD (253 registers) do not hide.  One token on 48 x up to 8 192 states, 4 key heads of 128: 132 us, 4.6 TB/s where a large copy reaches 4.92, and 10 for the
+// join of the splits: 145 a call.  float32 with heads of 16 (512 x 100 on 100): 66 us, bound by issue (products 33%, vector instructions 49%), half of the latter each wave's start and
+// end.  Backward of 2 x 1 500 on up to 2 049, 16 / 4 heads of 64: dq 87 us, (dk, dv) 92 us (matrix pipe 20 and 24%, vector pipe 33 and 37% busy).
 // Few rows: the key axis is split over workgroups and joined by a second launch.
 // Non-finite values where nothing may look (a masked key whose value is NaN): 0 * NaN would spoil the products, so a workgroup
 // whose accumulators end non-finite walks its tiles once more with the non-finite 16-byte pieces replaced by zeros and their
@@ -317,8 +318,8 @@ template <> struct Range<rr_f16> { static constexpr float UP = 11.f, SLACK = 4.f
 // second products take ds 2^n, n of a row's (a key's) own, undone in 32 bits at the end.  n begins at 60 and falls, the sums with it, whenever a value would pass 2^15: to where the largest
 // of the step stands at 2^9 .. 2^10, so that it rarely falls again.  Then the rounding of a small ds is off by 2^-34 of the row's (key's) largest at the most.  P <= 1 is taken times
 // 2^14: off by 2^-39 at the most.  It costs a comparison and a branch for
-// every 32 keys (rows) of a row (key) and dk a product for each weight: 2 x 1 500 on 2 049, 16 / 4 heads of 64, every key seen, dq 69 -> 77 us, (dk, dv) 122 -> 142, 120 on 60, 2 048 heads of 64:
-// 52 -> 57 and 35 -> 38; bfloat16, which has float32's exponents, does without
+// every 32 keys (rows) of a row (key) and dk a product for each weight; bfloat16, which has float32's exponents, does without.  float16 against bfloat16: 2 x 1 500 on 2 049, 16 / 4 heads of
+// 64, every key seen, dq 96 and 89 us, (dk, dv) 158 and 139; 120 on 60, 2 048 heads of 64, 58 and 53, 40 and 37
 #define RR_XA_UP 0x1p60f
 #define RR_XA_P_BITS 14
 template <typename T> struct Scaled { static constexpr bool v = std::is_same_v<T, rr_f16>; };

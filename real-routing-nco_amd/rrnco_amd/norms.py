@@ -10,6 +10,7 @@ def add_rms_norm(x, residual=None, weight=None, eps: float = 1e-5):
 
     x, residual [..., E], E up to 16 384, float32 / float16 / bfloat16 with any strides (a last axis that is not contiguous is copied);
     weight [E] in x's type or float32, None for ones.  The norm is taken of the sum before it is rounded to h.  residual=None: h is x.
+    eps >= 0; with eps = 0 a row whose root mean square is 2^-128 or less has no reciprocal in float32, and gives inf or NaN, as a row of zeros does.
     Differentiable once in x, residual and weight (backward; forward-mode tangents are refused); the sums of the backward have a fixed order."""
     return (L._native or L.native()).add_rms_norm(x, residual, weight, eps)
 
